@@ -10,6 +10,7 @@
 #include <vector>
 
 #include "common.cuh"
+#include "kv_internal.h"
 #include "moe_internal.h"
 
 namespace moe {
@@ -73,6 +74,36 @@ bool make_tmap_2d(CUtensorMap* map, const void* base, bool int8, uint64_t inner,
     snprintf(buf, sizeof(buf), "cuTensorMapEncodeTiled failed (%d): inner=%llu rows=%llu", (int)r,
              (unsigned long long)inner, (unsigned long long)rows);
     *err = buf;
+    return false;
+  }
+  return true;
+}
+
+// One layer's pages of a K or V pool as (dim, row, head, page, layer): a box is 64 dims
+// (one 128-byte swizzle atom) by the rows of a page, at most a tile's 128.
+bool make_tmap_pool(CUtensorMap* map, const void* base, bool bf16, const KvView& c,
+                    const int64_t (&strides)[4], std::string* err) {
+  auto fn = get_encode_fn();
+  if (!fn) {
+    *err = "cuTensorMapEncodeTiled unavailable from the driver";
+    return false;
+  }
+  const int sizes[4] = {c.page, c.heads, c.pages, c.layers};
+  cuuint64_t dims[5] = {static_cast<cuuint64_t>(c.hd)};
+  cuuint64_t str[4];
+  for (int i = 0; i < 4; ++i) {
+    dims[i + 1] = static_cast<cuuint64_t>(sizes[i]);
+    // the stride of a dimension of one entry is never used, but has to encode
+    str[i] = sizes[i] > 1 ? static_cast<cuuint64_t>(strides[3 - i]) : static_cast<cuuint64_t>(c.hd) * 2;
+  }
+  cuuint32_t box[5] = {64, static_cast<cuuint32_t>(c.page < 128 ? c.page : 128), 1, 1, 1};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  const CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
+                        const_cast<void*>(base), dims, str, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    *err = "cuTensorMapEncodeTiled failed (" + std::to_string(static_cast<int>(r)) + ") for a K/V pool";
     return false;
   }
   return true;

@@ -28,6 +28,10 @@ enum DevErr : int {
   DEV_RANGE = 8,             // an activation does not fit an f16 operand or output
   DEV_TILE_OVERFLOW = 9,     // a tile list needs more entries than the workspace holds
   DEV_TIMEOUT_PEER = 10,     // a peer GPU's epoch flag did not arrive in time
+  DEV_BAD_SEQ = 11,          // paged cache: a sequence index out of range or given twice
+  DEV_BAD_LENGTH = 12,       // paged cache: a length that does not fit
+  DEV_BAD_PAGE = 13,         // paged cache: a page out of range, missing or given twice
+  DEV_NO_PAGES = 14,         // paged cache: too few free pages
 };
 
 // f16 conversion of v stays finite (|v| rounds to at most 65504); false for NaN too.

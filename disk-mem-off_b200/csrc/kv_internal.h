@@ -1,0 +1,102 @@
+// Paged K/V cache: the view that its kernels take, and the launchers shared by
+// kv_pages.cu (pages, append) and kv_attend.cu (attention over the cache).
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common.cuh"
+#include "moe_internal.h"
+
+namespace moe {
+
+// Everything a cache kernel needs, by value.  Strides are in bytes: layer, page,
+// head, row (a row is one token's head_dim values, contiguous).
+struct KvView {
+  char* k;
+  char* v;
+  int64_t ks[4], vs[4];
+  int layers, pages, heads, page, page_shift, hd;
+  int* table;  // [nseq][max_blocks]
+  int nseq, max_blocks;
+  int* len;    // [nseq]
+  int* refs;   // [pages]
+  // scratch (see KvScratch)
+  int* err;
+  int* count;  // pages to copy, written by the kernel that plans a copy
+  int* src;    // [cap] pages to copy from
+  int* dst;    // [cap] pages to copy to
+  int* rows;   // [cap] rows of each page to copy
+  int* list;   // [pages] free pages / new page of each page
+  int* off;    // [nseq] first free page of each entry
+};
+
+// The caller's scratch, zeroed once: 16 words (error word, copy count), then the
+// arrays above.
+inline size_t kv_scratch_words(int pages, int nseq) {
+  const size_t cap = static_cast<size_t>(pages > nseq ? pages : nseq);
+  return 16 + 3 * cap + static_cast<size_t>(pages) + nseq;
+}
+
+// Most sequences of a cache: a bitmap of them is checked in shared memory.
+constexpr int kKvMaxSeqs = 65536;
+
+// One batch of new rows: row r of entry e is q_start[e] <= r < q_start[e + 1].
+struct KvBatch {
+  const int* seqs;     // [n]
+  const int* q_start;  // [n + 1]
+  int n;
+  int rows;  // rows of the tensors; those from q_start[n] on are left alone
+};
+
+#ifdef __CUDACC__
+// The entry of row r: the last e with q_start[e] <= r, by a warp (32 probes a round).
+MOE_DEV int entry_of_row(const int* __restrict__ q_start, int n, int r) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = n;  // answer in [lo, hi)
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32;
+    const int at = lo + lane * step;
+    const bool le = at < hi && q_start[at] <= r;
+    const uint32_t m = __ballot_sync(0xffffffffu, le);
+    if (!m) return -1;
+    const int j = 31 - __clz(m);
+    hi = min(hi, lo + (j + 1) * step);
+    lo += j * step;
+  }
+  return lo;
+}
+#endif
+
+cudaError_t kv_launch_append(const KvView& c, const KvBatch& b, int layer, const void* k,
+                             const void* v, const int64_t (&ks)[2], const int64_t (&vs)[2],
+                             int num_sms, cudaStream_t s);
+
+struct KvAttend {
+  const void* q;
+  void* out;
+  float* lse;         // null: not wanted
+  int64_t qs[2], os[2], ls[2];  // token and head strides in elements
+  int heads;
+  int layer;
+  float scale;
+};
+size_t kv_attend_workspace(const KvView& c, int heads, int rows, int n_seqs, int num_sms);
+cudaError_t kv_launch_attend(const KvView& c, const CUtensorMap& tk, const CUtensorMap& tv,
+                             bool bf16, const KvBatch& b, const KvAttend& a, void* ws,
+                             int num_sms, cudaStream_t s);
+
+bool make_tmap_pool(CUtensorMap* map, const void* base, bool bf16, const KvView& c,
+                    const int64_t (&strides)[4], std::string* err);
+
+}  // namespace moe
+
+// The opaque handle of the C ABI: host memory only.
+struct MoeKvCache {
+  moe::KvView v;
+  CUtensorMap tk, tv;
+  bool bf16;
+  int device;
+  int num_sms;
+};

@@ -22,6 +22,7 @@ MOE_ERR_NOT_BOUND = 6
 MOE_ERR_DEVICE = 7
 MOE_ERR_TIMEOUT = 8
 MOE_ERR_RANGE = 9
+MOE_ERR_NO_PAGES = 10
 
 MOE_STATIC_SCRATCH_BYTES = 32 * 1024 * 1024  # include/moe_sm100.h
 
@@ -29,6 +30,8 @@ MOE_SCORE_SOFTMAX = 0
 MOE_SCORE_SIGMOID = 1
 MOE_WEIGHTS_F16 = 0
 MOE_WEIGHTS_INT8_PC = 1
+MOE_KV_F16 = 0
+MOE_KV_BF16 = 1
 
 
 class MoeConfigC(ctypes.Structure):
@@ -53,6 +56,25 @@ class MoeTensorDescC(ctypes.Structure):
     _fields_ = [
         ("name", c_char_p), ("dtype", c_char_p), ("shape", c_int64 * 2), ("ndim", c_int32),
         ("offset", c_int64), ("nbytes", c_int64),
+    ]
+
+
+class MoeKvConfigC(ctypes.Structure):
+    _fields_ = [
+        ("k", c_void_p), ("v", c_void_p), ("k_strides", c_int64 * 4), ("v_strides", c_int64 * 4),
+        ("block_table", c_void_p), ("lengths", c_void_p), ("refs", c_void_p),
+        ("scratch", c_void_p), ("dtype", c_int32), ("layers", c_int32), ("pages", c_int32),
+        ("kv_heads", c_int32), ("page_size", c_int32), ("head_dim", c_int32),
+        ("sequences", c_int32), ("max_blocks", c_int32), ("device", c_int32),
+    ]
+
+
+class MoeKvAttendArgsC(ctypes.Structure):
+    _fields_ = [
+        ("q", c_void_p), ("out", c_void_p), ("lse", c_void_p), ("q_strides", c_int64 * 2),
+        ("out_strides", c_int64 * 2), ("lse_strides", c_int64 * 2), ("seqs", c_void_p),
+        ("q_start", c_void_p), ("n_seqs", c_int32), ("rows", c_int32), ("heads", c_int32),
+        ("layer", c_int32), ("scale", c_float),
     ]
 
 
@@ -124,6 +146,19 @@ _PROTOTYPES: dict[str, tuple] = {
     "moe_attn_forward": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_uint64,
                                    c_void_p]),
     "moe_attn_status": (c_int32, [c_void_p, c_void_p]),
+    "moe_kv_scratch_bytes": (c_uint64, [POINTER(MoeKvConfigC)]),
+    "moe_kv_create": (c_int32, [POINTER(MoeKvConfigC), POINTER(c_void_p)]),
+    "moe_kv_destroy": (c_int32, [c_void_p]),
+    "moe_kv_reserve": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_void_p]),
+    "moe_kv_fork": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_void_p]),
+    "moe_kv_truncate": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_void_p]),
+    "moe_kv_copy_pages": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_void_p]),
+    "moe_kv_compact": (c_int32, [c_void_p, c_void_p, c_void_p]),
+    "moe_kv_append": (c_int32, [c_void_p, c_int32, c_void_p, c_void_p, POINTER(c_int64),
+                                POINTER(c_int64), c_void_p, c_void_p, c_int32, c_int32, c_void_p]),
+    "moe_kv_attend_workspace_bytes": (c_uint64, [c_void_p, c_int32, c_int32, c_int32]),
+    "moe_kv_attend": (c_int32, [c_void_p, POINTER(MoeKvAttendArgsC), c_void_p, c_uint64, c_void_p]),
+    "moe_kv_status": (c_int32, [c_void_p, c_void_p]),
     "moe_wait_probe": (c_int32, [c_void_p, c_int64, c_void_p]),
     "moe_last_error": (c_char_p, []),
     "moe_version": (c_char_p, []),

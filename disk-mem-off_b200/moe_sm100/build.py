@@ -11,7 +11,8 @@ import sys
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(os.path.dirname(_HERE), "csrc")
-SOURCES = ["api.cu", "router.cu", "gemm_tc.cu", "combine.cu", "pack.cu", "attn.cu", "noalloc.cu", "p2p.cu"]
+SOURCES = ["api.cu", "router.cu", "gemm_tc.cu", "combine.cu", "pack.cu", "attn.cu", "noalloc.cu", "p2p.cu",
+           "kv_pages.cu", "kv_attend.cu"]
 OUT = os.path.join(_HERE, "libmoe_sm100.so")
 
 

@@ -44,7 +44,8 @@ enum {
   MOE_ERR_NOT_BOUND = 6,      /* forward before moe_bind_layer                       */
   MOE_ERR_DEVICE = 7,         /* a kernel reported an error (bad tile / route)       */
   MOE_ERR_TIMEOUT = 8,        /* a bounded device-side wait ran out of time          */
-  MOE_ERR_RANGE = 9           /* weight value not representable in the packed format */
+  MOE_ERR_RANGE = 9,          /* weight value not representable in the packed format */
+  MOE_ERR_NO_PAGES = 10       /* a paged cache's pool has too few free pages         */
 };
 
 /* router scoring */
@@ -350,6 +351,110 @@ int moe_attn_forward(MoeAttn* attn, const float* x_dev, float* out_dev, int32_t 
                      void* workspace, uint64_t workspace_bytes, void* stream);
 /* As moe_status, for the attention kernels' device error word. */
 int moe_attn_status(MoeAttn* attn, void* stream);
+
+/* ------------------------------------------------- paged K/V cache
+ * No counterpart in the reference, which re-runs the whole sequence for every token.
+ * Keys and values of many sequences live in pages of a pool that the caller owns:
+ *   k, v        [layers][pages][kv_heads][page_size][head_dim], f16 or bf16, any
+ *               strides that are multiples of 8 elements with head_dim contiguous
+ *   block_table [sequences][max_blocks] int32: the page of each block of page_size
+ *               tokens of a sequence; -1 past its last block
+ *   lengths     [sequences] int32 tokens
+ *   refs        [pages] int32 sequences that hold the page; 0: free
+ *   scratch     moe_kv_scratch_bytes bytes, zeroed once by the caller
+ * All of it is device memory; the handle holds host memory only and creating one
+ * allocates nothing on the device.  An empty cache is all -1, 0 and 0.
+ *
+ * Index arguments (seqs, counts, q_start, ...) are int32 arrays in device memory, so
+ * that calls can be captured in a graph.  A call on sequences outside [0, sequences),
+ * or on the same sequence twice where that would be written twice, changes nothing;
+ * such errors are found on the device and reported by moe_kv_status.  Calls on one
+ * cache run in stream order: the ones that change it (and attention while it is being
+ * changed) must not overlap on two streams; attention calls may overlap each other. */
+enum { MOE_KV_F16 = 0, MOE_KV_BF16 = 1 };
+
+typedef struct MoeKvConfig {
+  void* k;
+  void* v;
+  int64_t k_strides[4];  /* elements: layer, page, head, row (token of a page)        */
+  int64_t v_strides[4];
+  int32_t* block_table;
+  int32_t* lengths;
+  int32_t* refs;
+  void* scratch;
+  int32_t dtype;         /* MOE_KV_F16 or MOE_KV_BF16                                  */
+  int32_t layers;
+  int32_t pages;
+  int32_t kv_heads;
+  int32_t page_size;     /* 16, 32, 64, 128 or 256 tokens                              */
+  int32_t head_dim;      /* 64 or 128                                                  */
+  int32_t sequences;     /* rows of block_table, at most 65536                         */
+  int32_t max_blocks;    /* columns of block_table                                     */
+  int32_t device;
+} MoeKvConfig;
+
+typedef struct MoeKvCache MoeKvCache;
+
+uint64_t moe_kv_scratch_bytes(const MoeKvConfig* cfg);
+int moe_kv_create(const MoeKvConfig* cfg, MoeKvCache** out);
+int moe_kv_destroy(MoeKvCache* cache);
+/* lengths[seqs[i]] += counts[i], with pages for the new tokens: the lowest free pages, in
+ * the order of the entries.  A partly filled last page that other sequences hold too is
+ * replaced by a copy of its filled rows (every layer) first.  All entries or none:
+ * MOE_ERR_NO_PAGES in moe_kv_status when the free pages do not suffice. */
+int moe_kv_reserve(MoeKvCache* cache, const int32_t* seqs, const int32_t* counts, int32_t n,
+                   void* stream);
+/* children[i], an empty sequence, becomes a copy of parents[i] that shares its pages. */
+int moe_kv_fork(MoeKvCache* cache, const int32_t* parents, const int32_t* children, int32_t n,
+                void* stream);
+/* lengths[seqs[i]] = lengths_new[i] <= the old one; pages past the end are let go
+ * (a page that no sequence holds is free).  0 frees the sequence. */
+int moe_kv_truncate(MoeKvCache* cache, const int32_t* seqs, const int32_t* lengths_new, int32_t n,
+                    void* stream);
+/* Whole pages src[i] -> dst[i], every layer; tables and refs stay.  Refused when a dst
+ * comes twice or is also a src. */
+int moe_kv_copy_pages(MoeKvCache* cache, const int32_t* src, const int32_t* dst, int32_t n,
+                      void* stream);
+/* into NULL: the live pages move to the lowest page numbers (those already there stay).
+ * Otherwise they are copied, dense and in order, into another cache of the same device,
+ * dtype and page shape, whose tables are overwritten; MOE_ERR_NO_PAGES if they do not fit. */
+int moe_kv_compact(MoeKvCache* cache, MoeKvCache* into, void* stream);
+/* New rows of a batch: entry i owns rows q_start[i] .. q_start[i+1]-1 (q_start: n_seqs + 1
+ * non-decreasing offsets), the last tokens of sequence seqs[i]: row r is its token
+ * lengths[seqs[i]] - (q_start[i+1] - r).  Reserve first.  k, v: [rows][kv_heads][head_dim] in
+ * the cache's dtype, token and head strides in elements (multiples of 8).  Rows from
+ * q_start[n_seqs] on are ignored.  The same sequence twice: the rows of one entry win. */
+int moe_kv_append(MoeKvCache* cache, int32_t layer, const void* k, const void* v,
+                  const int64_t* k_strides, const int64_t* v_strides, const int32_t* seqs,
+                  const int32_t* q_start, int32_t n_seqs, int32_t rows, void* stream);
+/* out = softmax(scale * q k^T, causal) v of each new row over all tokens of its sequence up
+ * to its own position; fp32 softmax and accumulation, probabilities rounded to the cache's
+ * dtype for the product with v.  lse (may be NULL): natural logarithm of the sum of the
+ * exponentials.  A row that sees no token (more new rows than tokens) gives 0 and -inf.
+ * Rows of out and lse from q_start[n_seqs] on are left as they were.  No finite value in
+ * the pool past a sequence's length, and no NaN or infinity there either, reaches a result. */
+typedef struct MoeKvAttendArgs {
+  const void* q;          /* [rows][heads][head_dim], the cache's dtype                */
+  void* out;              /* as q                                                      */
+  float* lse;             /* [rows][heads] or NULL                                     */
+  int64_t q_strides[2];   /* elements: token, head                                     */
+  int64_t out_strides[2];
+  int64_t lse_strides[2];
+  const int32_t* seqs;
+  const int32_t* q_start;
+  int32_t n_seqs;
+  int32_t rows;
+  int32_t heads;          /* a multiple of kv_heads                                    */
+  int32_t layer;
+  float scale;            /* usually 1 / sqrt(head_dim)                                */
+} MoeKvAttendArgs;
+
+uint64_t moe_kv_attend_workspace_bytes(const MoeKvCache* cache, int32_t heads, int32_t rows,
+                                       int32_t n_seqs);
+int moe_kv_attend(MoeKvCache* cache, const MoeKvAttendArgs* args, void* workspace,
+                  uint64_t workspace_bytes, void* stream);
+/* As moe_status, for the cache's error word (in its scratch). */
+int moe_kv_status(MoeKvCache* cache, void* stream);
 
 /* ------------------------------------------- runtime (CUDABackend, ctypes) */
 int moe_rt_device_count(int32_t* count);
