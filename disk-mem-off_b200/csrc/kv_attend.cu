@@ -4,6 +4,25 @@
 //   o   = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),  m = max_j s_j
 //
 // in one pass over the keys with the running maximum and sum in fp32.
+//
+// Rows.  The `group` query heads that share a kv head read the same keys, so a row is
+// one (new token, head of the group) pair and an entry of m tokens has m * group rows
+// of each kv head.  128 rows fill the M of one tcgen05.mma.
+//
+// Work.  kv_plan_kernel (one CTA) cuts the entries into units: 256 rows that two
+// warpgroups work on against the same keys ("pair"), or up to 128 rows that one
+// warpgroup works on alone ("single": decode steps and the ends of chunks).  A unit of
+// one kv head costs its number of 128-key tiles.  All tiles are numbered in a row and
+// cut into equal shares, pairs for 148 CTAs and singles for 2 * 148 warpgroups, so the
+// load is even for any mix of lengths; a unit cut by a share's border leaves fp32
+// partial results that kv_merge_kernel joins in share order (same bits every time).
+//
+// kv_attend_kernel (one CTA an SM, 320 threads): warps 0-3 and 4-7 are the two softmax
+// warpgroups, a thread a row; warp 8 fetches K and V tiles page by page (TMA, 128-byte
+// swizzle) into one ring; warp 9 issues S = Q K^T (both operands in shared memory, K
+// major) and O += P V (P from TMEM, V as an N-major operand, so that V needs no
+// transposed copy).  TMEM: S0, S1 (128 columns each; P overwrites its S), O0, O1.  While
+// one warpgroup is in its softmax, the tensor cores work for the other.
 #include <cuda_bf16.h>
 #include <math.h>
 
@@ -14,16 +33,347 @@
 
 namespace moe {
 
-template <bool BF16>
-MOE_DEV float2 pair_to_float(uint32_t u) {
-  if constexpr (BF16) {
-    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u));
-  } else {
-    return __half22float2(*reinterpret_cast<const __half2*>(&u));
+constexpr int kTile = 128;       // keys of a tile, rows of a warpgroup
+constexpr int kPlanT = 1024;     // threads of the plan kernel
+constexpr int kPlanSmem = 1024;  // units of a list whose prefix sums fit its shared memory
+
+// Rows [r0, r0 + rows) of an entry, for every kv head.
+struct KaUnit {
+  int seq;    // -1: not a sequence (rows of zeros)
+  int row0;   // the entry's first row in q / out
+  int r0;     // first packed row (token * group + head of the group)
+  int rows;
+  int base;   // position of the entry's first new token (may be negative: sees nothing)
+  int len;    // tokens of the sequence
+  int tiles;  // key tiles that the last row needs
+  int pad;
+};
+static_assert(sizeof(KaUnit) == 32, "two 16-byte loads");
+
+// A share: `count` tiles from tile `tile` of kv head `head` of list entry `item` on.
+struct KaStart {
+  int item, head, tile, count;
+};
+// A unit cut by the end of share `w`: its pieces lie in shares w .. last.
+struct KaCut {
+  int item, head, last, valid;
+};
+
+struct KaWs {
+  size_t start[2], cut[2], list[2], pre[2], o[2], ml[2], total;
+  int cap[2];
+};
+
+// [0] pairs: num_sms shares of 256 rows; [1] singles: 2 * num_sms shares of 128 rows
+static KaWs ka_ws(const KvView& c, int heads, int rows, int n, int num_sms) {
+  KaWs w{};
+  size_t o = 0;
+  auto take = [&](size_t b) {
+    const size_t at = o;
+    o = (o + b + 255) & ~size_t(255);
+    return at;
+  };
+  const int64_t packed = static_cast<int64_t>(rows) * (heads / c.heads);
+  w.cap[0] = packed > kTile ? static_cast<int>(packed / (2 * kTile) + std::min<int64_t>(n, packed / kTile)) : 0;
+  w.cap[1] = n;
+  for (int k = 0; k < 2; ++k) {
+    const size_t shares = static_cast<size_t>(num_sms) * (k + 1);
+    const size_t prow = 2 * shares * (w.cap[k] ? kTile * (2 - k) : 0);
+    w.start[k] = take(shares * sizeof(KaStart));
+    w.cut[k] = take(shares * sizeof(KaCut));
+    w.list[k] = take(static_cast<size_t>(w.cap[k]) * sizeof(KaUnit));
+    w.pre[k] = take((static_cast<size_t>(w.cap[k]) + 1) * 8);
+    w.o[k] = take(prow * c.hd * 4);
+    w.ml[k] = take(prow * 8);
+  }
+  w.total = o;
+  return w;
+}
+
+size_t kv_attend_workspace(const KvView& c, int heads, int rows, int n_seqs, int num_sms) {
+  return ka_ws(c, heads, rows, n_seqs, num_sms).total;
+}
+
+// The workspace by kind (0 pairs, 1 singles), for the kernels.
+struct KaList {
+  KaStart* start;
+  KaCut* cut;
+  KaUnit* list;
+  long long* pre;
+  float* o;    // [share][0 its first unit, 1 its last][rows][hd] unnormalised
+  float2* ml;  // running maximum (base 2, scaled) and sum of the same rows
+};
+struct KaPtrs {
+  KaList pair, single;
+  MOE_DEV KaList kind(int k) const { return k ? single : pair; }
+};
+
+// ------------------------------------------------------------------ plan
+// Inclusive sum over the plan CTA; *total gets the whole sum.
+MOE_DEV long long plan_scan(long long v, long long* total) {
+  __shared__ long long part[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  if (lane == 31) part[warp] = v;
+  __syncthreads();
+  if (warp == 0) {
+    long long p = part[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(0xffffffffu, p, o);
+      if (lane >= o) p += u;
+    }
+    part[lane] = p;
+  }
+  __syncthreads();
+  *total = part[31];
+  const long long before = warp ? part[warp - 1] : 0;
+  __syncthreads();
+  return v + before;
+}
+
+MOE_DEV int key_tiles(int base, int last_token) {
+  // tokens visible to the unit's last row, at least one tile (rows that see nothing
+  // still have to be written); beyond the table they read as zeros and are masked
+  const long long vis = static_cast<long long>(max(base, 0)) + last_token + 1;
+  return static_cast<int>((vis + kTile - 1) / kTile);
+}
+
+// (1) entries -> units, (2) prefix sums of their tiles, (3) each share's first tile and
+// the units that the shares cut.  Two dependent loads and three scans: about 3 us.
+__global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const KvBatch b,
+                                                         const int group, const int num_sms,
+                                                         const KaPtrs w, const int cap0,
+                                                         const int min0, const int min1) {
+  pdl_enter();
+  __shared__ long long spre[2][kPlanSmem + 1];
+  const int tid = threadIdx.x, lane = tid & 31;
+  // (1)
+  int n_list[2] = {0, 0};
+  for (int i0 = 0; i0 < b.n; i0 += kPlanT) {
+    const int i = i0 + tid;
+    int seq = -1, row0 = 0, m = 0, len = 0;
+    if (i < b.n) {
+      seq = b.seqs[i];
+      row0 = b.q_start[i];
+      const long long end = b.q_start[i + 1];
+      if (row0 < 0 || end < row0 || end > b.rows) {
+        record_error(c.err, DEV_BAD_LENGTH);
+      } else {
+        m = static_cast<int>(end) - row0;
+      }
+      if (seq < 0 || seq >= c.nseq) {
+        if (m > 0) record_error(c.err, DEV_BAD_SEQ);
+        seq = -1;
+      } else {
+        len = max(c.len[seq], 0);
+        if (len > static_cast<long long>(c.max_blocks) << c.page_shift) {
+          record_error(c.err, DEV_BAD_LENGTH);
+          len = c.max_blocks << c.page_shift;
+        }
+      }
+    }
+    const int rows = m * group;
+    const int rem = rows & (2 * kTile - 1);
+    const int na = rows / (2 * kTile) + (rem > kTile ? 1 : 0), nb = rem > 0 && rem <= kTile ? 1 : 0;
+    long long total;
+    const long long mine = na | (static_cast<long long>(nb) << 32);
+    const long long before = plan_scan(mine, &total) - mine;
+    const int at_a = n_list[0] + static_cast<int>(before & 0xffffffff);
+    const int at_b = n_list[1] + static_cast<int>(before >> 32);
+    if (nb)
+      w.single.list[at_b] = KaUnit{seq, row0, rows - rem, rem, len - m, len, key_tiles(len - m, m - 1), 0};
+    // pairs of one entry: the warp's lanes side by side
+    for (uint32_t todo = __ballot_sync(0xffffffffu, na > 0); todo; todo &= todo - 1) {
+      const int l = __ffs(todo) - 1;
+      const int k = __shfl_sync(0xffffffffu, na, l), at = __shfl_sync(0xffffffffu, at_a, l);
+      const int rs = __shfl_sync(0xffffffffu, rows, l), q0 = __shfl_sync(0xffffffffu, row0, l);
+      const int sq = __shfl_sync(0xffffffffu, seq, l), ln = __shfl_sync(0xffffffffu, len, l);
+      const int mm = __shfl_sync(0xffffffffu, m, l);
+      for (int j = lane; j < k && at + j < cap0; j += 32) {
+        const int r0 = j * 2 * kTile, r1 = min(r0 + 2 * kTile, rs);
+        w.pair.list[at + j] = KaUnit{sq, q0, r0, r1 - r0, ln - mm, ln, key_tiles(ln - mm, (r1 - 1) / group), 0};
+      }
+    }
+    n_list[0] += static_cast<int>(total & 0xffffffff);
+    n_list[1] += static_cast<int>(total >> 32);
+  }
+  n_list[0] = min(n_list[0], cap0);
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    // (2)
+    const int n = n_list[k];
+    const KaList w_k = w.kind(k);
+    long long* pre = n <= kPlanSmem ? spre[k] : w_k.pre;
+    long long work = 0;
+    for (int i0 = 0; i0 < n; i0 += kPlanT) {
+      const int i = i0 + tid;
+      const long long t = i < n ? static_cast<long long>(w_k.list[i].tiles) * c.heads : 0;
+      long long total;
+      const long long incl = work + plan_scan(t, &total);
+      if (i < n) pre[i + 1] = incl;
+      work += total;
+    }
+    if (tid == 0) pre[0] = 0;
+    __syncthreads();
+    // (3)
+    const int shares = num_sms * (k + 1);
+    long long per = (work + shares - 1) / shares;
+    per = max(per, static_cast<long long>(k ? min1 : min0));
+    for (int s = tid; s <= shares; s += kPlanT) {
+      const long long w0 = s * per;
+      KaStart st{0, 0, 0, 0};
+      KaCut cut{0, 0, 0, 0};
+      if (w0 < work) {
+        int lo = 0, hi = n;  // pre[lo] <= w0 < pre[hi]
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (pre[mid] <= w0) lo = mid;
+          else hi = mid;
+        }
+        const int tiles = static_cast<int>((pre[lo + 1] - pre[lo]) / c.heads);
+        const long long r = w0 - pre[lo];
+        st.item = lo;
+        st.head = static_cast<int>(r / tiles);
+        st.tile = static_cast<int>(r - static_cast<long long>(st.head) * tiles);
+        st.count = static_cast<int>(min(per, work - w0));
+        const long long u0 = w0 - st.tile;
+        if (s > 0 && st.tile > 0 && u0 >= (s - 1) * per)
+          cut = KaCut{lo, st.head, static_cast<int>((u0 + tiles - 1) / per), 1};
+      }
+      if (s < shares) w_k.start[s] = st;
+      if (s > 0) w_k.cut[s - 1] = cut;
+    }
   }
 }
+
+// ------------------------------------------------------------------ the kernel
+template <int HD>
+struct KaCfg {
+  static constexpr int kQ = kTile * HD * 2;      // one warpgroup's Q tile
+  static constexpr int kStage = kTile * HD * 2;  // one K or V tile
+  static constexpr int kStages = HD == 128 ? 5 : 8;
+  static constexpr int kLoads = HD / 64;         // 64-dim blocks of a tile
+  static constexpr size_t kSmem = 1024 + 2 * kQ + kStages * kStage + 512;
+};
+static_assert(KaCfg<128>::kSmem <= 227 * 1024 && KaCfg<64>::kSmem > 114 * 1024,
+              "one CTA, and with it all of TMEM, an SM");
+
+// Twelve warps (8: K / V, 9: MMA, 10 and 11 idle), so that each third is a warpgroup and
+// registers can move between them: 384 * 168 at launch = 2 * 128 * 208 + 128 * 80 + rest.
+constexpr int kAttThreads = 384;
+constexpr int kRegsSoftmax = 208, kRegsOther = 80;
+static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kAttThreads * 168, "more than the launch had");
+template <int N>
+MOE_DEV void regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+MOE_DEV void regs_fewer() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+constexpr uint32_t kOCols = 2 * kTile;  // TMEM: S0 S1 at 0, 128; O0 O1 at 256, 384
+
+// Five-dimensional tiled load (dim, row, head, page, layer); a page past the end reads
+// as zeros.
+MOE_DEV void tma_load_5d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, int c4,
+                         uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4),
+      "r"(smem_u32(bar))
+      : "memory");
+}
+
+MOE_DEV void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+MOE_DEV void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// Instruction descriptor of f16 (fmt 0) or bf16 (1) operands, M = 128, B K-major or (nmajor) N-major.
+__host__ __device__ constexpr uint32_t ka_idesc(uint32_t fmt, int n, uint32_t nmajor) {
+  return (1u << 4) | (fmt << 7) | (fmt << 10) | (nmajor << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(kTile >> 4) << 24);
+}
+
+// Descriptor of a V tile as the N-major B operand: rows of a key with 64 dims (128
+// bytes, 128-byte swizzle), 8 keys every 1024 bytes (SBO), the next 64 dims 16 KiB on (LBO).
+MOE_DEV uint64_t nmajor_desc(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFF);
+  d |= static_cast<uint64_t>(16384 >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+
+// The tiles of a share in order.
+struct KaCursor {
+  const KaUnit* list;
+  KaUnit u;
+  int item, head, tile, left, heads;
+  MOE_DEV void load() {
+    const int4* p = reinterpret_cast<const int4*>(list + item);
+    const int4 a = p[0], b = p[1];
+    u.seq = a.x; u.row0 = a.y; u.r0 = a.z; u.rows = a.w;
+    u.base = b.x; u.len = b.y; u.tiles = b.z;
+  }
+  MOE_DEV void init(const KaPtrs& w, int kind, int share, int kv_heads) {
+    const KaList l = w.kind(kind);
+    const int4 s = *reinterpret_cast<const int4*>(l.start + share);
+    list = l.list;
+    item = s.x;
+    head = s.y;
+    tile = s.z;
+    left = s.w;
+    heads = kv_heads;
+    if (left > 0) load();
+  }
+  // this share's last tile of the unit
+  MOE_DEV bool ends_unit() const { return tile + 1 == u.tiles || left == 1; }
+  MOE_DEV void next() {
+    --left;
+    if (++tile == u.tiles) {
+      tile = 0;
+      if (++head == heads) {
+        head = 0;
+        ++item;
+        if (left > 0) load();
+      }
+    }
+  }
+};
+
+// Page numbers of a sequence, 32 blocks at a time in the lanes of the producer warp,
+// the next 32 already on their way.
+struct KaPages {
+  int seq = -2, chunk = -1, ids = -1, nxt = -1;
+  MOE_DEV static int fetch(const KvView& c, const KaUnit& u, int chunk) {
+    const int blk = chunk * 32 + (threadIdx.x & 31);
+    const int need = (u.len + c.page - 1) >> c.page_shift;
+    return u.seq >= 0 && blk < need ? c.table[static_cast<long long>(u.seq) * c.max_blocks + blk] : -1;
+  }
+  MOE_DEV void at(const KvView& c, const KaUnit& u, int block) {
+    const int want = block >> 5;
+    if (u.seq != seq || want != chunk) {
+      ids = u.seq == seq && want == chunk + 1 ? nxt : fetch(c, u, want);
+      nxt = fetch(c, u, want + 1);
+      seq = u.seq;
+      chunk = want;
+    }
+  }
+};
+
+// The whole warp waits and takes the same way out.
+MOE_DEV bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag));
+}
+
 template <bool BF16>
-MOE_DEV uint32_t float_to_pair(float a, float b) {
+MOE_DEV uint32_t pack2(float a, float b) {
   if constexpr (BF16) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -33,87 +383,590 @@ MOE_DEV uint32_t float_to_pair(float a, float b) {
   }
 }
 
-// A warp per (row, head), each lane HD / 32 dims, one key a step.
+MOE_DEV float exp2_ftz(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 32 TMEM columns of a row on their way; they may be read after tmem_landed.
+MOE_DEV void tmem_ld32_start(uint32_t taddr, float* v) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+        "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+        "=r"(r[31])
+      : "r"(taddr));
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+// Waits for this thread's TMEM loads; v passes through, so that no use moves above.
+MOE_DEV void tmem_landed(float* v, int n) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < n; ++i) asm volatile("" : "+f"(v[i]));
+}
+MOE_DEV void load_s(uint32_t taddr, float (&sc)[kTile]) {
+#pragma unroll
+  for (int i = 0; i < kTile / 32; ++i) tmem_ld32_start(taddr + i * 32, sc + i * 32);
+  tmem_landed(sc, kTile);
+}
+
 template <int HD, bool BF16>
-__global__ void __launch_bounds__(128) kv_attend_kernel(const KvView c, const KvBatch b,
-                                                        const KvAttend a) {
-  pdl_enter();
-  constexpr int V = HD / 64;  // pairs a lane
-  const int lane = threadIdx.x & 31;
-  const int64_t total = static_cast<int64_t>(min(b.q_start[b.n], b.rows)) * a.heads;
-  const int64_t warps = static_cast<int64_t>(gridDim.x) * 4;
-  for (int64_t it = blockIdx.x * 4 + (threadIdx.x >> 5); it < total; it += warps) {
-    const int r = static_cast<int>(it / a.heads), h = static_cast<int>(it - static_cast<int64_t>(r) * a.heads);
-    const int e = entry_of_row(b.q_start, b.n, r);
-    if (e < 0) continue;
-    const int s = b.seqs[e];
-    const bool known = s >= 0 && s < c.nseq;
-    if (!known && lane == 0) record_error(c.err, DEV_BAD_SEQ);
-    const int len = known ? c.len[s] : 0;
-    const int64_t pos = static_cast<int64_t>(len) - (b.q_start[e + 1] - r);
-    float q[2 * V], o[2 * V];
-    const uint32_t* qp = reinterpret_cast<const uint32_t*>(static_cast<const __half*>(a.q) + r * a.qs[0] +
-                                                           h * a.qs[1]) + lane * V;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float2 f = pair_to_float<BF16>(qp[i]);
-      q[2 * i] = f.x * a.scale;
-      q[2 * i + 1] = f.y * a.scale;
-      o[2 * i] = o[2 * i + 1] = 0.f;
+__global__ void __launch_bounds__(kAttThreads, 1)
+    kv_attend_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                     const KvView c, const KvAttend a, const KaPtrs w, const int group,
+                     const float scale_log2) {
+  using C = KaCfg<HD>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sR = sQ + 2 * C::kQ;  // the K / V ring
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sR + C::kStages * C::kStage);
+  uint64_t* full = bars;                   // [kStages]
+  uint64_t* empty = bars + C::kStages;     // [kStages]
+  uint64_t* q_full = bars + 2 * C::kStages;  // [2] Q tile of the next unit written
+  uint64_t* s_full = q_full + 2;           // [2] S of a tile done (and every MMA before it)
+  uint64_t* p_full = q_full + 4;           // [2] P of a tile written
+  uint64_t* o_done = q_full + 6;           // [2] P V of a tile done
+  uint64_t* mma_done = q_full + 8;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 9);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
     }
-    float m = -INFINITY, l = 0.f;
-    const int kvh = h / (a.heads / c.heads);
-    for (int64_t j = 0; j <= pos; ++j) {
-      const int64_t blk = j >> c.page_shift;
-      const int pg = blk < c.max_blocks ? c.table[static_cast<int64_t>(s) * c.max_blocks + blk] : -1;
-      if (pg < 0 || pg >= c.pages) {
-        if (lane == 0) record_error(c.err, DEV_BAD_PAGE);
-        break;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 4);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_done[i], 1);
+    }
+    mbar_init(mma_done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  if (warp == 8 && lane == 0) {
+    tma_prefetch_desc(&tk);
+    tma_prefetch_desc(&tv);
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+
+  const int cta = blockIdx.x, ctas = gridDim.x;
+  if (warp >= 8) {
+  regs_fewer<kRegsOther>();
+  if (warp == 8) {
+    // ------------------------------------------------------------ K / V tiles
+    int n = 0;  // tiles put into the ring so far
+    bool ok = true;
+    auto put = [&](const KaUnit& u, int head, int tile, KaPages& pg, bool val) {
+      const int st = n % C::kStages;
+      if (!warp_wait(&empty[st], ((n / C::kStages) & 1) ^ 1, abort_flag)) {
+        ok = false;
+        return;
       }
-      const int64_t slot = j & (c.page - 1);
-      const uint32_t* kp = reinterpret_cast<const uint32_t*>(c.k + a.layer * c.ks[0] + pg * c.ks[1] +
-                                                             kvh * c.ks[2] + slot * c.ks[3]) + lane * V;
-      const uint32_t* vp = reinterpret_cast<const uint32_t*>(c.v + a.layer * c.vs[0] + pg * c.vs[1] +
-                                                             kvh * c.vs[2] + slot * c.vs[3]) + lane * V;
-      float x = 0.f;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float2 f = pair_to_float<BF16>(kp[i]);
-        x = fmaf(q[2 * i], f.x, x);
-        x = fmaf(q[2 * i + 1], f.y, x);
+      const int key0 = tile * kTile;
+      const int blk = key0 >> c.page_shift;
+      pg.at(c, u, blk);
+      if (lane == 0) mbar_arrive_expect_tx(&full[st], C::kStage);
+      __syncwarp();
+      const int per = max(kTile >> c.page_shift, 1);  // pages of a tile
+      const int p = lane / C::kLoads, kb = lane - p * C::kLoads;
+      int id = __shfl_sync(0xffffffffu, pg.ids, (blk + p) & 31);
+      if (lane < per * C::kLoads) {
+        if (id < 0 || id >= c.pages) {
+          // past the sequence's last page: zeros; before it: a hole in the table
+          if (static_cast<long long>(blk + p) << c.page_shift < u.len) record_error(c.err, DEV_BAD_PAGE);
+          id = c.pages;
+        }
+        tma_load_5d(smem_u32(sR + st * C::kStage) + kb * 16384 + p * c.page * 128, val ? &tv : &tk, kb * 64,
+                    key0 & (c.page - 1), head, id, a.layer, &full[st]);
       }
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-      const float mn = fmaxf(m, x);
-      const float keep = m == -INFINITY ? 0.f : __expf(m - mn), p = __expf(x - mn);
-      m = mn;
-      l = l * keep + p;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float2 f = pair_to_float<BF16>(vp[i]);
-        o[2 * i] = fmaf(p, f.x, o[2 * i] * keep);
-        o[2 * i + 1] = fmaf(p, f.y, o[2 * i + 1] * keep);
+      ++n;
+    };
+    KaCursor x;
+    KaPages px;
+    x.init(w, 0, cta, c.heads);
+    while (ok && x.left > 0) {
+      put(x.u, x.head, x.tile, px, false);
+      if (ok) put(x.u, x.head, x.tile, px, true);
+      x.next();
+    }
+    KaCursor y;
+    KaPages py;
+    x.init(w, 1, cta, c.heads);
+    y.init(w, 1, cta + ctas, c.heads);
+    if (ok && x.left > 0) put(x.u, x.head, x.tile, px, false);
+    if (ok && y.left > 0) put(y.u, y.head, y.tile, py, false);
+    while (ok && (x.left > 0 || y.left > 0)) {
+      if (x.left > 0) {
+        put(x.u, x.head, x.tile, px, true);
+        x.next();
+        if (ok && x.left > 0) put(x.u, x.head, x.tile, px, false);
+      }
+      if (ok && y.left > 0) {
+        put(y.u, y.head, y.tile, py, true);
+        y.next();
+        if (ok && y.left > 0) put(y.u, y.head, y.tile, py, false);
       }
     }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    uint32_t* op = reinterpret_cast<uint32_t*>(static_cast<__half*>(a.out) + r * a.os[0] + h * a.os[1]) + lane * V;
+    if (!ok) {
+      *abort_flag = 1;
+      if (lane == 0) record_error(c.err, DEV_TIMEOUT_EMPTY);
+    }
+    // every copy must land before the CTA exits
+    for (int j = n - 1; j >= 0 && j >= n - C::kStages; --j)
+      mbar_wait_drain(&full[j % C::kStages], (j / C::kStages) & 1);
+  } else if (warp == 9) {
+    // ------------------------------------------------------------ MMA issue
+    constexpr uint32_t fmt = BF16 ? 1 : 0;
+    constexpr uint32_t id_s = ka_idesc(fmt, kTile, 0), id_o = ka_idesc(fmt, HD, 1);
+    const uint32_t aq = smem_u32(sQ), ar = smem_u32(sR);
+    bool ok = true;
+    int n = 0;             // ring tiles taken
+    int np[2] = {0, 0};    // P tiles taken, by stream
+    int nq[2] = {0, 0};    // units begun
+    // the next ring tile has landed
+    auto take = [&]() -> int {
+      const int st = n % C::kStages;
+      if (!warp_wait(&full[st], (n / C::kStages) & 1, abort_flag)) ok = false;
+      ++n;
+      return st;
+    };
+    // S of stream s from Q tile s and ring stage st
+    auto issue_s = [&](int s, int st, bool begins) {
+      if (begins) {
+        if (!warp_wait(&q_full[s], nq[s] & 1, abort_flag)) ok = false;
+        ++nq[s];
+      }
+      tc_fence_after();
+      if (ok && lane == 0) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) op[i] = float_to_pair<BF16>(o[2 * i] * inv, o[2 * i + 1] * inv);
-    if (a.lse && lane == 0) a.lse[r * a.ls[0] + h * a.ls[1]] = l > 0.f ? m + logf(l) : -INFINITY;
+        for (int k = 0; k < HD / 16; ++k) {
+          const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
+          tc_mma_f16(tmem + s * kTile, sw128_desc(aq + s * C::kQ + off), sw128_desc(ar + st * C::kStage + off),
+                     id_s, k > 0 ? 1u : 0u);
+        }
+        tc_commit(&s_full[s]);
+      }
+      __syncwarp();
+    };
+    // keys past the sequence's end hold whatever was in the page: their rows of V are
+    // zeroed, since P is zero there but 0 * NaN is not
+    auto clear_v = [&](int st, const KaUnit& u, int tile) {
+      const int valid = u.len - tile * kTile;
+      if (valid >= kTile) return;
+      const int from = max(valid, 0) * 128;
+      for (int kb = 0; kb < C::kLoads; ++kb)
+        for (int o = from + lane * 16; o < 16384; o += 512)
+          *reinterpret_cast<uint4*>(sR + st * C::kStage + kb * 16384 + o) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async_smem();
+      __syncwarp();
+    };
+    auto issue_o = [&](int s, int st, bool first) {
+      if (!warp_wait(&p_full[s], np[s] & 1, abort_flag)) ok = false;
+      ++np[s];
+      tc_fence_after();
+      if (ok && lane == 0) {
+#pragma unroll
+        for (int k = 0; k < kTile / 16; ++k)
+          tc_mma_f16_ts(tmem + kOCols + s * kTile, tmem + s * kTile + k * 8,
+                        nmajor_desc(ar + st * C::kStage + k * 2048), id_o, (!first || k > 0) ? 1u : 0u);
+        tc_commit(&o_done[s]);
+      }
+      __syncwarp();
+    };
+    auto release = [&](int st) {
+      if (ok && lane == 0) tc_commit(&empty[st]);
+      __syncwarp();
+    };
+    // pairs: both streams read the same K and V tiles.  At a unit's end the next S (which
+    // waits for the next Q) comes after both products with V.
+    KaCursor x;
+    x.init(w, 0, cta, c.heads);
+    if (x.left > 0) {
+      int kst = take();
+      if (ok) issue_s(0, kst, true);
+      if (ok) issue_s(1, kst, true);
+      if (ok) release(kst);
+      bool first = true;
+      while (ok) {
+        const KaUnit u = x.u;
+        const int tile = x.tile;
+        const bool ends = x.ends_unit();
+        x.next();
+        const bool more = x.left > 0;
+        const int vst = take();
+        if (!ok) break;
+        clear_v(vst, u, tile);
+        issue_o(0, vst, first);
+        if (ok && more && !ends) {
+          kst = take();
+          if (ok) issue_s(0, kst, false);
+        }
+        if (ok) issue_o(1, vst, first);
+        if (ok) release(vst);
+        if (ok && more && ends) {
+          kst = take();
+          if (ok) issue_s(0, kst, true);
+        }
+        if (ok && more) {
+          issue_s(1, kst, ends);
+          if (ok) release(kst);
+        }
+        first = ends;
+        if (!more) break;
+      }
+    }
+    // singles: each stream has its own units
+    KaCursor y[2];
+    bool first[2] = {true, true};
+#pragma unroll
+    for (int s = 0; s < 2; ++s) y[s].init(w, 1, cta + s * ctas, c.heads);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      if (ok && y[s].left > 0) {
+        const int st = take();
+        if (ok) issue_s(s, st, true);
+        if (ok) release(st);
+      }
+    }
+    while (ok && (y[0].left > 0 || y[1].left > 0)) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if (!ok || y[s].left <= 0) continue;
+        const bool ends = y[s].ends_unit();
+        const int vst = take();
+        if (!ok) break;
+        clear_v(vst, y[s].u, y[s].tile);
+        issue_o(s, vst, first[s]);
+        if (ok) release(vst);
+        first[s] = ends;
+        y[s].next();
+        if (ok && y[s].left > 0) {
+          const int kst = take();
+          if (ok) issue_s(s, kst, ends);
+          if (ok) release(kst);
+        }
+      }
+    }
+    if (!ok) {
+      *abort_flag = 1;
+      if (lane == 0) record_error(c.err, DEV_TIMEOUT_FULL);
+    }
+    if (lane == 0) {
+      tc_commit(mma_done);  // no MMA may still write TMEM when it is released
+      mbar_wait_drain(mma_done, 0);
+    }
+    __syncwarp();
+  }
+  } else {
+    // ------------------------------------------------------------ softmax
+    regs_more<kRegsSoftmax>();
+    const int s = warp >> 2;           // stream
+    const int quad = warp & 3;         // TMEM lanes 32 * quad ..
+    const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t t_s = tmem + lanes + s * kTile;           // S, then P, of this stream
+    const uint32_t t_o = tmem + lanes + kOCols + s * kTile;  // O
+    // P is scaled by 2^shift: f16 keeps probabilities down to 2^-31 of the largest
+    // (the reference maximum may lag by 2^8: 2^15 at most, below f16's 65504)
+    constexpr float shift = BF16 ? 0.f : 7.f;
+    const __half* q16 = static_cast<const __half*>(a.q);
+    __half* out16 = static_cast<__half*>(a.out);
+    bool ok = true;
+    int nt = 0;  // tiles of this stream so far
+    // this warp's 32 rows of a unit's Q, swizzled as the MMA reads them; two rows a step
+    auto load_q = [&](const KaUnit& u, int head, int part) {
+      constexpr int ch = HD / 8;       // 16-byte chunks of a row
+      const int row_in = lane / ch, chunk = lane - row_in * ch;
+      const uint32_t base = smem_u32(sQ) + s * C::kQ + (chunk >> 3) * 16384;
+      for (int r = row_in; r < 32; r += 32 / ch) {
+        const int row = quad * 32 + r;
+        const int pr = part * kTile + row;
+        if (pr < u.rows) {
+          const int packed = u.r0 + pr;
+          const int tok = packed / group, hg = packed - tok * group;
+          const __half* src = q16 + (static_cast<long long>(u.row0) + tok) * a.qs[0] +
+                              (static_cast<long long>(head) * group + hg) * a.qs[1] + chunk * 8;
+          cp_async16(base + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), src);
+        }
+      }
+    };
+    auto q_ready = [&]() {
+      cp_async_wait();
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full[s]);
+    };
+#pragma unroll 1
+    for (int kind = 0; kind < 2 && ok; ++kind) {
+      const int share = kind ? cta + s * ctas : cta;
+      const int part = kind ? 0 : s;  // the unit's rows of this warpgroup: part * 128 ..
+      KaCursor x;
+      x.init(w, kind, share, c.heads);
+      if (x.left <= 0) continue;
+      load_q(x.u, x.head, part);
+      q_ready();
+      bool cut_front = x.tile > 0;  // the unit began in an earlier share
+      while (x.left > 0 && ok) {
+        const KaUnit u = x.u;
+        const int head = x.head;
+        const int pr = part * kTile + quad * 32 + lane;
+        const bool valid = pr < u.rows;
+        const bool any = part * kTile + quad * 32 < u.rows;  // a row in this warp
+        const int packed = u.r0 + (valid ? pr : 0);
+        const int tok = packed / group, hg = packed - tok * group;
+        // tokens that the row sees: all up to its own position
+        const int seen = valid ? max(min(u.base + tok + 1, u.len), 0) : 0;
+        float m = -INFINITY, l = 0.f;
+        bool first = true, whole = true;
+        for (bool ends = false; !ends; first = false) {
+          ends = x.ends_unit();
+          const int key0 = x.tile * kTile;
+          if (ends) whole = x.tile + 1 == u.tiles;
+          x.next();
+          if (!warp_wait(&s_full[s], nt & 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const bool load_next = ends && x.left > 0;
+          if (load_next) load_q(x.u, x.head, part);  // S of this unit is done: Q is free
+          if (any) {
+            float sc[kTile];
+            load_s(t_s, sc);
+            const int lim = seen - key0;
+            if (__any_sync(0xffffffffu, lim < kTile)) {
+#pragma unroll
+              for (int j = 0; j < kTile; ++j)
+                if (j >= lim) sc[j] = -INFINITY;
+            }
+            float mx[4] = {sc[0], sc[1], sc[2], sc[3]};
+#pragma unroll
+            for (int j = 4; j < kTile; ++j) mx[j & 3] = fmaxf(mx[j & 3], sc[j]);
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;
+            // m, the maximum that P, l and O refer to, moves (and l and O are rescaled)
+            // only when it grows by more than 2^8
+            const bool grow = valid && top - m > 8.f;
+            float alpha = 1.f;
+            if (grow) {
+              alpha = exp2f(m - top);
+              m = top;
+            }
+            const float ref = m == -INFINITY ? 0.f : m - shift;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < kTile; ++j) {
+              sc[j] = exp2_ftz(fmaf(sc[j], scale_log2, -ref));
+              sum[j & 3] += sc[j];
+            }
+            l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+            if (!first && __any_sync(0xffffffffu, grow)) {
+              // s_full of this tile also says that O is complete up to the one before
+#pragma unroll
+              for (int i = 0; i < HD / 16; ++i) {
+                float o[16];
+                tmem_ld16(t_o + i * 16, o);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) o[j] *= alpha;
+                tmem_st16(t_o + i * 16, o);
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              uint32_t pk[32];
+#pragma unroll
+              for (int j = 0; j < 32; ++j) pk[j] = pack2<BF16>(sc[i * 64 + 2 * j], sc[i * 64 + 2 * j + 1]);
+              tmem_st32_nowait(t_s + i * 32, pk);
+            }
+            tmem_wait_st();
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[s]);
+          if (load_next) q_ready();
+          ++nt;
+        }
+        if (!ok) break;
+        if (!warp_wait(&o_done[s], (nt - 1) & 1, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (any) {
+          if (whole && !cut_front) {
+            const long long row = static_cast<long long>(u.row0) + tok;
+            const int h = head * group + hg;
+            const float inv = l > 0.f ? 1.f / l : 0.f;
+            uint4* dst = reinterpret_cast<uint4*>(out16 + row * a.os[0] + h * a.os[1]);
+#pragma unroll
+            for (int i = 0; i < HD / 32; ++i) {
+              float o[32];
+              tmem_ld32(t_o + i * 32, o);
+              uint32_t pk[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                pk[j] = l > 0.f ? pack2<BF16>(o[2 * j] * inv, o[2 * j + 1] * inv) : 0u;
+              if (valid) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) dst[i * 4 + j] = make_uint4(pk[4 * j], pk[4 * j + 1], pk[4 * j + 2], pk[4 * j + 3]);
+              }
+            }
+            if (valid && a.lse)
+              a.lse[row * a.ls[0] + h * a.ls[1]] =
+                  l > 0.f ? (m - shift + log2f(l)) * 0.6931471805599453f : -INFINITY;
+          } else {
+            // a piece: unnormalised, to the share's slot 0 (its first unit) or 1 (its last)
+            const int per = kind ? kTile : 2 * kTile;
+            const long long slot = (2ll * share + (cut_front ? 0 : 1)) * per + pr;
+            float4* dst = reinterpret_cast<float4*>(w.kind(kind).o + slot * HD);
+#pragma unroll
+            for (int i = 0; i < HD / 32; ++i) {
+              float o[32];
+              tmem_ld32(t_o + i * 32, o);
+              if (valid) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                  dst[i * 8 + j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+              }
+            }
+            if (valid) w.kind(kind).ml[slot] = make_float2(l > 0.f ? m - shift : -INFINITY, l);
+          }
+        }
+        tc_fence_before();  // O is read: the next unit's first product may overwrite it
+        cut_front = false;
+      }
+    }
+    if (!ok) {
+      *abort_flag = 1;
+      if (lane == 0) record_error(c.err, DEV_TIMEOUT_TMEM_FULL);
+      cp_async_wait();
+    }
+  }
+  pdl_release();
+  __syncthreads();
+  if (warp == 9) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
   }
 }
 
-size_t kv_attend_workspace(const KvView&, int, int, int, int) { return 256; }
+// ------------------------------------------------------------------ merge
+// Rows of the units that a share's border cut: pieces in shares first .. last, joined in
+// that order.  A warp a row.
+template <int HD, bool BF16>
+__global__ void __launch_bounds__(256) kv_merge_kernel(const KvAttend a, const KaPtrs w, const int group,
+                                                       const int num_sms) {
+  pdl_enter();
+  constexpr int V = HD / 32;
+  const int kind = static_cast<int>(blockIdx.x) >= num_sms ? 1 : 0;
+  const int share = blockIdx.x - kind * num_sms;
+  const KaList wk = w.kind(kind);
+  const int4 cut = *reinterpret_cast<const int4*>(wk.cut + share);
+  if (!cut.w) return;
+  const KaUnit u = wk.list[cut.x];
+  const int lane = threadIdx.x & 31;
+  const int per = kind ? kTile : 2 * kTile;
+  for (int pr = blockIdx.y * 8 + (threadIdx.x >> 5); pr < u.rows; pr += gridDim.y * 8) {
+    float top = -INFINITY;
+    for (int p = share + lane; p <= cut.z; p += 32)
+      top = fmaxf(top, wk.ml[(2ll * p + (p == share ? 1 : 0)) * per + pr].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float acc[V] = {}, l = 0.f;
+    if (top != -INFINITY) {
+#pragma unroll 4
+      for (int p = share; p <= cut.z; ++p) {
+        const long long slot = (2ll * p + (p == share ? 1 : 0)) * per + pr;
+        const float2 ml = wk.ml[slot];
+        const float f = exp2f(ml.x - top);
+        float v[V];
+        const float* src = wk.o + slot * HD + lane * V;
+        if constexpr (V == 4) {
+          const float4 t = *reinterpret_cast<const float4*>(src);
+          v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+        } else {
+          const float2 t = *reinterpret_cast<const float2*>(src);
+          v[0] = t.x; v[1] = t.y;
+        }
+        l += f * ml.y;
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = fmaf(f, v[i], acc[i]);
+      }
+    }
+    const int packed = u.r0 + pr;
+    const int tok = packed / group, hg = packed - tok * group;
+    const long long row = static_cast<long long>(u.row0) + tok;
+    const int h = cut.y * group + hg;
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<__half*>(a.out) + row * a.os[0] + h * a.os[1]) + lane * (V / 2);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) dst[i] = pack2<BF16>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+    if (a.lse && lane == 0)
+      a.lse[row * a.ls[0] + h * a.ls[1]] = l > 0.f ? (top + log2f(l)) * 0.6931471805599453f : -INFINITY;
+  }
+}
 
-cudaError_t kv_launch_attend(const KvView& c, const CUtensorMap&, const CUtensorMap&, bool bf16,
-                             const KvBatch& b, const KvAttend& a, void*, int num_sms, cudaStream_t s) {
-  const int64_t items = static_cast<int64_t>(b.rows) * a.heads;
-  const dim3 grid(static_cast<int>(std::min<int64_t>((items + 3) / 4, num_sms * 16)));
+template <int HD, bool BF16>
+static cudaError_t ka_launch(const KvView& c, const CUtensorMap& tk, const CUtensorMap& tv,
+                             const KvBatch& b, const KvAttend& a, char* ws, int num_sms, cudaStream_t s) {
+  const int group = a.heads / c.heads;
+  const KaWs l = ka_ws(c, a.heads, b.rows, b.n, num_sms);
+  KaPtrs w{};
+  for (int k = 0; k < 2; ++k) {
+    KaList& d = k ? w.single : w.pair;
+    d.start = reinterpret_cast<KaStart*>(ws + l.start[k]);
+    d.cut = reinterpret_cast<KaCut*>(ws + l.cut[k]);
+    d.list = reinterpret_cast<KaUnit*>(ws + l.list[k]);
+    d.pre = reinterpret_cast<long long*>(ws + l.pre[k]);
+    d.o = reinterpret_cast<float*>(ws + l.o[k]);
+    d.ml = reinterpret_cast<float2*>(ws + l.ml[k]);
+  }
+  constexpr size_t smem = KaCfg<HD>::kSmem;
+  static bool attr_set[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    const cudaError_t st = cudaFuncSetAttribute(kv_attend_kernel<HD, BF16>,
+                                                cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                static_cast<int>(smem));
+    if (st != cudaSuccess) return st;
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
+  MOE_PDL(kv_plan_kernel, dim3(1), dim3(kPlanT), 0, s, c, b, group, num_sms, w, l.cap[0], 1, 1);
+  MOE_PDL(kv_attend_kernel<HD, BF16>, dim3(num_sms), dim3(kAttThreads), smem, s, tk, tv, c, a, w, group,
+          static_cast<float>(a.scale * 1.4426950408889634));
+  const int64_t packed = static_cast<int64_t>(b.rows) * group;
+  const int chunks = static_cast<int>(std::min<int64_t>((packed + 7) / 8, packed > kTile ? 16 : 8));
+  MOE_PDL(kv_merge_kernel<HD, BF16>, dim3(num_sms * 3, chunks), dim3(256), 0, s, a, w, group, num_sms);
+  return cudaSuccess;
+}
+
+cudaError_t kv_launch_attend(const KvView& c, const CUtensorMap& tk, const CUtensorMap& tv, bool bf16,
+                             const KvBatch& b, const KvAttend& a, void* ws, int num_sms, cudaStream_t s) {
+  char* p = static_cast<char*>(ws);
   if (c.hd == 128)
-    return bf16 ? pdl_launch(kv_attend_kernel<128, true>, grid, dim3(128), 0, s, c, b, a)
-                : pdl_launch(kv_attend_kernel<128, false>, grid, dim3(128), 0, s, c, b, a);
-  return bf16 ? pdl_launch(kv_attend_kernel<64, true>, grid, dim3(128), 0, s, c, b, a)
-              : pdl_launch(kv_attend_kernel<64, false>, grid, dim3(128), 0, s, c, b, a);
+    return bf16 ? ka_launch<128, true>(c, tk, tv, b, a, p, num_sms, s)
+                : ka_launch<128, false>(c, tk, tv, b, a, p, num_sms, s);
+  return bf16 ? ka_launch<64, true>(c, tk, tv, b, a, p, num_sms, s)
+              : ka_launch<64, false>(c, tk, tv, b, a, p, num_sms, s);
 }
 
 }  // namespace moe
