@@ -59,12 +59,19 @@ struct KaCut {
   int item, head, last, valid;
 };
 
+// Kinds of units: rows of a unit, shares an SM.
+constexpr int kPair = 0, kSingle = 1, kFew = 2, kKinds = 3;
+constexpr int kFewRows = 64;
+// What beginning and ending a unit costs, in tiles of its kind.
+__host__ __device__ constexpr int kind_extra(int k) { return k == kFew ? 2 : 1; }
+__host__ __device__ constexpr int kind_rows(int k) { return k == kPair ? 2 * kTile : k == kSingle ? kTile : kFewRows; }
+__host__ __device__ constexpr int kind_shares(int k) { return k == kSingle ? 2 : 1; }
+
 struct KaWs {
-  size_t start[2], cut[2], list[2], pre[2], o[2], ml[2], total;
-  int cap[2];
+  size_t start[kKinds], cut[kKinds], list[kKinds], pre[kKinds], o[kKinds], ml[kKinds], total;
+  int cap[kKinds];
 };
 
-// [0] pairs: num_sms shares of 256 rows; [1] singles: 2 * num_sms shares of 128 rows
 static KaWs ka_ws(const KvView& c, int heads, int rows, int n, int num_sms) {
   KaWs w{};
   size_t o = 0;
@@ -75,10 +82,11 @@ static KaWs ka_ws(const KvView& c, int heads, int rows, int n, int num_sms) {
   };
   const int64_t packed = static_cast<int64_t>(rows) * (heads / c.heads);
   w.cap[0] = packed > kTile ? static_cast<int>(packed / (2 * kTile) + std::min<int64_t>(n, packed / kTile)) : 0;
-  w.cap[1] = n;
-  for (int k = 0; k < 2; ++k) {
-    const size_t shares = static_cast<size_t>(num_sms) * (k + 1);
-    const size_t prow = 2 * shares * (w.cap[k] ? kTile * (2 - k) : 0);
+  w.cap[1] = packed > kFewRows ? n : 0;
+  w.cap[2] = n;
+  for (int k = 0; k < kKinds; ++k) {
+    const size_t shares = static_cast<size_t>(num_sms) * kind_shares(k);
+    const size_t prow = 2 * shares * (w.cap[k] ? kind_rows(k) : 0);
     w.start[k] = take(shares * sizeof(KaStart));
     w.cut[k] = take(shares * sizeof(KaCut));
     w.list[k] = take(static_cast<size_t>(w.cap[k]) * sizeof(KaUnit));
@@ -104,8 +112,8 @@ struct KaList {
   float2* ml;  // running maximum (base 2, scaled) and sum of the same rows
 };
 struct KaPtrs {
-  KaList pair, single;
-  MOE_DEV KaList kind(int k) const { return k ? single : pair; }
+  KaList pair, single, few;
+  MOE_DEV KaList kind(int k) const { return k == kPair ? pair : k == kSingle ? single : few; }
 };
 
 // ------------------------------------------------------------------ plan
@@ -147,13 +155,12 @@ MOE_DEV int key_tiles(int base, int last_token) {
 // the units that the shares cut.  Two dependent loads and three scans: about 3 us.
 __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const KvBatch b,
                                                          const int group, const int num_sms,
-                                                         const KaPtrs w, const int cap0,
-                                                         const int min0, const int min1) {
+                                                         const KaPtrs w, const int cap0) {
   pdl_enter();
-  __shared__ long long spre[2][kPlanSmem + 1];
+  __shared__ long long spre[kKinds][kPlanSmem + 1];
   const int tid = threadIdx.x, lane = tid & 31;
   // (1)
-  int n_list[2] = {0, 0};
+  int n_list[kKinds] = {0, 0, 0};
   for (int i0 = 0; i0 < b.n; i0 += kPlanT) {
     const int i = i0 + tid;
     int seq = -1, row0 = 0, m = 0, len = 0;
@@ -179,14 +186,16 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
     }
     const int rows = m * group;
     const int rem = rows & (2 * kTile - 1);
-    const int na = rows / (2 * kTile) + (rem > kTile ? 1 : 0), nb = rem > 0 && rem <= kTile ? 1 : 0;
+    const int na = rows / (2 * kTile) + (rem > kTile ? 1 : 0);
+    const bool single = rem > kFewRows && rem <= kTile, few = rem > 0 && rem <= kFewRows;
+    // pairs in the low 40 bits, the other two (at most one a thread) above
     long long total;
-    const long long mine = na | (static_cast<long long>(nb) << 32);
+    const long long mine = na | (single ? 1ll << 40 : 0) | (few ? 1ll << 52 : 0);
     const long long before = plan_scan(mine, &total) - mine;
-    const int at_a = n_list[0] + static_cast<int>(before & 0xffffffff);
-    const int at_b = n_list[1] + static_cast<int>(before >> 32);
-    if (nb)
-      w.single.list[at_b] = KaUnit{seq, row0, rows - rem, rem, len - m, len, key_tiles(len - m, m - 1), 0};
+    const int at_a = n_list[0] + static_cast<int>(before & 0xffffffffff);
+    const KaUnit rest{seq, row0, rows - rem, rem, len - m, len, key_tiles(len - m, m - 1), 0};
+    if (single) w.single.list[n_list[1] + (static_cast<int>(before >> 40) & 0xfff)] = rest;
+    if (few) w.few.list[n_list[2] + static_cast<int>(before >> 52)] = rest;
     // pairs of one entry: the warp's lanes side by side
     for (uint32_t todo = __ballot_sync(0xffffffffu, na > 0); todo; todo &= todo - 1) {
       const int l = __ffs(todo) - 1;
@@ -199,21 +208,23 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
         w.pair.list[at + j] = KaUnit{sq, q0, r0, r1 - r0, ln - mm, ln, key_tiles(ln - mm, (r1 - 1) / group), 0};
       }
     }
-    n_list[0] += static_cast<int>(total & 0xffffffff);
-    n_list[1] += static_cast<int>(total >> 32);
+    n_list[0] += static_cast<int>(total & 0xffffffffff);
+    n_list[1] += static_cast<int>(total >> 40) & 0xfff;
+    n_list[2] += static_cast<int>(total >> 52);
   }
   n_list[0] = min(n_list[0], cap0);
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
+  for (int k = 0; k < kKinds; ++k) {
     // (2)
     const int n = n_list[k];
     const KaList w_k = w.kind(k);
+    const int extra = kind_extra(k);
     long long* pre = n <= kPlanSmem ? spre[k] : w_k.pre;
     long long work = 0;
     for (int i0 = 0; i0 < n; i0 += kPlanT) {
       const int i = i0 + tid;
-      const long long t = i < n ? static_cast<long long>(w_k.list[i].tiles) * c.heads : 0;
+      const long long t = i < n ? static_cast<long long>(w_k.list[i].tiles + extra) * c.heads : 0;
       long long total;
       const long long incl = work + plan_scan(t, &total);
       if (i < n) pre[i + 1] = incl;
@@ -222,29 +233,40 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
     if (tid == 0) pre[0] = 0;
     __syncthreads();
     // (3)
-    const int shares = num_sms * (k + 1);
-    long long per = (work + shares - 1) / shares;
-    per = max(per, static_cast<long long>(k ? min1 : min0));
+    const int shares = num_sms * kind_shares(k);
+    const long long per = max((work + shares - 1) / shares, 1ll);
+    // where the cost w0 lies: a unit's extra comes before its tiles, so a border inside
+    // it leaves the unit whole
+    auto locate = [&](long long w0, KaStart& st) -> long long {  // -> tiles before it
+      int lo = 0, hi = n;  // pre[lo] <= w0 < pre[hi]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (pre[mid] <= w0) lo = mid;
+        else hi = mid;
+      }
+      const int cost = static_cast<int>((pre[lo + 1] - pre[lo]) / c.heads);
+      const long long r = w0 - pre[lo];
+      st.item = lo;
+      st.head = static_cast<int>(r / cost);
+      st.tile = max(static_cast<int>(r - static_cast<long long>(st.head) * cost) - extra, 0);
+      return pre[lo] + static_cast<long long>(st.head) * (cost - extra) + st.tile -
+             static_cast<long long>(lo) * extra * c.heads;
+    };
+    const long long tiles_all = work - static_cast<long long>(n) * extra * c.heads;
     for (int s = tid; s <= shares; s += kPlanT) {
-      const long long w0 = s * per;
-      KaStart st{0, 0, 0, 0};
+      const long long w0 = s * per, w1 = w0 + per;
+      KaStart st{0, 0, 0, 0}, end;
       KaCut cut{0, 0, 0, 0};
       if (w0 < work) {
-        int lo = 0, hi = n;  // pre[lo] <= w0 < pre[hi]
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) >> 1;
-          if (pre[mid] <= w0) lo = mid;
-          else hi = mid;
+        const long long t0 = locate(w0, st);
+        st.count = static_cast<int>((w1 < work ? locate(w1, end) : tiles_all) - t0);
+        if (s > 0 && st.tile > 0) {
+          const int cost = static_cast<int>((pre[st.item + 1] - pre[st.item]) / c.heads);
+          const long long u0 = pre[st.item] + static_cast<long long>(st.head) * cost;  // the unit's cost begins
+          // cut by this border first if its first tile lies in the share before
+          if (u0 + extra >= w0 - per)
+            cut = KaCut{st.item, st.head, static_cast<int>((u0 + cost - 1) / per), 1};
         }
-        const int tiles = static_cast<int>((pre[lo + 1] - pre[lo]) / c.heads);
-        const long long r = w0 - pre[lo];
-        st.item = lo;
-        st.head = static_cast<int>(r / tiles);
-        st.tile = static_cast<int>(r - static_cast<long long>(st.head) * tiles);
-        st.count = static_cast<int>(min(per, work - w0));
-        const long long u0 = w0 - st.tile;
-        if (s > 0 && st.tile > 0 && u0 >= (s - 1) * per)
-          cut = KaCut{lo, st.head, static_cast<int>((u0 + tiles - 1) / per), 1};
       }
       if (s < shares) w_k.start[s] = st;
       if (s > 0) w_k.cut[s - 1] = cut;
@@ -259,7 +281,8 @@ struct KaCfg {
   static constexpr int kStage = kTile * HD * 2;  // one K or V tile
   static constexpr int kStages = HD == 128 ? 5 : 8;
   static constexpr int kLoads = HD / 64;         // 64-dim blocks of a tile
-  static constexpr size_t kSmem = 1024 + 2 * kQ + kStages * kStage + 512;
+  // barriers, and the 8 warps' (max, sum) of 16 rows each
+  static constexpr size_t kSmem = 1024 + 2 * kQ + kStages * kStage + 512 + 1024;
 };
 static_assert(KaCfg<128>::kSmem <= 227 * 1024 && KaCfg<64>::kSmem > 114 * 1024,
               "one CTA, and with it all of TMEM, an SM");
@@ -367,6 +390,18 @@ struct KaPages {
   }
 };
 
+// One lane of a converged warp, the same one every time.
+MOE_DEV bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
+}
+// The same value in every lane, known as such to the compiler: the tensor-core
+// instructions take their descriptors from uniform registers, and values that it must
+// first move there cost more issue time than the products take.
+MOE_DEV uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 // The whole warp waits and takes the same way out.
 MOE_DEV bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag));
@@ -418,6 +453,302 @@ MOE_DEV void load_s(uint32_t taddr, float (&sc)[kTile]) {
   tmem_landed(sc, kTile);
 }
 
+// ------------------------------------------------------------------ few rows
+// Units of at most 64 rows (decode steps).  They are bound by the reading of K and V, and
+// a tcgen05.mma of 128 rows would spend its time, and its softmax warps theirs, on padding.
+// So eight warps share each 128-key tile: MT 16-row blocks times 8 / MT slices of 16 * MT
+// keys, mma.sync m16n8k16 from the same swizzled tiles.  A warp keeps its own running
+// maximum, sum and O (fp32, registers) over its slices: no exchange inside a unit, one
+// join of the slices through shared memory (the idle Q tiles) at its end, while the next
+// tiles load.
+MOE_DEV void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+MOE_DEV void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <bool BF16>
+MOE_DEV void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (BF16) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  } else {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+}
+
+// Two fp32 operations in one instruction.
+MOE_DEV uint64_t pair_of(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+MOE_DEV float2 split_pair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+MOE_DEV uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+MOE_DEV uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+template <int HD, bool BF16>
+struct KaFew {
+  using C = KaCfg<HD>;
+  const KvView& c;
+  const KvAttend& a;
+  const KaPtrs& w;
+  const int group;
+  const float scale_log2;
+  uint8_t *sQ, *sR;
+  uint64_t *full, *empty, *joined;
+  float2* s_ml;
+  volatile int* abort_flag;
+  int n = 0;      // ring tiles taken
+  int units = 0;  // joins so far
+  uint32_t next_q[HD / 16][4];  // Q fragments of the next unit
+  int next_seen[2];             // tokens that its rows see
+
+  // Q fragments of rows mi * 16 + g and + 8 of the cursor's unit, and the tokens they see
+  MOE_DEV void fetch_q(const KaCursor& x) {
+    const KaUnit& u = x.u;
+    const int warp = threadIdx.x >> 5, g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+    const int mi = u.rows <= 16 ? 0 : u.rows <= 32 ? warp >> 2 : warp >> 1;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int pr = mi * 16 + g + 8 * r;
+      const bool valid = pr < u.rows;
+      const int packed = u.r0 + (valid ? pr : 0);
+      const int tok = packed / group, hg = packed - tok * group;
+      next_seen[r] = valid ? max(min(u.base + tok + 1, u.len), 0) : 0;
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(
+          static_cast<const __half*>(a.q) + (static_cast<long long>(u.row0) + tok) * a.qs[0] +
+          (static_cast<long long>(x.head) * group + hg) * a.qs[1]);
+#pragma unroll
+      for (int k = 0; k < HD / 16; ++k) {
+        next_q[k][r] = valid ? src[k * 8 + t] : 0u;
+        next_q[k][r + 2] = valid ? src[k * 8 + t + 4] : 0u;
+      }
+    }
+  }
+
+  // One unit, or this share's piece of it; false when a wait ran out.
+  template <int MT>
+  MOE_DEV bool unit(KaCursor& x, int share) {
+    constexpr float shift = BF16 ? 0.f : 7.f;  // as in the softmax warpgroups
+    constexpr int kSlices = 8 / MT;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int mi = warp / kSlices, slice = warp - mi * kSlices;
+    const int g = lane >> 2, t = lane & 3;
+    const KaUnit u = x.u;
+    const int head = x.head;
+    const bool cut_front = x.tile > 0;
+    uint32_t q[HD / 16][4];
+#pragma unroll
+    for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[k][e] = next_q[k][e];
+    const int seen[2] = {next_seen[0], next_seen[1]};
+    float o[HD / 8][4];
+#pragma unroll
+    for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    bool whole = true;
+    // lane addresses inside a 16-key group: K rows (lane >> 4) * 8 + (lane & 7), chunk
+    // (lane >> 3 & 1); V rows (lane >> 3 & 1) * 8 + (lane & 7), chunk lane >> 4
+    const int krow = ((lane >> 4) << 3) + (lane & 7), vrow = (lane & 15);
+    for (bool ends = false; !ends;) {
+      ends = x.ends_unit();
+      const int key0 = x.tile * kTile;
+      if (ends) whole = x.tile + 1 == u.tiles;
+      x.next();
+      if (ends && x.left > 0) fetch_q(x);  // lands while this unit ends
+      // S = Q K^T of this warp's 16 * MT keys
+      int st = n % C::kStages;
+      if (!warp_wait(&full[st], (n / C::kStages) & 1, abort_flag)) return false;
+      uint32_t tile = smem_u32(sR) + st * C::kStage;
+      float sc[MT][2][4];
+#pragma unroll
+      for (int kg = 0; kg < MT; ++kg) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) sc[kg][i][0] = sc[kg][i][1] = sc[kg][i][2] = sc[kg][i][3] = 0.f;
+        const int row = (slice * MT + kg) * 16 + krow;
+        const uint32_t base = tile + row * 128;
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+          const int chunk = (k & 3) * 2 + ((lane >> 3) & 1);
+          uint32_t b[4];
+          ldsm4(base + (k >> 2) * 16384 + ((chunk ^ (row & 7)) << 4), b);
+          mma16816<BF16>(sc[kg][0], q[k], b[0], b[1]);
+          mma16816<BF16>(sc[kg][1], q[k], b[2], b[3]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+      ++n;
+      // softmax of the slice
+      const int col0 = key0 + slice * MT * 16 + 2 * t;
+      if (__any_sync(0xffffffffu, min(seen[0], seen[1]) < key0 + (slice + 1) * MT * 16)) {
+#pragma unroll
+        for (int kg = 0; kg < MT; ++kg)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (col0 + kg * 16 + i * 8 + (e & 1) >= seen[e >> 1]) sc[kg][i][e] = -INFINITY;
+      }
+      float alpha[2];
+      bool grow = false;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int kg = 0; kg < MT; ++kg)
+          top = fmaxf(top, fmaxf(fmaxf(sc[kg][0][2 * r], sc[kg][0][2 * r + 1]),
+                                 fmaxf(sc[kg][1][2 * r], sc[kg][1][2 * r + 1])));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) * scale_log2;
+        alpha[r] = 1.f;
+        if (top - m[r] > 8.f) {
+          alpha[r] = exp2f(m[r] - top);
+          m[r] = top;
+          grow = true;
+        }
+        const float ref = m[r] == -INFINITY ? 0.f : m[r] - shift;
+        float sum = 0.f;
+#pragma unroll
+        for (int kg = 0; kg < MT; ++kg)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 2 * r; e < 2 * r + 2; ++e) {
+              sc[kg][i][e] = exp2_ftz(fmaf(sc[kg][i][e], scale_log2, -ref));
+              sum += sc[kg][i][e];
+            }
+        l[r] = l[r] * alpha[r] + sum;
+      }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i) {
+          o[i][0] *= alpha[0];
+          o[i][1] *= alpha[0];
+          o[i][2] *= alpha[1];
+          o[i][3] *= alpha[1];
+        }
+      }
+      // O += P V
+      st = n % C::kStages;
+      if (!warp_wait(&full[st], (n / C::kStages) & 1, abort_flag)) return false;
+      tile = smem_u32(sR) + st * C::kStage;
+      if (u.len - key0 < (slice + 1) * MT * 16) {
+        // keys past the sequence's end: P is zero there, V must be (0 * NaN is not)
+        for (int row = max(u.len - key0, slice * MT * 16); row < (slice + 1) * MT * 16; ++row)
+          if (lane < HD / 8)
+            *reinterpret_cast<uint4*>(sR + st * C::kStage + (lane >> 3) * 16384 + row * 128 + (lane & 7) * 16) =
+                make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+#pragma unroll
+      for (int kg = 0; kg < MT; ++kg) {
+        const uint32_t p[4] = {pack2<BF16>(sc[kg][0][0], sc[kg][0][1]), pack2<BF16>(sc[kg][0][2], sc[kg][0][3]),
+                               pack2<BF16>(sc[kg][1][0], sc[kg][1][1]), pack2<BF16>(sc[kg][1][2], sc[kg][1][3])};
+        const int row = (slice * MT + kg) * 16 + vrow;
+        const uint32_t base = tile + row * 128;
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) {
+          const int chunk = (i & 3) * 2 + (lane >> 4);
+          uint32_t b[4];
+          ldsm4_t(base + (i >> 2) * 16384 + ((chunk ^ (row & 7)) << 4), b);
+          mma16816<BF16>(o[2 * i], p, b[0], b[1]);
+          mma16816<BF16>(o[2 * i + 1], p, b[2], b[3]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+      ++n;
+    }
+    // join the slices: [8 warps][16 rows][HD] fp32, columns in pairs, pair p of row g at
+    // p ^ (g << 2) so that a warp's stores meet no bank twice
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&joined[0]);
+    if (!warp_wait(&joined[0], units & 1, abort_flag)) return false;
+    float* part = reinterpret_cast<float*>(sQ);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float2* dst = reinterpret_cast<float2*>(part + (warp * 16 + g + 8 * r) * HD);
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i) dst[(i * 4 + t) ^ (g << 2)] = make_float2(o[i][2 * r], o[i][2 * r + 1]);
+      float sum = l[r];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      if (t == 0) s_ml[warp * 16 + g + 8 * r] = make_float2(sum > 0.f ? m[r] - shift : -INFINITY, sum);
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&joined[1]);
+    if (!warp_wait(&joined[1], units & 1, abort_flag)) return false;
+    ++units;
+    constexpr int V = HD / 32;
+    for (int pr = warp; pr < u.rows; pr += 8) {
+      const int r = pr & 15, first = (pr >> 4) * kSlices;
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kSlices; ++i) top = fmaxf(top, s_ml[(first + i) * 16 + r].x);
+      float acc[V] = {}, sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < kSlices; ++i) {
+        const float2 ml = s_ml[(first + i) * 16 + r];
+        const float f = ml.y > 0.f ? exp2f(ml.x - top) : 0.f;
+        const float* src = part + ((first + i) * 16 + r) * HD + (((lane * V / 2) ^ ((r & 7) << 2)) << 1);
+        sum += f * ml.y;
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] = fmaf(f, src[e], acc[e]);
+      }
+      const int packed = u.r0 + pr;
+      const int tok = packed / group, hg = packed - tok * group;
+      const long long row = static_cast<long long>(u.row0) + tok;
+      const int h = head * group + hg;
+      if (whole && !cut_front) {
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<__half*>(a.out) + row * a.os[0] + h * a.os[1]) + lane * (V / 2);
+#pragma unroll
+        for (int e = 0; e < V / 2; ++e) dst[e] = pack2<BF16>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+        if (a.lse && lane == 0)
+          a.lse[row * a.ls[0] + h * a.ls[1]] = sum > 0.f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+      } else {
+        const long long slot = (2ll * share + (cut_front ? 0 : 1)) * kFewRows + pr;
+        float* dst = w.few.o + slot * HD + lane * V;
+#pragma unroll
+        for (int e = 0; e < V; ++e) dst[e] = acc[e];
+        if (lane == 0) w.few.ml[slot] = make_float2(top, sum);
+      }
+    }
+    return true;
+  }
+};
+
+// 16 TMEM columns of a row, not waited for.
+MOE_DEV void tmem_st16_start(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+
 template <int HD, bool BF16>
 __global__ void __launch_bounds__(kAttThreads, 1)
     kv_attend_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
@@ -435,8 +766,13 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   uint64_t* s_full = q_full + 2;           // [2] S of a tile done (and every MMA before it)
   uint64_t* p_full = q_full + 4;           // [2] P of a tile written
   uint64_t* o_done = q_full + 6;           // [2] P V of a tile done
-  uint64_t* mma_done = q_full + 8;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 9);
+  uint64_t* p_half = q_full + 8;           // [2] its first 64 keys
+  uint64_t* mma_done = q_full + 10;
+  uint64_t* few_full = q_full + 11;           // [kStages] the ring in the few-rows phase
+  uint64_t* few_empty = few_full + C::kStages;  // [kStages]
+  uint64_t* joined = few_empty + C::kStages;  // [2] 8 warps: partials may be written, are written
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(joined + 2);
+  float2* s_ml = reinterpret_cast<float2*>(bars + 64);  // [8][16]
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -444,11 +780,15 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     for (int i = 0; i < C::kStages; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
+      mbar_init(&few_full[i], 1);
+      mbar_init(&few_empty[i], 8);
     }
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&joined[i], 8);
       mbar_init(&q_full[i], 4);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
+      mbar_init(&p_half[i], 4);
       mbar_init(&o_done[i], 1);
     }
     mbar_init(mma_done, 1);
@@ -475,16 +815,17 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     // ------------------------------------------------------------ K / V tiles
     int n = 0;  // tiles put into the ring so far
     bool ok = true;
+    uint64_t *fullb = full, *emptyb = empty;
     auto put = [&](const KaUnit& u, int head, int tile, KaPages& pg, bool val) {
       const int st = n % C::kStages;
-      if (!warp_wait(&empty[st], ((n / C::kStages) & 1) ^ 1, abort_flag)) {
+      if (!warp_wait(&emptyb[st], ((n / C::kStages) & 1) ^ 1, abort_flag)) {
         ok = false;
         return;
       }
       const int key0 = tile * kTile;
       const int blk = key0 >> c.page_shift;
       pg.at(c, u, blk);
-      if (lane == 0) mbar_arrive_expect_tx(&full[st], C::kStage);
+      if (lane == 0) mbar_arrive_expect_tx(&fullb[st], C::kStage);
       __syncwarp();
       const int per = max(kTile >> c.page_shift, 1);  // pages of a tile
       const int p = lane / C::kLoads, kb = lane - p * C::kLoads;
@@ -496,13 +837,13 @@ __global__ void __launch_bounds__(kAttThreads, 1)
           id = c.pages;
         }
         tma_load_5d(smem_u32(sR + st * C::kStage) + kb * 16384 + p * c.page * 128, val ? &tv : &tk, kb * 64,
-                    key0 & (c.page - 1), head, id, a.layer, &full[st]);
+                    key0 & (c.page - 1), head, id, a.layer, &fullb[st]);
       }
       ++n;
     };
     KaCursor x;
     KaPages px;
-    x.init(w, 0, cta, c.heads);
+    x.init(w, kPair, cta, c.heads);
     while (ok && x.left > 0) {
       put(x.u, x.head, x.tile, px, false);
       if (ok) put(x.u, x.head, x.tile, px, true);
@@ -510,8 +851,8 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     }
     KaCursor y;
     KaPages py;
-    x.init(w, 1, cta, c.heads);
-    y.init(w, 1, cta + ctas, c.heads);
+    x.init(w, kSingle, cta, c.heads);
+    y.init(w, kSingle, cta + ctas, c.heads);
     if (ok && x.left > 0) put(x.u, x.head, x.tile, px, false);
     if (ok && y.left > 0) put(y.u, y.head, y.tile, py, false);
     while (ok && (x.left > 0 || y.left > 0)) {
@@ -526,18 +867,33 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         if (ok && y.left > 0) put(y.u, y.head, y.tile, py, false);
       }
     }
+    // few rows: the same stages with barriers of their own, once the MMAs have let them go
+    const int n_mma = n;
+    for (int j = max(n - C::kStages, 0); ok && j < n; ++j)
+      ok = warp_wait(&empty[j % C::kStages], (j / C::kStages) & 1, abort_flag);
+    n = 0;
+    fullb = few_full;
+    emptyb = few_empty;
+    x.init(w, kFew, cta, c.heads);
+    while (ok && x.left > 0) {
+      put(x.u, x.head, x.tile, px, false);
+      if (ok) put(x.u, x.head, x.tile, px, true);
+      x.next();
+    }
     if (!ok) {
       *abort_flag = 1;
       if (lane == 0) record_error(c.err, DEV_TIMEOUT_EMPTY);
     }
     // every copy must land before the CTA exits
-    for (int j = n - 1; j >= 0 && j >= n - C::kStages; --j)
+    for (int j = n_mma - 1; j >= 0 && j >= n_mma - C::kStages; --j)
       mbar_wait_drain(&full[j % C::kStages], (j / C::kStages) & 1);
+    for (int j = n - 1; j >= 0 && j >= n - C::kStages; --j)
+      mbar_wait_drain(&few_full[j % C::kStages], (j / C::kStages) & 1);
   } else if (warp == 9) {
     // ------------------------------------------------------------ MMA issue
     constexpr uint32_t fmt = BF16 ? 1 : 0;
     constexpr uint32_t id_s = ka_idesc(fmt, kTile, 0), id_o = ka_idesc(fmt, HD, 1);
-    const uint32_t aq = smem_u32(sQ), ar = smem_u32(sR);
+    const uint32_t aq = uniform(smem_u32(sQ)), ar = uniform(smem_u32(sR)), tm = uniform(tmem);
     bool ok = true;
     int n = 0;             // ring tiles taken
     int np[2] = {0, 0};    // P tiles taken, by stream
@@ -556,12 +912,12 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         ++nq[s];
       }
       tc_fence_after();
-      if (ok && lane == 0) {
+      const uint64_t dq = sw128_desc(aq + s * C::kQ), dk = sw128_desc(ar + uniform(st) * C::kStage);
+      if (ok && elect_one()) {
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
-          const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-          tc_mma_f16(tmem + s * kTile, sw128_desc(aq + s * C::kQ + off), sw128_desc(ar + st * C::kStage + off),
-                     id_s, k > 0 ? 1u : 0u);
+          const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;  // in the descriptors' units
+          tc_mma_f16(tm + s * kTile, dq + off, dk + off, id_s, k > 0 ? 1u : 0u);
         }
         tc_commit(&s_full[s]);
       }
@@ -580,26 +936,32 @@ __global__ void __launch_bounds__(kAttThreads, 1)
       __syncwarp();
     };
     auto issue_o = [&](int s, int st, bool first) {
-      if (!warp_wait(&p_full[s], np[s] & 1, abort_flag)) ok = false;
-      ++np[s];
-      tc_fence_after();
-      if (ok && lane == 0) {
+      const uint64_t dv = nmajor_desc(ar + uniform(st) * C::kStage);
+      const uint32_t add = uniform(first ? 0u : 1u);
 #pragma unroll
-        for (int k = 0; k < kTile / 16; ++k)
-          tc_mma_f16_ts(tmem + kOCols + s * kTile, tmem + s * kTile + k * 8,
-                        nmajor_desc(ar + st * C::kStage + k * 2048), id_o, (!first || k > 0) ? 1u : 0u);
-        tc_commit(&o_done[s]);
+      for (int half = 0; half < 2; ++half) {
+        if (ok && !warp_wait(half ? &p_full[s] : &p_half[s], np[s] & 1, abort_flag)) ok = false;
+        tc_fence_after();
+        if (ok && elect_one()) {
+#pragma unroll
+          for (int k = half * 4; k < half * 4 + 4; ++k)
+            tc_mma_f16_ts(tm + kOCols + s * kTile, tm + s * kTile + k * 8, dv + k * (2048 >> 4), id_o,
+                          k > 0 ? 1u : add);
+          if (half) tc_commit(&o_done[s]);
+        }
+        __syncwarp();
       }
-      __syncwarp();
+      ++np[s];
     };
     auto release = [&](int st) {
-      if (ok && lane == 0) tc_commit(&empty[st]);
+      uint64_t* bar = &empty[uniform(st)];
+      if (ok && elect_one()) tc_commit(bar);
       __syncwarp();
     };
     // pairs: both streams read the same K and V tiles.  At a unit's end the next S (which
     // waits for the next Q) comes after both products with V.
     KaCursor x;
-    x.init(w, 0, cta, c.heads);
+    x.init(w, kPair, cta, c.heads);
     if (x.left > 0) {
       int kst = take();
       if (ok) issue_s(0, kst, true);
@@ -638,7 +1000,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     KaCursor y[2];
     bool first[2] = {true, true};
 #pragma unroll
-    for (int s = 0; s < 2; ++s) y[s].init(w, 1, cta + s * ctas, c.heads);
+    for (int s = 0; s < 2; ++s) y[s].init(w, kSingle, cta + s * ctas, c.heads);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       if (ok && y[s].left > 0) {
@@ -670,7 +1032,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
       *abort_flag = 1;
       if (lane == 0) record_error(c.err, DEV_TIMEOUT_FULL);
     }
-    if (lane == 0) {
+    if (elect_one()) {
       tc_commit(mma_done);  // no MMA may still write TMEM when it is released
       mbar_wait_drain(mma_done, 0);
     }
@@ -715,7 +1077,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
       if (lane == 0) mbar_arrive(&q_full[s]);
     };
 #pragma unroll 1
-    for (int kind = 0; kind < 2 && ok; ++kind) {
+    for (int kind = kPair; kind <= kSingle && ok; ++kind) {
       const int share = kind ? cta + s * ctas : cta;
       const int part = kind ? 0 : s;  // the unit's rows of this warpgroup: part * 128 ..
       KaCursor x;
@@ -769,14 +1131,6 @@ __global__ void __launch_bounds__(kAttThreads, 1)
               alpha = exp2f(m - top);
               m = top;
             }
-            const float ref = m == -INFINITY ? 0.f : m - shift;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int j = 0; j < kTile; ++j) {
-              sc[j] = exp2_ftz(fmaf(sc[j], scale_log2, -ref));
-              sum[j & 3] += sc[j];
-            }
-            l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
             if (!first && __any_sync(0xffffffffu, grow)) {
               // s_full of this tile also says that O is complete up to the one before
 #pragma unroll
@@ -788,18 +1142,47 @@ __global__ void __launch_bounds__(kAttThreads, 1)
                 tmem_st16(t_o + i * 16, o);
               }
             }
+            // P in four chunks of 32 keys: the conversions and TMEM stores of one run
+            // under the exponentials of the next, and the first 64 keys are handed to
+            // the MMA warp while the rest is computed
+            const float ref = m == -INFINITY ? 0.f : m - shift;
+            const uint64_t scale2 = pair_of(scale_log2, scale_log2), nref2 = pair_of(-ref, -ref);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              uint32_t pk[32];
+            for (int i = 0; i < 4; ++i) {
+              uint32_t pk[16];
 #pragma unroll
-              for (int j = 0; j < 32; ++j) pk[j] = pack2<BF16>(sc[i * 64 + 2 * j], sc[i * 64 + 2 * j + 1]);
-              tmem_st32_nowait(t_s + i * 32, pk);
+              for (int j = 0; j < 16; ++j) {
+                float* e = sc + i * 32 + 2 * j;
+                const float2 x2 = split_pair(fma_pair(pair_of(e[0], e[1]), scale2, nref2));
+                e[0] = exp2_ftz(x2.x);
+                e[1] = exp2_ftz(x2.y);
+                pk[j] = pack2<BF16>(e[0], e[1]);
+              }
+              if (i == 2) {
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_half[s]);
+              }
+              tmem_st16_start(t_s + i * 16, pk);
             }
             tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[s]);
+            // the row sum, off the path to the next product
+            uint64_t sum[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < kTile / 2; ++j) sum[j & 3] = add_pair(sum[j & 3], pair_of(sc[2 * j], sc[2 * j + 1]));
+            const float2 sum2 = split_pair(add_pair(add_pair(sum[0], sum[1]), add_pair(sum[2], sum[3])));
+            l = l * alpha + (sum2.x + sum2.y);
+          } else {
+            tc_fence_before();
+            if (lane == 0) {
+              mbar_arrive(&p_half[s]);
+              mbar_arrive(&p_full[s]);
+            }
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[s]);
           if (load_next) q_ready();
           ++nt;
         }
@@ -833,7 +1216,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
                   l > 0.f ? (m - shift + log2f(l)) * 0.6931471805599453f : -INFINITY;
           } else {
             // a piece: unnormalised, to the share's slot 0 (its first unit) or 1 (its last)
-            const int per = kind ? kTile : 2 * kTile;
+            const int per = kind_rows(kind);
             const long long slot = (2ll * share + (cut_front ? 0 : 1)) * per + pr;
             float4* dst = reinterpret_cast<float4*>(w.kind(kind).o + slot * HD);
 #pragma unroll
@@ -851,6 +1234,17 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         }
         tc_fence_before();  // O is read: the next unit's first product may overwrite it
         cut_front = false;
+      }
+    }
+    // few rows: all eight warps on one unit
+    if (ok) {
+      KaFew<HD, BF16> f{c, a, w, group, scale_log2, sQ, sR, few_full, few_empty, joined, s_ml, abort_flag};
+      KaCursor x;
+      x.init(w, kFew, cta, c.heads);
+      if (x.left > 0) f.fetch_q(x);
+      while (ok && x.left > 0) {
+        const int rows = x.u.rows;
+        ok = rows <= 16 ? f.template unit<1>(x, cta) : rows <= 32 ? f.template unit<2>(x, cta) : f.template unit<4>(x, cta);
       }
     }
     if (!ok) {
@@ -876,14 +1270,14 @@ __global__ void __launch_bounds__(256) kv_merge_kernel(const KvAttend a, const K
                                                        const int num_sms) {
   pdl_enter();
   constexpr int V = HD / 32;
-  const int kind = static_cast<int>(blockIdx.x) >= num_sms ? 1 : 0;
-  const int share = blockIdx.x - kind * num_sms;
+  int kind = kPair, share = blockIdx.x;
+  while (share >= num_sms * kind_shares(kind)) share -= num_sms * kind_shares(kind++);
   const KaList wk = w.kind(kind);
   const int4 cut = *reinterpret_cast<const int4*>(wk.cut + share);
   if (!cut.w) return;
   const KaUnit u = wk.list[cut.x];
   const int lane = threadIdx.x & 31;
-  const int per = kind ? kTile : 2 * kTile;
+  const int per = kind_rows(kind);
   for (int pr = blockIdx.y * 8 + (threadIdx.x >> 5); pr < u.rows; pr += gridDim.y * 8) {
     float top = -INFINITY;
     for (int p = share + lane; p <= cut.z; p += 32)
@@ -930,8 +1324,8 @@ static cudaError_t ka_launch(const KvView& c, const CUtensorMap& tk, const CUten
   const int group = a.heads / c.heads;
   const KaWs l = ka_ws(c, a.heads, b.rows, b.n, num_sms);
   KaPtrs w{};
-  for (int k = 0; k < 2; ++k) {
-    KaList& d = k ? w.single : w.pair;
+  for (int k = 0; k < kKinds; ++k) {
+    KaList& d = k == kPair ? w.pair : k == kSingle ? w.single : w.few;
     d.start = reinterpret_cast<KaStart*>(ws + l.start[k]);
     d.cut = reinterpret_cast<KaCut*>(ws + l.cut[k]);
     d.list = reinterpret_cast<KaUnit*>(ws + l.list[k]);
@@ -950,12 +1344,12 @@ static cudaError_t ka_launch(const KvView& c, const CUtensorMap& tk, const CUten
     if (st != cudaSuccess) return st;
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
-  MOE_PDL(kv_plan_kernel, dim3(1), dim3(kPlanT), 0, s, c, b, group, num_sms, w, l.cap[0], 1, 1);
+  MOE_PDL(kv_plan_kernel, dim3(1), dim3(kPlanT), 0, s, c, b, group, num_sms, w, l.cap[0]);
   MOE_PDL(kv_attend_kernel<HD, BF16>, dim3(num_sms), dim3(kAttThreads), smem, s, tk, tv, c, a, w, group,
           static_cast<float>(a.scale * 1.4426950408889634));
   const int64_t packed = static_cast<int64_t>(b.rows) * group;
   const int chunks = static_cast<int>(std::min<int64_t>((packed + 7) / 8, packed > kTile ? 16 : 8));
-  MOE_PDL(kv_merge_kernel<HD, BF16>, dim3(num_sms * 3, chunks), dim3(256), 0, s, a, w, group, num_sms);
+  MOE_PDL(kv_merge_kernel<HD, BF16>, dim3(num_sms * 4, chunks), dim3(256), 0, s, a, w, group, num_sms);
   return cudaSuccess;
 }
 
