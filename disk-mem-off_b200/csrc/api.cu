@@ -80,7 +80,7 @@ bool make_tmap_2d(CUtensorMap* map, const void* base, bool int8, uint64_t inner,
 }
 
 // One layer's pages of a K or V pool as (dim, row, head, page, layer): a box is 64 dims
-// (one 128-byte swizzle atom) by the rows of a page, at most a tile's 128.
+// (one 128-byte swizzle atom) by the rows of a page, at most 64.
 bool make_tmap_pool(CUtensorMap* map, const void* base, bool bf16, const KvView& c,
                     const int64_t (&strides)[4], std::string* err) {
   auto fn = get_encode_fn();
@@ -96,7 +96,7 @@ bool make_tmap_pool(CUtensorMap* map, const void* base, bool bf16, const KvView&
     // the stride of a dimension of one entry is never used, but has to encode
     str[i] = sizes[i] > 1 ? static_cast<cuuint64_t>(strides[3 - i]) : static_cast<cuuint64_t>(c.hd) * 2;
   }
-  cuuint32_t box[5] = {64, static_cast<cuuint32_t>(c.page < 128 ? c.page : 128), 1, 1, 1};
+  cuuint32_t box[5] = {64, static_cast<cuuint32_t>(c.page < 64 ? c.page : 64), 1, 1, 1};
   cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   const CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
                         const_cast<void*>(base), dims, str, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,

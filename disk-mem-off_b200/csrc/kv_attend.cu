@@ -63,9 +63,10 @@ struct KaCut {
 constexpr int kPair = 0, kSingle = 1, kFew = 2, kKinds = 3;
 constexpr int kFewRows = 64;
 // What beginning and ending a unit costs, in tiles of its kind.
-__host__ __device__ constexpr int kind_extra(int k) { return k == kFew ? 2 : 1; }
+__host__ __device__ constexpr int kind_extra(int k) { return k == kFew ? 3 : 1; }
 __host__ __device__ constexpr int kind_rows(int k) { return k == kPair ? 2 * kTile : k == kSingle ? kTile : kFewRows; }
-__host__ __device__ constexpr int kind_shares(int k) { return k == kSingle ? 2 : 1; }
+__host__ __device__ constexpr int kind_shares(int k) { return k == kPair ? 1 : 2; }
+__host__ __device__ constexpr int kind_keys(int k) { return k == kFew ? 64 : kTile; }  // of a tile
 
 struct KaWs {
   size_t start[kKinds], cut[kKinds], list[kKinds], pre[kKinds], o[kKinds], ml[kKinds], total;
@@ -144,11 +145,11 @@ MOE_DEV long long plan_scan(long long v, long long* total) {
   return v + before;
 }
 
-MOE_DEV int key_tiles(int base, int last_token) {
+MOE_DEV int key_tiles(int base, int last_token, int keys) {
   // tokens visible to the unit's last row, at least one tile (rows that see nothing
   // still have to be written); beyond the table they read as zeros and are masked
   const long long vis = static_cast<long long>(max(base, 0)) + last_token + 1;
-  return static_cast<int>((vis + kTile - 1) / kTile);
+  return static_cast<int>((vis + keys - 1) / keys);
 }
 
 // (1) entries -> units, (2) prefix sums of their tiles, (3) each share's first tile and
@@ -193,7 +194,8 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
     const long long mine = na | (single ? 1ll << 40 : 0) | (few ? 1ll << 52 : 0);
     const long long before = plan_scan(mine, &total) - mine;
     const int at_a = n_list[0] + static_cast<int>(before & 0xffffffffff);
-    const KaUnit rest{seq, row0, rows - rem, rem, len - m, len, key_tiles(len - m, m - 1), 0};
+    const KaUnit rest{seq, row0, rows - rem, rem, len - m, len,
+                      key_tiles(len - m, m - 1, kind_keys(few ? kFew : kSingle)), 0};
     if (single) w.single.list[n_list[1] + (static_cast<int>(before >> 40) & 0xfff)] = rest;
     if (few) w.few.list[n_list[2] + static_cast<int>(before >> 52)] = rest;
     // pairs of one entry: the warp's lanes side by side
@@ -205,7 +207,7 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
       const int mm = __shfl_sync(0xffffffffu, m, l);
       for (int j = lane; j < k && at + j < cap0; j += 32) {
         const int r0 = j * 2 * kTile, r1 = min(r0 + 2 * kTile, rs);
-        w.pair.list[at + j] = KaUnit{sq, q0, r0, r1 - r0, ln - mm, ln, key_tiles(ln - mm, (r1 - 1) / group), 0};
+        w.pair.list[at + j] = KaUnit{sq, q0, r0, r1 - r0, ln - mm, ln, key_tiles(ln - mm, (r1 - 1) / group, kTile), 0};
       }
     }
     n_list[0] += static_cast<int>(total & 0xffffffffff);
@@ -281,8 +283,10 @@ struct KaCfg {
   static constexpr int kStage = kTile * HD * 2;  // one K or V tile
   static constexpr int kStages = HD == 128 ? 5 : 8;
   static constexpr int kLoads = HD / 64;         // 64-dim blocks of a tile
+  static constexpr int kHalf = kStage / 2;       // 64 keys: a tile of the few-row units,
+  static constexpr int kHalves = kStages;        // whose two rings share the same memory
   // barriers, and the 8 warps' (max, sum) of 16 rows each
-  static constexpr size_t kSmem = 1024 + 2 * kQ + kStages * kStage + 512 + 1024;
+  static constexpr size_t kSmem = 1024 + 2 * kQ + kStages * kStage + 640 + 1024;
 };
 static_assert(KaCfg<128>::kSmem <= 227 * 1024 && KaCfg<64>::kSmem > 114 * 1024,
               "one CTA, and with it all of TMEM, an SM");
@@ -390,6 +394,43 @@ struct KaPages {
   }
 };
 
+// A ring of K and V tiles, filled by one warp.
+struct KaRing {
+  const KvView& c;
+  const CUtensorMap &tk, &tv;
+  const int layer;
+  uint64_t *full, *empty;
+  const uint32_t smem;
+  const int stages, keys, bytes, loads;
+  volatile int* abort_flag;
+  // Tile `tile` of the unit's keys or values into the next stage: boxes of up to 64 rows by
+  // 64 dims, a lane each.
+  MOE_DEV bool put(const KaUnit& u, int head, int tile, KaPages& pg, bool val, int& n) {
+    const int lane = threadIdx.x & 31;
+    const int st = n % stages;
+    if (!__all_sync(0xffffffffu, mbar_wait_bounded(&empty[st], ((n / stages) & 1) ^ 1, abort_flag))) return false;
+    const int box = min(c.page, 64);
+    const int p = lane / loads, kb = lane - p * loads;
+    const int key = tile * keys + p * box;
+    pg.at(c, u, (tile * keys) >> c.page_shift);
+    if (lane == 0) mbar_arrive_expect_tx(&full[st], bytes);
+    __syncwarp();
+    const int blk = key >> c.page_shift;
+    int id = __shfl_sync(0xffffffffu, pg.ids, blk & 31);
+    if (p * box < keys) {
+      if (id < 0 || id >= c.pages) {
+        // past the sequence's last page: zeros; before it: a hole in the table
+        if (key < u.len) record_error(c.err, DEV_BAD_PAGE);
+        id = c.pages;
+      }
+      tma_load_5d(smem + st * bytes + kb * (keys * 128) + p * box * 128, val ? &tv : &tk, kb * 64,
+                  key & (c.page - 1), head, id, layer, &full[st]);
+    }
+    ++n;
+    return true;
+  }
+};
+
 // One lane of a converged warp, the same one every time.
 MOE_DEV bool elect_one() {
   uint32_t p;
@@ -456,11 +497,11 @@ MOE_DEV void load_s(uint32_t taddr, float (&sc)[kTile]) {
 // ------------------------------------------------------------------ few rows
 // Units of at most 64 rows (decode steps).  They are bound by the reading of K and V, and
 // a tcgen05.mma of 128 rows would spend its time, and its softmax warps theirs, on padding.
-// So eight warps share each 128-key tile: MT 16-row blocks times 8 / MT slices of 16 * MT
-// keys, mma.sync m16n8k16 from the same swizzled tiles.  A warp keeps its own running
-// maximum, sum and O (fp32, registers) over its slices: no exchange inside a unit, one
-// join of the slices through shared memory (the idle Q tiles) at its end, while the next
-// tiles load.
+// So each warpgroup works alone on 64-key tiles of its own ring: MT 16-row blocks times
+// 4 / MT slices of 16 * MT keys, mma.sync m16n8k16 from the same swizzled tiles.  A warp
+// keeps its own running maximum, sum and O (fp32, registers) over its slices: no exchange
+// inside a unit, one join of the slices through shared memory (the idle Q tile) at its
+// end, while the next tiles load and the other warpgroup computes.
 MOE_DEV void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -512,9 +553,9 @@ struct KaFew {
   const KaPtrs& w;
   const int group;
   const float scale_log2;
-  uint8_t *sQ, *sR;
+  uint8_t *sQ, *sR;  // this warpgroup's Q tile and ring
   uint64_t *full, *empty, *joined;
-  float2* s_ml;
+  float2* s_ml;  // [4][16]
   volatile int* abort_flag;
   int n = 0;      // ring tiles taken
   int units = 0;  // joins so far
@@ -524,8 +565,8 @@ struct KaFew {
   // Q fragments of rows mi * 16 + g and + 8 of the cursor's unit, and the tokens they see
   MOE_DEV void fetch_q(const KaCursor& x) {
     const KaUnit& u = x.u;
-    const int warp = threadIdx.x >> 5, g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
-    const int mi = u.rows <= 16 ? 0 : u.rows <= 32 ? warp >> 2 : warp >> 1;
+    const int warp = (threadIdx.x >> 5) & 3, g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+    const int mi = u.rows <= 16 ? 0 : u.rows <= 32 ? warp >> 1 : warp;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int pr = mi * 16 + g + 8 * r;
@@ -548,9 +589,9 @@ struct KaFew {
   template <int MT>
   MOE_DEV bool unit(KaCursor& x, int share) {
     constexpr float shift = BF16 ? 0.f : 7.f;  // as in the softmax warpgroups
-    constexpr int kSlices = 8 / MT;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int mi = warp / kSlices, slice = warp - mi * kSlices;
+    constexpr int kSlices = 4 / MT, kKeys = 16 * MT;
+    const int warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
+    const int slice = warp % kSlices;  // of 16-row block warp / kSlices
     const int g = lane >> 2, t = lane & 3;
     const KaUnit u = x.u;
     const int head = x.head;
@@ -567,30 +608,27 @@ struct KaFew {
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     bool whole = true;
     // lane addresses inside a 16-key group: K rows (lane >> 4) * 8 + (lane & 7), chunk
-    // (lane >> 3 & 1); V rows (lane >> 3 & 1) * 8 + (lane & 7), chunk lane >> 4
-    const int krow = ((lane >> 4) << 3) + (lane & 7), vrow = (lane & 15);
+    // (lane >> 3 & 1); V rows lane & 15, chunk lane >> 4
+    const int krow = slice * kKeys + ((lane >> 4) << 3) + (lane & 7), vrow = slice * kKeys + (lane & 15);
     for (bool ends = false; !ends;) {
       ends = x.ends_unit();
-      const int key0 = x.tile * kTile;
+      const int key0 = x.tile * 64;
       if (ends) whole = x.tile + 1 == u.tiles;
       x.next();
-      if (ends && x.left > 0) fetch_q(x);  // lands while this unit ends
-      // S = Q K^T of this warp's 16 * MT keys
-      int st = n % C::kStages;
-      if (!warp_wait(&full[st], (n / C::kStages) & 1, abort_flag)) return false;
-      uint32_t tile = smem_u32(sR) + st * C::kStage;
+      // S = Q K^T of this warp's slice
+      int st = n % C::kHalves;
+      if (!warp_wait(&full[st], (n / C::kHalves) & 1, abort_flag)) return false;
+      uint32_t base = smem_u32(sR) + st * C::kHalf + krow * 128;
       float sc[MT][2][4];
 #pragma unroll
       for (int kg = 0; kg < MT; ++kg) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) sc[kg][i][0] = sc[kg][i][1] = sc[kg][i][2] = sc[kg][i][3] = 0.f;
-        const int row = (slice * MT + kg) * 16 + krow;
-        const uint32_t base = tile + row * 128;
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
           const int chunk = (k & 3) * 2 + ((lane >> 3) & 1);
           uint32_t b[4];
-          ldsm4(base + (k >> 2) * 16384 + ((chunk ^ (row & 7)) << 4), b);
+          ldsm4(base + kg * 2048 + (k >> 2) * 8192 + ((chunk ^ (krow & 7)) << 4), b);
           mma16816<BF16>(sc[kg][0], q[k], b[0], b[1]);
           mma16816<BF16>(sc[kg][1], q[k], b[2], b[3]);
         }
@@ -599,8 +637,9 @@ struct KaFew {
       if (lane == 0) mbar_arrive(&empty[st]);
       ++n;
       // softmax of the slice
-      const int col0 = key0 + slice * MT * 16 + 2 * t;
-      if (__any_sync(0xffffffffu, min(seen[0], seen[1]) < key0 + (slice + 1) * MT * 16)) {
+      const int slice_end = key0 + (slice + 1) * kKeys;
+      if (__any_sync(0xffffffffu, min(seen[0], seen[1]) < slice_end)) {
+        const int col0 = key0 + slice * kKeys + 2 * t;
 #pragma unroll
         for (int kg = 0; kg < MT; ++kg)
 #pragma unroll
@@ -622,7 +661,7 @@ struct KaFew {
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) * scale_log2;
         alpha[r] = 1.f;
         if (top - m[r] > 8.f) {
-          alpha[r] = exp2f(m[r] - top);
+          alpha[r] = exp2_ftz(m[r] - top);
           m[r] = top;
           grow = true;
         }
@@ -648,30 +687,29 @@ struct KaFew {
           o[i][3] *= alpha[1];
         }
       }
+      if (ends && x.left > 0) fetch_q(x);  // lands while this unit ends
       // O += P V
-      st = n % C::kStages;
-      if (!warp_wait(&full[st], (n / C::kStages) & 1, abort_flag)) return false;
-      tile = smem_u32(sR) + st * C::kStage;
-      if (u.len - key0 < (slice + 1) * MT * 16) {
+      st = n % C::kHalves;
+      if (!warp_wait(&full[st], (n / C::kHalves) & 1, abort_flag)) return false;
+      if (u.len < slice_end) {
         // keys past the sequence's end: P is zero there, V must be (0 * NaN is not)
-        for (int row = max(u.len - key0, slice * MT * 16); row < (slice + 1) * MT * 16; ++row)
+        for (int row = max(u.len - key0, slice * kKeys); row < (slice + 1) * kKeys; ++row)
           if (lane < HD / 8)
-            *reinterpret_cast<uint4*>(sR + st * C::kStage + (lane >> 3) * 16384 + row * 128 + (lane & 7) * 16) =
+            *reinterpret_cast<uint4*>(sR + st * C::kHalf + (lane >> 3) * 8192 + row * 128 + (lane & 7) * 16) =
                 make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();
         __syncwarp();
       }
+      base = smem_u32(sR) + st * C::kHalf + vrow * 128;
 #pragma unroll
       for (int kg = 0; kg < MT; ++kg) {
         const uint32_t p[4] = {pack2<BF16>(sc[kg][0][0], sc[kg][0][1]), pack2<BF16>(sc[kg][0][2], sc[kg][0][3]),
                                pack2<BF16>(sc[kg][1][0], sc[kg][1][1]), pack2<BF16>(sc[kg][1][2], sc[kg][1][3])};
-        const int row = (slice * MT + kg) * 16 + vrow;
-        const uint32_t base = tile + row * 128;
 #pragma unroll
         for (int i = 0; i < HD / 16; ++i) {
           const int chunk = (i & 3) * 2 + (lane >> 4);
           uint32_t b[4];
-          ldsm4_t(base + (i >> 2) * 16384 + ((chunk ^ (row & 7)) << 4), b);
+          ldsm4_t(base + kg * 2048 + (i >> 2) * 8192 + ((chunk ^ (vrow & 7)) << 4), b);
           mma16816<BF16>(o[2 * i], p, b[0], b[1]);
           mma16816<BF16>(o[2 * i + 1], p, b[2], b[3]);
         }
@@ -680,11 +718,10 @@ struct KaFew {
       if (lane == 0) mbar_arrive(&empty[st]);
       ++n;
     }
-    // join the slices: [8 warps][16 rows][HD] fp32, columns in pairs, pair p of row g at
-    // p ^ (g << 2) so that a warp's stores meet no bank twice
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&joined[0]);
-    if (!warp_wait(&joined[0], units & 1, abort_flag)) return false;
+    // join the slices: [4 warps][16 rows][HD] fp32, columns in pairs, pair p of row g at
+    // p ^ (g << 2) so that a warp's stores meet no bank twice.  The parts of the unit
+    // before have been read when every warp has said so at its end.
+    if (units > 0 && !warp_wait(&joined[0], (units - 1) & 1, abort_flag)) return false;
     float* part = reinterpret_cast<float*>(sQ);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -701,26 +738,31 @@ struct KaFew {
     if (!warp_wait(&joined[1], units & 1, abort_flag)) return false;
     ++units;
     constexpr int V = HD / 32;
-    for (int pr = warp; pr < u.rows; pr += 8) {
+    const bool direct = whole && !cut_front;
+#pragma unroll 4
+    for (int pr = warp; pr < u.rows; pr += 4) {
       const int r = pr & 15, first = (pr >> 4) * kSlices;
+      float2 ml[kSlices];
       float top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < kSlices; ++i) top = fmaxf(top, s_ml[(first + i) * 16 + r].x);
+      for (int i = 0; i < kSlices; ++i) {
+        ml[i] = s_ml[(first + i) * 16 + r];
+        top = fmaxf(top, ml[i].x);
+      }
       float acc[V] = {}, sum = 0.f;
 #pragma unroll
       for (int i = 0; i < kSlices; ++i) {
-        const float2 ml = s_ml[(first + i) * 16 + r];
-        const float f = ml.y > 0.f ? exp2f(ml.x - top) : 0.f;
+        const float f = ml[i].y > 0.f ? exp2_ftz(ml[i].x - top) : 0.f;
         const float* src = part + ((first + i) * 16 + r) * HD + (((lane * V / 2) ^ ((r & 7) << 2)) << 1);
-        sum += f * ml.y;
+        sum += f * ml[i].y;
 #pragma unroll
         for (int e = 0; e < V; ++e) acc[e] = fmaf(f, src[e], acc[e]);
       }
-      const int packed = u.r0 + pr;
-      const int tok = packed / group, hg = packed - tok * group;
-      const long long row = static_cast<long long>(u.row0) + tok;
-      const int h = head * group + hg;
-      if (whole && !cut_front) {
+      if (direct) {
+        const int packed = u.r0 + pr;
+        const int tok = packed / group, hg = packed - tok * group;
+        const long long row = static_cast<long long>(u.row0) + tok;
+        const int h = head * group + hg;
         const float inv = sum > 0.f ? 1.f / sum : 0.f;
         uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<__half*>(a.out) + row * a.os[0] + h * a.os[1]) + lane * (V / 2);
 #pragma unroll
@@ -735,6 +777,8 @@ struct KaFew {
         if (lane == 0) w.few.ml[slot] = make_float2(top, sum);
       }
     }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&joined[0]);
     return true;
   }
 };
@@ -768,11 +812,12 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   uint64_t* o_done = q_full + 6;           // [2] P V of a tile done
   uint64_t* p_half = q_full + 8;           // [2] its first 64 keys
   uint64_t* mma_done = q_full + 10;
-  uint64_t* few_full = q_full + 11;           // [kStages] the ring in the few-rows phase
-  uint64_t* few_empty = few_full + C::kStages;  // [kStages]
-  uint64_t* joined = few_empty + C::kStages;  // [2] 8 warps: partials may be written, are written
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(joined + 2);
-  float2* s_ml = reinterpret_cast<float2*>(bars + 64);  // [8][16]
+  uint64_t* few_full = q_full + 11;                 // [2][kHalves] the few-row units' rings
+  uint64_t* few_empty = few_full + 2 * C::kHalves;  // [2][kHalves]
+  uint64_t* joined = few_empty + 2 * C::kHalves;    // [2][2] 4 warps: parts read, parts written
+  uint64_t* ring_free = joined + 4;                 // the MMAs have let all stages go
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ring_free + 1);
+  float2* s_ml = reinterpret_cast<float2*>(bars + 80);  // [2][4][16]
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -780,11 +825,15 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     for (int i = 0; i < C::kStages; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
-      mbar_init(&few_full[i], 1);
-      mbar_init(&few_empty[i], 8);
     }
+    for (int i = 0; i < 2 * C::kHalves; ++i) {
+      mbar_init(&few_full[i], 1);
+      mbar_init(&few_empty[i], 4);
+    }
+    mbar_init(ring_free, 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&joined[i], 8);
+      mbar_init(&joined[i], 4);
+      mbar_init(&joined[i + 2], 4);
       mbar_init(&q_full[i], 4);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
@@ -815,31 +864,9 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     // ------------------------------------------------------------ K / V tiles
     int n = 0;  // tiles put into the ring so far
     bool ok = true;
-    uint64_t *fullb = full, *emptyb = empty;
+    KaRing ring{c, tk, tv, a.layer, full, empty, smem_u32(sR), C::kStages, kTile, C::kStage, C::kLoads, abort_flag};
     auto put = [&](const KaUnit& u, int head, int tile, KaPages& pg, bool val) {
-      const int st = n % C::kStages;
-      if (!warp_wait(&emptyb[st], ((n / C::kStages) & 1) ^ 1, abort_flag)) {
-        ok = false;
-        return;
-      }
-      const int key0 = tile * kTile;
-      const int blk = key0 >> c.page_shift;
-      pg.at(c, u, blk);
-      if (lane == 0) mbar_arrive_expect_tx(&fullb[st], C::kStage);
-      __syncwarp();
-      const int per = max(kTile >> c.page_shift, 1);  // pages of a tile
-      const int p = lane / C::kLoads, kb = lane - p * C::kLoads;
-      int id = __shfl_sync(0xffffffffu, pg.ids, (blk + p) & 31);
-      if (lane < per * C::kLoads) {
-        if (id < 0 || id >= c.pages) {
-          // past the sequence's last page: zeros; before it: a hole in the table
-          if (static_cast<long long>(blk + p) << c.page_shift < u.len) record_error(c.err, DEV_BAD_PAGE);
-          id = c.pages;
-        }
-        tma_load_5d(smem_u32(sR + st * C::kStage) + kb * 16384 + p * c.page * 128, val ? &tv : &tk, kb * 64,
-                    key0 & (c.page - 1), head, id, a.layer, &fullb[st]);
-      }
-      ++n;
+      ok = ring.put(u, head, tile, pg, val, n);
     };
     KaCursor x;
     KaPages px;
@@ -867,28 +894,45 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         if (ok && y.left > 0) put(y.u, y.head, y.tile, py, false);
       }
     }
-    // few rows: the same stages with barriers of their own, once the MMAs have let them go
-    const int n_mma = n;
-    for (int j = max(n - C::kStages, 0); ok && j < n; ++j)
-      ok = warp_wait(&empty[j % C::kStages], (j / C::kStages) & 1, abort_flag);
-    n = 0;
-    fullb = few_full;
-    emptyb = few_empty;
-    x.init(w, kFew, cta, c.heads);
-    while (ok && x.left > 0) {
-      put(x.u, x.head, x.tile, px, false);
-      if (ok) put(x.u, x.head, x.tile, px, true);
-      x.next();
-    }
     if (!ok) {
       *abort_flag = 1;
       if (lane == 0) record_error(c.err, DEV_TIMEOUT_EMPTY);
     }
-    // every copy must land before the CTA exits
-    for (int j = n_mma - 1; j >= 0 && j >= n_mma - C::kStages; --j)
+    // every copy must land before the CTA exits, and every MMA have read its stage before
+    // the few-row units use it
+    for (int j = max(n - C::kStages, 0); j < n; ++j) {
+      if (ok) ok = warp_wait(&empty[j % C::kStages], (j / C::kStages) & 1, abort_flag);
       mbar_wait_drain(&full[j % C::kStages], (j / C::kStages) & 1);
-    for (int j = n - 1; j >= 0 && j >= n - C::kStages; --j)
-      mbar_wait_drain(&few_full[j % C::kStages], (j / C::kStages) & 1);
+    }
+    __syncwarp();
+    if (ok && lane == 0) mbar_arrive(ring_free);
+  }
+  if (warp == 8 || warp == 10) {
+    // ------------------------------------------------------------ few rows: 64-key tiles
+    // a ring and a producer warp for each of the two warpgroups
+    const int r = warp == 10;
+    KaCursor x;
+    x.init(w, kFew, cta + r * ctas, c.heads);
+    if (x.left > 0) {
+      // the other kinds may run for long: a limit of about two minutes
+      bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(ring_free, 0, abort_flag, 128 * kWaitLimitCycles));
+      KaRing ring{c, tk, tv, a.layer, few_full + r * C::kHalves, few_empty + r * C::kHalves,
+                  smem_u32(sR) + r * C::kHalves * C::kHalf, C::kHalves, 64, C::kHalf, C::kLoads, abort_flag};
+      KaPages px;
+      int n = 0;
+      while (ok && x.left > 0) {
+        ok = ring.put(x.u, x.head, x.tile, px, false, n);
+        if (ok) ok = ring.put(x.u, x.head, x.tile, px, true, n);
+        x.next();
+      }
+      if (!ok) {
+        *abort_flag = 1;
+        if (lane == 0) record_error(c.err, DEV_TIMEOUT_EMPTY);
+      }
+      for (int j = max(n - C::kHalves, 0); j < n; ++j)
+        mbar_wait_drain(&ring.full[j % C::kHalves], (j / C::kHalves) & 1);
+      __syncwarp();
+    }
   } else if (warp == 9) {
     // ------------------------------------------------------------ MMA issue
     constexpr uint32_t fmt = BF16 ? 1 : 0;
@@ -1236,15 +1280,18 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         cut_front = false;
       }
     }
-    // few rows: all eight warps on one unit
+    // few rows: this warpgroup's share
     if (ok) {
-      KaFew<HD, BF16> f{c, a, w, group, scale_log2, sQ, sR, few_full, few_empty, joined, s_ml, abort_flag};
+      KaFew<HD, BF16> f{c, a, w, group, scale_log2, sQ + s * C::kQ, sR + s * C::kHalves * C::kHalf,
+                        few_full + s * C::kHalves, few_empty + s * C::kHalves, joined + 2 * s, s_ml + s * 64,
+                        abort_flag};
+      const int share = cta + s * ctas;
       KaCursor x;
-      x.init(w, kFew, cta, c.heads);
+      x.init(w, kFew, share, c.heads);
       if (x.left > 0) f.fetch_q(x);
       while (ok && x.left > 0) {
         const int rows = x.u.rows;
-        ok = rows <= 16 ? f.template unit<1>(x, cta) : rows <= 32 ? f.template unit<2>(x, cta) : f.template unit<4>(x, cta);
+        ok = rows <= 16 ? f.template unit<1>(x, share) : rows <= 32 ? f.template unit<2>(x, share) : f.template unit<4>(x, share);
       }
     }
     if (!ok) {
@@ -1349,7 +1396,7 @@ static cudaError_t ka_launch(const KvView& c, const CUtensorMap& tk, const CUten
           static_cast<float>(a.scale * 1.4426950408889634));
   const int64_t packed = static_cast<int64_t>(b.rows) * group;
   const int chunks = static_cast<int>(std::min<int64_t>((packed + 7) / 8, packed > kTile ? 16 : 8));
-  MOE_PDL(kv_merge_kernel<HD, BF16>, dim3(num_sms * 4, chunks), dim3(256), 0, s, a, w, group, num_sms);
+  MOE_PDL(kv_merge_kernel<HD, BF16>, dim3(num_sms * 5, chunks), dim3(256), 0, s, a, w, group, num_sms);
   return cudaSuccess;
 }
 
