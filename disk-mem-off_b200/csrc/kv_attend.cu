@@ -33,6 +33,10 @@
 
 namespace moe {
 
+#ifndef KA_LF
+#define KA_LF 4
+#define KA_LP 4
+#endif
 constexpr int kTile = 128;       // keys of a tile, rows of a warpgroup
 constexpr int kPlanT = 1024;     // threads of the plan kernel
 constexpr int kPlanSmem = 1024;  // units of a list whose prefix sums fit its shared memory
@@ -54,22 +58,27 @@ static_assert(sizeof(KaUnit) == 32, "two 16-byte loads");
 struct KaStart {
   int item, head, tile, count;
 };
-// A unit cut by the end of share `w`: its pieces lie in shares w .. last.
-struct KaCut {
-  int item, head, last, valid;
+// 16 rows of a unit that the ends of shares cut: its pieces lie in shares first .. last.
+struct KaMerge {
+  int kind, first, last, row;
+  int item, head, pad[2];
 };
+static_assert(sizeof(KaStart) == 16 && sizeof(KaMerge) == 32, "16-byte loads");
+constexpr int kMergeRows = 16;
 
 // Kinds of units: rows of a unit, shares an SM.
 constexpr int kPair = 0, kSingle = 1, kFew = 2, kKinds = 3;
 constexpr int kFewRows = 64;
 // What beginning and ending a unit costs, in tiles of its kind.
 __host__ __device__ constexpr int kind_extra(int k) { return k == kFew ? 3 : 1; }
+// The least share worth a CTA or warpgroup of its own, in cost.
+__host__ __device__ constexpr int kind_least(int k) { return k == kFew ? KA_LF : KA_LP; }
 __host__ __device__ constexpr int kind_rows(int k) { return k == kPair ? 2 * kTile : k == kSingle ? kTile : kFewRows; }
 __host__ __device__ constexpr int kind_shares(int k) { return k == kPair ? 1 : 2; }
 __host__ __device__ constexpr int kind_keys(int k) { return k == kFew ? 64 : kTile; }  // of a tile
 
 struct KaWs {
-  size_t start[kKinds], cut[kKinds], list[kKinds], pre[kKinds], o[kKinds], ml[kKinds], total;
+  size_t start[kKinds], list[kKinds], pre[kKinds], o[kKinds], ml[kKinds], merge, n_merge, total;
   int cap[kKinds];
 };
 
@@ -82,6 +91,7 @@ static KaWs ka_ws(const KvView& c, int heads, int rows, int n, int num_sms) {
     return at;
   };
   const int64_t packed = static_cast<int64_t>(rows) * (heads / c.heads);
+  size_t merges = 0;
   w.cap[0] = packed > kTile ? static_cast<int>(packed / (2 * kTile) + std::min<int64_t>(n, packed / kTile)) : 0;
   w.cap[1] = packed > kFewRows ? n : 0;
   w.cap[2] = n;
@@ -89,12 +99,14 @@ static KaWs ka_ws(const KvView& c, int heads, int rows, int n, int num_sms) {
     const size_t shares = static_cast<size_t>(num_sms) * kind_shares(k);
     const size_t prow = 2 * shares * (w.cap[k] ? kind_rows(k) : 0);
     w.start[k] = take(shares * sizeof(KaStart));
-    w.cut[k] = take(shares * sizeof(KaCut));
     w.list[k] = take(static_cast<size_t>(w.cap[k]) * sizeof(KaUnit));
     w.pre[k] = take((static_cast<size_t>(w.cap[k]) + 1) * 8);
     w.o[k] = take(prow * c.hd * 4);
     w.ml[k] = take(prow * 8);
+    merges += shares * (kind_rows(k) / kMergeRows);
   }
+  w.merge = take(merges * sizeof(KaMerge));
+  w.n_merge = take(4);
   w.total = o;
   return w;
 }
@@ -106,7 +118,6 @@ size_t kv_attend_workspace(const KvView& c, int heads, int rows, int n_seqs, int
 // The workspace by kind (0 pairs, 1 singles), for the kernels.
 struct KaList {
   KaStart* start;
-  KaCut* cut;
   KaUnit* list;
   long long* pre;
   float* o;    // [share][0 its first unit, 1 its last][rows][hd] unnormalised
@@ -114,35 +125,44 @@ struct KaList {
 };
 struct KaPtrs {
   KaList pair, single, few;
+  KaMerge* merge;
+  int* n_merge;
   MOE_DEV KaList kind(int k) const { return k == kPair ? pair : k == kSingle ? single : few; }
 };
 
 // ------------------------------------------------------------------ plan
-// Inclusive sum over the plan CTA; *total gets the whole sum.
-MOE_DEV long long plan_scan(long long v, long long* total) {
-  __shared__ long long part[32];
+// Inclusive sums of three numbers over the plan CTA, in place; total gets the whole sums.
+MOE_DEV void plan_scan(long long (&v)[3], long long (&total)[3]) {
+  __shared__ long long part[3][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long u = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += u;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const long long u = __shfl_up_sync(0xffffffffu, v[k], o);
+      if (lane >= o) v[k] += u;
+    }
   }
-  if (lane == 31) part[warp] = v;
+#pragma unroll
+  for (int k = 0; k < 3; ++k)
+    if (lane == 31) part[k][warp] = v[k];
   __syncthreads();
-  if (warp == 0) {
-    long long p = part[lane];
+  if (warp < 3) {
+    long long p = part[warp][lane];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long u = __shfl_up_sync(0xffffffffu, p, o);
       if (lane >= o) p += u;
     }
-    part[lane] = p;
+    part[warp][lane] = p;
   }
   __syncthreads();
-  *total = part[31];
-  const long long before = warp ? part[warp - 1] : 0;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    total[k] = part[k][31];
+    if (warp) v[k] += part[k][warp - 1];
+  }
   __syncthreads();
-  return v + before;
 }
 
 MOE_DEV int key_tiles(int base, int last_token, int keys) {
@@ -152,16 +172,51 @@ MOE_DEV int key_tiles(int base, int last_token, int keys) {
   return static_cast<int>((vis + keys - 1) / keys);
 }
 
-// (1) entries -> units, (2) prefix sums of their tiles, (3) each share's first tile and
-// the units that the shares cut.  Two dependent loads and three scans: about 3 us.
+// Where the cost w0 lies in a list whose prefix sums (of one kv head) are pre[0 .. n]; T:
+// 32 bits when every cost fits.  A unit's extra comes before its tiles, so a border
+// inside it leaves the unit whole.
+struct KaPlace {
+  int item, head, tile;
+  long long unit;   // the unit's cost begins here
+  long long cost;   // and is this
+  long long tiles;  // tiles before w0
+};
+template <typename T>
+MOE_DEV KaPlace plan_place(const long long* pre, int n, T w0, int heads, int extra) {
+  int lo = 0, hi = n;  // heads * pre[lo] <= w0 < heads * pre[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (static_cast<T>(pre[mid]) * heads <= w0) lo = mid;
+    else hi = mid;
+  }
+  const T base = static_cast<T>(pre[lo]) * heads, cost = static_cast<T>(pre[lo + 1] - pre[lo]);
+  const T r = w0 - base, head = r / cost, at = r - head * cost;
+  KaPlace p;
+  p.item = lo;
+  p.head = static_cast<int>(head);
+  p.tile = at > static_cast<T>(extra) ? static_cast<int>(at) - extra : 0;
+  p.unit = static_cast<long long>(base + head * cost);
+  p.cost = static_cast<long long>(cost);
+  p.tiles = p.unit - (static_cast<long long>(lo) * heads + p.head) * extra + p.tile;
+  return p;
+}
+
+// (1) entries -> units and the prefix sums of their costs, (2) each share's first tile and
+// the units that the shares' ends cut.  One CTA, a chain of two dependent loads, one
+// scan and a search: about 4 us, the price of shares of equal work for any mix.
 __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const KvBatch b,
                                                          const int group, const int num_sms,
                                                          const KaPtrs w, const int cap0) {
   pdl_enter();
   __shared__ long long spre[kKinds][kPlanSmem + 1];
+  __shared__ long long stiles[5 * kKvMaxSms + kKinds];
   const int tid = threadIdx.x, lane = tid & 31;
+  __shared__ int s_merges;
+  if (tid == 0) s_merges = 0;
   // (1)
   int n_list[kKinds] = {0, 0, 0};
+  long long work[kKinds] = {0, 0, 0};  // of one kv head
+  long long* pre[kKinds] = {spre[0], b.n <= kPlanSmem ? spre[1] : w.single.pre, b.n <= kPlanSmem ? spre[2] : w.few.pre};
   for (int i0 = 0; i0 < b.n; i0 += kPlanT) {
     const int i = i0 + tid;
     int seq = -1, row0 = 0, m = 0, len = 0;
@@ -189,91 +244,106 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
     const int rem = rows & (2 * kTile - 1);
     const int na = rows / (2 * kTile) + (rem > kTile ? 1 : 0);
     const bool single = rem > kFewRows && rem <= kTile, few = rem > 0 && rem <= kFewRows;
-    // pairs in the low 40 bits, the other two (at most one a thread) above
-    long long total;
-    const long long mine = na | (single ? 1ll << 40 : 0) | (few ? 1ll << 52 : 0);
-    const long long before = plan_scan(mine, &total) - mine;
+    const int tiles = key_tiles(len - m, m - 1, kind_keys(few ? kFew : kSingle));
+    // [0] pairs in the low 40 bits, the other two (at most one a thread) above
+    long long at[3] = {na | (single ? 1ll << 40 : 0) | (few ? 1ll << 52 : 0),
+                       single ? tiles + kind_extra(kSingle) : 0, few ? tiles + kind_extra(kFew) : 0};
+    const long long mine = at[0];
+    long long total[3];
+    plan_scan(at, total);
+    const long long before = at[0] - mine;
     const int at_a = n_list[0] + static_cast<int>(before & 0xffffffffff);
-    const KaUnit rest{seq, row0, rows - rem, rem, len - m, len,
-                      key_tiles(len - m, m - 1, kind_keys(few ? kFew : kSingle)), 0};
-    if (single) w.single.list[n_list[1] + (static_cast<int>(before >> 40) & 0xfff)] = rest;
-    if (few) w.few.list[n_list[2] + static_cast<int>(before >> 52)] = rest;
+    const KaUnit rest{seq, row0, rows - rem, rem, len - m, len, tiles, 0};
+    if (single) {
+      const int j = n_list[1] + (static_cast<int>(before >> 40) & 0xfff);
+      w.single.list[j] = rest;
+      pre[1][j + 1] = work[1] + at[1];
+    }
+    if (few) {
+      const int j = n_list[2] + static_cast<int>(before >> 52);
+      w.few.list[j] = rest;
+      pre[2][j + 1] = work[2] + at[2];
+    }
     // pairs of one entry: the warp's lanes side by side
     for (uint32_t todo = __ballot_sync(0xffffffffu, na > 0); todo; todo &= todo - 1) {
       const int l = __ffs(todo) - 1;
-      const int k = __shfl_sync(0xffffffffu, na, l), at = __shfl_sync(0xffffffffu, at_a, l);
+      const int k = __shfl_sync(0xffffffffu, na, l), to = __shfl_sync(0xffffffffu, at_a, l);
       const int rs = __shfl_sync(0xffffffffu, rows, l), q0 = __shfl_sync(0xffffffffu, row0, l);
       const int sq = __shfl_sync(0xffffffffu, seq, l), ln = __shfl_sync(0xffffffffu, len, l);
       const int mm = __shfl_sync(0xffffffffu, m, l);
-      for (int j = lane; j < k && at + j < cap0; j += 32) {
+      for (int j = lane; j < k && to + j < cap0; j += 32) {
         const int r0 = j * 2 * kTile, r1 = min(r0 + 2 * kTile, rs);
-        w.pair.list[at + j] = KaUnit{sq, q0, r0, r1 - r0, ln - mm, ln, key_tiles(ln - mm, (r1 - 1) / group, kTile), 0};
+        w.pair.list[to + j] = KaUnit{sq, q0, r0, r1 - r0, ln - mm, ln, key_tiles(ln - mm, (r1 - 1) / group, kTile), 0};
       }
     }
-    n_list[0] += static_cast<int>(total & 0xffffffffff);
-    n_list[1] += static_cast<int>(total >> 40) & 0xfff;
-    n_list[2] += static_cast<int>(total >> 52);
+    n_list[0] += static_cast<int>(total[0] & 0xffffffffff);
+    n_list[1] += static_cast<int>(total[0] >> 40) & 0xfff;
+    n_list[2] += static_cast<int>(total[0] >> 52);
+    work[1] += total[1];
+    work[2] += total[2];
   }
   n_list[0] = min(n_list[0], cap0);
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < kKinds; ++k) {
-    // (2)
-    const int n = n_list[k];
-    const KaList w_k = w.kind(k);
-    const int extra = kind_extra(k);
-    long long* pre = n <= kPlanSmem ? spre[k] : w_k.pre;
-    long long work = 0;
-    for (int i0 = 0; i0 < n; i0 += kPlanT) {
-      const int i = i0 + tid;
-      const long long t = i < n ? static_cast<long long>(w_k.list[i].tiles + extra) * c.heads : 0;
-      long long total;
-      const long long incl = work + plan_scan(t, &total);
-      if (i < n) pre[i + 1] = incl;
-      work += total;
-    }
-    if (tid == 0) pre[0] = 0;
+  if (n_list[0] > kPlanSmem) pre[0] = w.pair.pre;
+  if (n_list[0] > 0) {
     __syncthreads();
-    // (3)
-    const int shares = num_sms * kind_shares(k);
-    const long long per = max((work + shares - 1) / shares, 1ll);
-    // where the cost w0 lies: a unit's extra comes before its tiles, so a border inside
-    // it leaves the unit whole
-    auto locate = [&](long long w0, KaStart& st) -> long long {  // -> tiles before it
-      int lo = 0, hi = n;  // pre[lo] <= w0 < pre[hi]
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (pre[mid] <= w0) lo = mid;
-        else hi = mid;
-      }
-      const int cost = static_cast<int>((pre[lo + 1] - pre[lo]) / c.heads);
-      const long long r = w0 - pre[lo];
-      st.item = lo;
-      st.head = static_cast<int>(r / cost);
-      st.tile = max(static_cast<int>(r - static_cast<long long>(st.head) * cost) - extra, 0);
-      return pre[lo] + static_cast<long long>(st.head) * (cost - extra) + st.tile -
-             static_cast<long long>(lo) * extra * c.heads;
-    };
-    const long long tiles_all = work - static_cast<long long>(n) * extra * c.heads;
-    for (int s = tid; s <= shares; s += kPlanT) {
-      const long long w0 = s * per, w1 = w0 + per;
-      KaStart st{0, 0, 0, 0}, end;
-      KaCut cut{0, 0, 0, 0};
-      if (w0 < work) {
-        const long long t0 = locate(w0, st);
-        st.count = static_cast<int>((w1 < work ? locate(w1, end) : tiles_all) - t0);
-        if (s > 0 && st.tile > 0) {
-          const int cost = static_cast<int>((pre[st.item + 1] - pre[st.item]) / c.heads);
-          const long long u0 = pre[st.item] + static_cast<long long>(st.head) * cost;  // the unit's cost begins
-          // cut by this border first if its first tile lies in the share before
-          if (u0 + extra >= w0 - per)
-            cut = KaCut{st.item, st.head, static_cast<int>((u0 + cost - 1) / per), 1};
-        }
-      }
-      if (s < shares) w_k.start[s] = st;
-      if (s > 0) w_k.cut[s - 1] = cut;
+    for (int i0 = 0; i0 < n_list[0]; i0 += kPlanT) {
+      const int i = i0 + tid;
+      long long at[3] = {i < n_list[0] ? w.pair.list[i].tiles + kind_extra(kPair) : 0, 0, 0}, total[3];
+      plan_scan(at, total);
+      if (i < n_list[0]) pre[0][i + 1] = work[0] + at[0];
+      work[0] += total[0];
     }
   }
+  __shared__ long long s_work[kKinds];
+  __shared__ const long long* s_pre[kKinds];
+  __shared__ int s_n[kKinds];
+  if (tid == 0) {
+#pragma unroll
+    for (int k = 0; k < kKinds; ++k) {
+      pre[k][0] = 0;
+      s_pre[k] = pre[k];
+      s_work[k] = work[k];
+      s_n[k] = n_list[k];
+    }
+  }
+  __syncthreads();
+  // (2) a thread for each share of each kind, and one past the last
+  const int counts = 5 * num_sms + kKinds;
+#pragma unroll 1
+  for (int phase = 0; phase < 2; ++phase) {
+    for (int j = tid; j < counts; j += kPlanT) {
+      int k = kPair, s = j;
+      while (s > num_sms * kind_shares(k)) s -= num_sms * kind_shares(k++) + 1;
+      const int shares = num_sms * kind_shares(k), extra = kind_extra(k), n = s_n[k];
+      const long long all = s_work[k] * c.heads;
+      const bool small = all < 0x40000000;
+      const long long per = small ? max((static_cast<int>(all) + shares - 1) / shares, kind_least(k)) : (all + shares - 1) / shares;
+      const long long w0 = s * per;
+      const KaList l = w.kind(k);
+      KaPlace p{};
+      if (w0 < all)
+        p = small ? plan_place<uint32_t>(s_pre[k], n, static_cast<uint32_t>(w0), c.heads, extra)
+                  : plan_place<unsigned long long>(s_pre[k], n, static_cast<unsigned long long>(w0), c.heads, extra);
+      if (phase == 0) {
+        stiles[j] = w0 < all ? p.tiles : all - static_cast<long long>(n) * extra * c.heads;
+        continue;
+      }
+      if (s < shares) {
+        const int count = w0 < all ? static_cast<int>(stiles[j + 1] - stiles[j]) : 0;
+        l.start[s] = KaStart{p.item, p.head, p.tile, count};
+      }
+      // a unit that begins in the share before and is cut here first
+      if (p.tile > 0 && p.unit + extra >= w0 - per) {
+        const int last = small ? static_cast<uint32_t>(p.unit + p.cost - 1) / static_cast<uint32_t>(per)
+                               : static_cast<int>((p.unit + p.cost - 1) / per);
+        const int rows = l.list[p.item].rows;
+        const int nb = (rows + kMergeRows - 1) / kMergeRows, at = atomicAdd(&s_merges, nb);
+        for (int i = 0; i < nb; ++i) w.merge[at + i] = KaMerge{k, s - 1, last, i * kMergeRows, p.item, p.head, {0, 0}};
+      }
+    }
+    __syncthreads();
+  }
+  if (tid == 0) *w.n_merge = s_merges;
 }
 
 // ------------------------------------------------------------------ the kernel
@@ -545,6 +615,30 @@ MOE_DEV uint64_t add_pair(uint64_t a, uint64_t b) {
   return r;
 }
 
+// A unit cut by the ends of shares leaves a piece in each of its shares: rows
+// unnormalised in fp32 with their maximum (base 2, scaled) and sum, in the share's slot 0
+// (the unit began in an earlier share) or 1 (it goes on in a later one).
+MOE_DEV long long piece_slot(int kind, int share, bool tail, int row) {
+  return (2ll * share + (tail ? 1 : 0)) * kind_rows(kind) + row;
+}
+
+// Results of one packed row: lane's HD / 32 values, the log of the sum.
+template <int HD, bool BF16>
+MOE_DEV void write_row(const KvAttend& a, const KaUnit& u, int head, int group, int pr, const float* v,
+                       float top, float sum) {
+  constexpr int V = HD / 32;
+  const int lane = threadIdx.x & 31;
+  const int packed = u.r0 + pr;
+  const int tok = packed / group, h = head * group + (packed - tok * group);
+  const long long row = static_cast<long long>(u.row0) + tok;
+  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<__half*>(a.out) + row * a.os[0] + h * a.os[1]) + lane * (V / 2);
+#pragma unroll
+  for (int e = 0; e < V / 2; ++e) dst[e] = pack2<BF16>(v[2 * e] * inv, v[2 * e + 1] * inv);
+  if (a.lse && lane == 0)
+    a.lse[row * a.ls[0] + h * a.ls[1]] = sum > 0.f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+}
+
 template <int HD, bool BF16>
 struct KaFew {
   using C = KaCfg<HD>;
@@ -759,18 +853,9 @@ struct KaFew {
         for (int e = 0; e < V; ++e) acc[e] = fmaf(f, src[e], acc[e]);
       }
       if (direct) {
-        const int packed = u.r0 + pr;
-        const int tok = packed / group, hg = packed - tok * group;
-        const long long row = static_cast<long long>(u.row0) + tok;
-        const int h = head * group + hg;
-        const float inv = sum > 0.f ? 1.f / sum : 0.f;
-        uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<__half*>(a.out) + row * a.os[0] + h * a.os[1]) + lane * (V / 2);
-#pragma unroll
-        for (int e = 0; e < V / 2; ++e) dst[e] = pack2<BF16>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-        if (a.lse && lane == 0)
-          a.lse[row * a.ls[0] + h * a.ls[1]] = sum > 0.f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+        write_row<HD, BF16>(a, u, head, group, pr, acc, top, sum);
       } else {
-        const long long slot = (2ll * share + (cut_front ? 0 : 1)) * kFewRows + pr;
+        const long long slot = piece_slot(kFew, share, !cut_front, pr);
         float* dst = w.few.o + slot * HD + lane * V;
 #pragma unroll
         for (int e = 0; e < V; ++e) dst[e] = acc[e];
@@ -1260,9 +1345,9 @@ __global__ void __launch_bounds__(kAttThreads, 1)
                   l > 0.f ? (m - shift + log2f(l)) * 0.6931471805599453f : -INFINITY;
           } else {
             // a piece: unnormalised, to the share's slot 0 (its first unit) or 1 (its last)
-            const int per = kind_rows(kind);
-            const long long slot = (2ll * share + (cut_front ? 0 : 1)) * per + pr;
-            float4* dst = reinterpret_cast<float4*>(w.kind(kind).o + slot * HD);
+            const KaList l_k = w.kind(kind);
+            const long long slot = piece_slot(kind, share, !cut_front, pr);
+            float4* dst = reinterpret_cast<float4*>(l_k.o + slot * HD);
 #pragma unroll
             for (int i = 0; i < HD / 32; ++i) {
               float o[32];
@@ -1273,7 +1358,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
                   dst[i * 8 + j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
               }
             }
-            if (valid) w.kind(kind).ml[slot] = make_float2(l > 0.f ? m - shift : -INFINITY, l);
+            if (valid) l_k.ml[slot] = make_float2(l > 0.f ? m - shift : -INFINITY, l);
           }
         }
         tc_fence_before();  // O is read: the next unit's first product may overwrite it
@@ -1310,36 +1395,45 @@ __global__ void __launch_bounds__(kAttThreads, 1)
 }
 
 // ------------------------------------------------------------------ merge
-// Rows of the units that a share's border cut: pieces in shares first .. last, joined in
-// that order.  A warp a row.
+// Joins the pieces of cut units, in share order: 16 rows a CTA and step, two rows a warp.
+// A kernel of its own, since its reading (two or more fp32 pieces a row) wants the whole
+// GPU: joined by the last warp of a unit inside the attention kernel, 64 mixed chunks took
+// 293 us instead of 241.
 template <int HD, bool BF16>
-__global__ void __launch_bounds__(256) kv_merge_kernel(const KvAttend a, const KaPtrs w, const int group,
-                                                       const int num_sms) {
+__global__ void __launch_bounds__(256) kv_merge_kernel(const KvAttend a, const KaPtrs w, const int group) {
   pdl_enter();
   constexpr int V = HD / 32;
-  int kind = kPair, share = blockIdx.x;
-  while (share >= num_sms * kind_shares(kind)) share -= num_sms * kind_shares(kind++);
-  const KaList wk = w.kind(kind);
-  const int4 cut = *reinterpret_cast<const int4*>(wk.cut + share);
-  if (!cut.w) return;
-  const KaUnit u = wk.list[cut.x];
+  const int n = *w.n_merge;
   const int lane = threadIdx.x & 31;
-  const int per = kind_rows(kind);
-  for (int pr = blockIdx.y * 8 + (threadIdx.x >> 5); pr < u.rows; pr += gridDim.y * 8) {
-    float top = -INFINITY;
-    for (int p = share + lane; p <= cut.z; p += 32)
-      top = fmaxf(top, wk.ml[(2ll * p + (p == share ? 1 : 0)) * per + pr].x);
+  for (int i = blockIdx.x; i < n; i += gridDim.x) {
+    const int4 e = *reinterpret_cast<const int4*>(w.merge + i);
+    const int2 at = *reinterpret_cast<const int2*>(&w.merge[i].item);
+    const int kind = e.x, first = e.y, last = e.z;
+    const KaList l = w.kind(kind);
+    const KaUnit u = l.list[at.x];
+    const int r0 = e.w + 2 * (threadIdx.x >> 5);
+    if (r0 >= u.rows) continue;
+    const bool two = r0 + 1 < u.rows;
+    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, acc[2][V] = {};
+    for (int s = first + lane; s <= last; s += 32) {
+      const long long slot = piece_slot(kind, s, s == first, r0);
+      top[0] = fmaxf(top[0], l.ml[slot].x);
+      if (two) top[1] = fmaxf(top[1], l.ml[slot + 1].x);
+    }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float acc[V] = {}, l = 0.f;
-    if (top != -INFINITY) {
+    for (int o = 16; o > 0; o >>= 1) {
+      top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], o));
+      top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], o));
+    }
 #pragma unroll 4
-      for (int p = share; p <= cut.z; ++p) {
-        const long long slot = (2ll * p + (p == share ? 1 : 0)) * per + pr;
-        const float2 ml = wk.ml[slot];
-        const float f = exp2f(ml.x - top);
+    for (int s = first; s <= last; ++s) {
+      const long long slot = piece_slot(kind, s, s == first, r0);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (j && !two) continue;
+        const float2 ml = l.ml[slot + j];
+        const float* src = l.o + (slot + j) * HD + lane * V;
         float v[V];
-        const float* src = wk.o + slot * HD + lane * V;
         if constexpr (V == 4) {
           const float4 t = *reinterpret_cast<const float4*>(src);
           v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
@@ -1347,21 +1441,14 @@ __global__ void __launch_bounds__(256) kv_merge_kernel(const KvAttend a, const K
           const float2 t = *reinterpret_cast<const float2*>(src);
           v[0] = t.x; v[1] = t.y;
         }
-        l += f * ml.y;
+        const float f = ml.y > 0.f ? exp2_ftz(ml.x - top[j]) : 0.f;
+        sum[j] += f * ml.y;
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = fmaf(f, v[i], acc[i]);
+        for (int e2 = 0; e2 < V; ++e2) acc[j][e2] = fmaf(f, v[e2], acc[j][e2]);
       }
     }
-    const int packed = u.r0 + pr;
-    const int tok = packed / group, hg = packed - tok * group;
-    const long long row = static_cast<long long>(u.row0) + tok;
-    const int h = cut.y * group + hg;
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<__half*>(a.out) + row * a.os[0] + h * a.os[1]) + lane * (V / 2);
-#pragma unroll
-    for (int i = 0; i < V / 2; ++i) dst[i] = pack2<BF16>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
-    if (a.lse && lane == 0)
-      a.lse[row * a.ls[0] + h * a.ls[1]] = l > 0.f ? (top + log2f(l)) * 0.6931471805599453f : -INFINITY;
+    write_row<HD, BF16>(a, u, at.y, group, r0, acc[0], top[0], sum[0]);
+    if (two) write_row<HD, BF16>(a, u, at.y, group, r0 + 1, acc[1], top[1], sum[1]);
   }
 }
 
@@ -1374,12 +1461,13 @@ static cudaError_t ka_launch(const KvView& c, const CUtensorMap& tk, const CUten
   for (int k = 0; k < kKinds; ++k) {
     KaList& d = k == kPair ? w.pair : k == kSingle ? w.single : w.few;
     d.start = reinterpret_cast<KaStart*>(ws + l.start[k]);
-    d.cut = reinterpret_cast<KaCut*>(ws + l.cut[k]);
     d.list = reinterpret_cast<KaUnit*>(ws + l.list[k]);
     d.pre = reinterpret_cast<long long*>(ws + l.pre[k]);
     d.o = reinterpret_cast<float*>(ws + l.o[k]);
     d.ml = reinterpret_cast<float2*>(ws + l.ml[k]);
   }
+  w.merge = reinterpret_cast<KaMerge*>(ws + l.merge);
+  w.n_merge = reinterpret_cast<int*>(ws + l.n_merge);
   constexpr size_t smem = KaCfg<HD>::kSmem;
   static bool attr_set[64] = {};
   int dev = 0;
@@ -1394,9 +1482,7 @@ static cudaError_t ka_launch(const KvView& c, const CUtensorMap& tk, const CUten
   MOE_PDL(kv_plan_kernel, dim3(1), dim3(kPlanT), 0, s, c, b, group, num_sms, w, l.cap[0]);
   MOE_PDL(kv_attend_kernel<HD, BF16>, dim3(num_sms), dim3(kAttThreads), smem, s, tk, tv, c, a, w, group,
           static_cast<float>(a.scale * 1.4426950408889634));
-  const int64_t packed = static_cast<int64_t>(b.rows) * group;
-  const int chunks = static_cast<int>(std::min<int64_t>((packed + 7) / 8, packed > kTile ? 16 : 8));
-  MOE_PDL(kv_merge_kernel<HD, BF16>, dim3(num_sms * 5, chunks), dim3(256), 0, s, a, w, group, num_sms);
+  MOE_PDL(kv_merge_kernel<HD, BF16>, dim3(num_sms * 4), dim3(256), 0, s, a, w, group);
   return cudaSuccess;
 }
 

@@ -41,6 +41,9 @@ inline size_t kv_scratch_words(int pages, int nseq) {
 
 // Most sequences of a cache: a bitmap of them is checked in shared memory.
 constexpr int kKvMaxSeqs = 65536;
+// Most SMs that a cache's kernels are spread over (a B200 has 148): the attention's plan
+// keeps a number for each share in shared memory.
+constexpr int kKvMaxSms = 192;
 
 // One batch of new rows: row r of entry e is q_start[e] <= r < q_start[e + 1].
 struct KvBatch {

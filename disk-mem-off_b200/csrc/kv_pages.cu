@@ -635,7 +635,7 @@ int moe_kv_create(const MoeKvConfig* cfg, MoeKvCache** out) {
   h->device = c.device;
   int sms = 0;
   h->num_sms = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, c.device) == cudaSuccess && sms > 0
-                   ? sms : 148;
+                   ? std::min(sms, kKvMaxSms) : 148;
   std::string err;
   if (!make_tmap_pool(&h->tk, c.k, h->bf16, v, v.ks, &err) ||
       !make_tmap_pool(&h->tv, c.v, h->bf16, v, v.vs, &err)) {
@@ -730,16 +730,17 @@ int moe_kv_compact(MoeKvCache* cache, MoeKvCache* into, void* stream) {
 }
 
 int moe_kv_append(MoeKvCache* cache, int32_t layer, const void* k, const void* v,
-                  const int64_t* k_strides, const int64_t* v_strides, const int32_t* seqs,
-                  const int32_t* q_start, int32_t n_seqs, int32_t rows, void* stream) {
+                  int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head,
+                  const int32_t* seqs, const int32_t* q_start, int32_t n_seqs, int32_t rows,
+                  void* stream) {
   MOE_KV_ENTER(cache);
   if (const int rc = check_batch(cache, layer, seqs, q_start, n_seqs, rows)) return rc;
   if (n_seqs == 0 || rows == 0) return MOE_OK;
-  if (!k || !v || !k_strides || !v_strides) return kfail(MOE_ERR_INVALID, "null k / v");
-  if (misaligned16(k) || misaligned16(v) || bad_strides(k_strides) || bad_strides(v_strides))
+  if (!k || !v) return kfail(MOE_ERR_INVALID, "null k / v");
+  const int64_t ks[2] = {k_token, k_head}, vs[2] = {v_token, v_head};
+  if (misaligned16(k) || misaligned16(v) || bad_strides(ks) || bad_strides(vs))
     return kfail(MOE_ERR_INVALID, "k and v must be 16-byte aligned, with strides that are multiples of 8");
   const KvBatch b{seqs, q_start, n_seqs, rows};
-  const int64_t ks[2] = {k_strides[0], k_strides[1]}, vs[2] = {v_strides[0], v_strides[1]};
   MOE_KV_CUDA(kv_launch_append(cache->v, b, layer, k, v, ks, vs, cache->num_sms,
                                static_cast<cudaStream_t>(stream)));
   return MOE_OK;

@@ -70,11 +70,13 @@ class MoeKvConfigC(ctypes.Structure):
 
 
 class MoeKvAttendArgsC(ctypes.Structure):
+    # the pairs of strides (token, head) one by one: filled on every call
     _fields_ = [
-        ("q", c_void_p), ("out", c_void_p), ("lse", c_void_p), ("q_strides", c_int64 * 2),
-        ("out_strides", c_int64 * 2), ("lse_strides", c_int64 * 2), ("seqs", c_void_p),
-        ("q_start", c_void_p), ("n_seqs", c_int32), ("rows", c_int32), ("heads", c_int32),
-        ("layer", c_int32), ("scale", c_float),
+        ("q", c_void_p), ("out", c_void_p), ("lse", c_void_p),
+        ("q_token", c_int64), ("q_head", c_int64), ("out_token", c_int64), ("out_head", c_int64),
+        ("lse_token", c_int64), ("lse_head", c_int64), ("seqs", c_void_p), ("q_start", c_void_p),
+        ("n_seqs", c_int32), ("rows", c_int32), ("heads", c_int32), ("layer", c_int32),
+        ("scale", c_float),
     ]
 
 
@@ -154,8 +156,8 @@ _PROTOTYPES: dict[str, tuple] = {
     "moe_kv_truncate": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_void_p]),
     "moe_kv_copy_pages": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_void_p]),
     "moe_kv_compact": (c_int32, [c_void_p, c_void_p, c_void_p]),
-    "moe_kv_append": (c_int32, [c_void_p, c_int32, c_void_p, c_void_p, POINTER(c_int64),
-                                POINTER(c_int64), c_void_p, c_void_p, c_int32, c_int32, c_void_p]),
+    "moe_kv_append": (c_int32, [c_void_p, c_int32, c_void_p, c_void_p, c_int64, c_int64, c_int64,
+                                c_int64, c_void_p, c_void_p, c_int32, c_int32, c_void_p]),
     "moe_kv_attend_workspace_bytes": (c_uint64, [c_void_p, c_int32, c_int32, c_int32]),
     "moe_kv_attend": (c_int32, [c_void_p, POINTER(MoeKvAttendArgsC), c_void_p, c_uint64, c_void_p]),
     "moe_kv_status": (c_int32, [c_void_p, c_void_p]),

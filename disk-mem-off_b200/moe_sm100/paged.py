@@ -30,8 +30,6 @@ from . import _lib
 from ._lib import check, lib
 from .layer import _stream_handle, _torch
 
-_PAIR = c_int64 * 2
-
 
 def _strides(t: Any) -> list[int]:
     """Element strides; a dimension of one entry gets 0 (torch leaves it arbitrary)."""
@@ -87,6 +85,11 @@ class PagedKVCache:
         self.device = k.device
         self.dtype = k.dtype
         self.kv_heads, self.page_size, self.head_dim = kv_heads, page_size, head_dim
+        self._dev = k.get_device()
+        self._lib = lib()
+        self._i32, self._f32, self._u8 = torch.int32, torch.float32, torch.uint8
+        self._empty, self._current_stream = torch.empty, torch.cuda.current_stream
+        self._scale = 1.0 / math.sqrt(head_dim)
         cfg = _lib.MoeKvConfigC(
             k=k.data_ptr(), v=v.data_ptr(), k_strides=(c_int64 * 4)(*_strides(k)[:4]),
             v_strides=(c_int64 * 4)(*_strides(v)[:4]), block_table=block_table.data_ptr(),
@@ -130,60 +133,67 @@ class PagedKVCache:
             pass
 
     # -- arguments ----------------------------------------------------------------
+    # A decode step makes these calls once a layer, and its kernels take some
+    # microseconds: the checks compare the devices' numbers and dtype objects.
     def _index(self, name: str, t: Any) -> Any:
-        torch = _torch()
-        if not isinstance(t, torch.Tensor):
+        if not hasattr(t, "data_ptr"):
+            torch = _torch()
             t = torch.tensor(list(t), dtype=torch.int32).to(self.device)
-        if t.dtype != torch.int32 or t.dim() != 1 or t.device != self.device:
+        if t.dtype is not self._i32 or t.dim() != 1 or t.get_device() != self._dev:
             raise TypeError(f"{name} must be a 1-D int32 tensor on {self.device}")
         return t if t.is_contiguous() else t.contiguous()
 
-    def _indices(self, a: str, x: Any, b: str, y: Any) -> tuple[Any, Any]:
+    def _indices(self, a: str, x: Any, b: str, y: Any) -> tuple[Any, Any, int]:
         x, y = self._index(a, x), self._index(b, y)
-        if x.shape[0] != y.shape[0]:
+        n = x.shape[0]
+        if y.shape[0] != n:
             raise ValueError(f"{a} and {b} must have one entry each")
-        return x, y
+        return x, y, n
 
-    def _batch(self, seqs: Any, starts: Any) -> tuple[Any, Any]:
+    def _batch(self, seqs: Any, starts: Any) -> tuple[Any, Any, int]:
         seqs, starts = self._index("seqs", seqs), self._index("starts", starts)
-        if starts.shape[0] != seqs.shape[0] + 1:
+        n = seqs.shape[0]
+        if starts.shape[0] != n + 1:
             raise ValueError("starts must have one entry more than seqs")
-        return seqs, starts
+        return seqs, starts, n
 
-    def _rows(self, name: str, t: Any) -> Any:
-        torch = _torch()
-        if not (isinstance(t, torch.Tensor) and t.dtype == self.dtype and t.device == self.device):
+    def _rows(self, name: str, t: Any) -> tuple[int, int, int, int]:
+        """Rows and heads of ``t`` and their strides."""
+        if not hasattr(t, "data_ptr") or t.dtype is not self.dtype or t.get_device() != self._dev:
             raise TypeError(f"{name} must be a {self.dtype} tensor on {self.device}")
-        if t.dim() != 3 or t.shape[2] != self.head_dim or (t.stride(2) != 1 and t.numel()):
-            raise ValueError(f"{name} must be [rows, heads, {self.head_dim}], the last dimension "
-                             "contiguous")
-        return t
+        shape = t.shape
+        if len(shape) != 3 or shape[2] != self.head_dim:
+            raise ValueError(f"{name} must be [rows, heads, {self.head_dim}]")
+        rows, heads, _ = shape
+        token, head, dim = t.stride()
+        if dim != 1 and rows and heads:
+            raise ValueError(f"the last dimension of {name} must be contiguous")
+        return rows, heads, token if rows > 1 else 0, head if heads > 1 else 0
 
     def _stream(self) -> int:
-        return _torch().cuda.current_stream(self.device).cuda_stream
+        return self._current_stream(self._dev).cuda_stream
 
     # -- pages --------------------------------------------------------------------
     @_on_stream
     def reserve(self, seqs: Any, counts: Any) -> None:
         """Lengthen ``seqs[i]`` by ``counts[i]`` tokens, with pages for them."""
-        seqs, counts = self._indices("seqs", seqs, "counts", counts)
-        check(lib().moe_kv_reserve(self._h, seqs.data_ptr(), counts.data_ptr(), seqs.shape[0],
-                                   self._stream()))
+        seqs, counts, n = self._indices("seqs", seqs, "counts", counts)
+        check(self._lib.moe_kv_reserve(self._h, seqs.data_ptr(), counts.data_ptr(), n, self._stream()))
 
     @_on_stream
     def fork(self, parents: Any, children: Any) -> None:
         """Make the empty sequence ``children[i]`` a copy of ``parents[i]`` that shares
         its pages; a page is copied when one of its holders next writes to it."""
-        parents, children = self._indices("parents", parents, "children", children)
-        check(lib().moe_kv_fork(self._h, parents.data_ptr(), children.data_ptr(),
-                                parents.shape[0], self._stream()))
+        parents, children, n = self._indices("parents", parents, "children", children)
+        check(self._lib.moe_kv_fork(self._h, parents.data_ptr(), children.data_ptr(), n,
+                                    self._stream()))
 
     @_on_stream
     def truncate(self, seqs: Any, lengths: Any) -> None:
         """Shorten ``seqs[i]`` to ``lengths[i]`` tokens and let its other pages go."""
-        seqs, lengths = self._indices("seqs", seqs, "lengths", lengths)
-        check(lib().moe_kv_truncate(self._h, seqs.data_ptr(), lengths.data_ptr(), seqs.shape[0],
-                                    self._stream()))
+        seqs, lengths, n = self._indices("seqs", seqs, "lengths", lengths)
+        check(self._lib.moe_kv_truncate(self._h, seqs.data_ptr(), lengths.data_ptr(), n,
+                                        self._stream()))
 
     @_on_stream
     def free(self, seqs: Any) -> None:
@@ -194,30 +204,29 @@ class PagedKVCache:
     @_on_stream
     def copy_pages(self, src: Any, dst: Any) -> None:
         """Copy pages ``src[i]`` to ``dst[i]`` in every layer; tables and refs stay."""
-        src, dst = self._indices("src", src, "dst", dst)
-        check(lib().moe_kv_copy_pages(self._h, src.data_ptr(), dst.data_ptr(), src.shape[0],
-                                      self._stream()))
+        src, dst, n = self._indices("src", src, "dst", dst)
+        check(self._lib.moe_kv_copy_pages(self._h, src.data_ptr(), dst.data_ptr(), n,
+                                          self._stream()))
 
     @_on_stream
     def compact(self, into: "PagedKVCache | None" = None) -> None:
         """Move the live pages to the lowest numbers, or, dense and in order, ``into``
         another cache (whose sequences are overwritten): how a pool changes its size."""
-        check(lib().moe_kv_compact(self._h, into._h if into is not None else None,
-                                   self._stream()))
+        check(self._lib.moe_kv_compact(self._h, into._h if into is not None else None,
+                                       self._stream()))
 
     # -- tokens -------------------------------------------------------------------
     @_on_stream
     def append(self, k: Any, v: Any, seqs: Any, starts: Any, layer: int = 0) -> None:
         """Write the batch's keys and values ``[rows, kv_heads, head_dim]`` to the last
         places of their sequences (after ``reserve``)."""
-        seqs, starts = self._batch(seqs, starts)
-        k, v = self._rows("k", k), self._rows("v", v)
-        if k.shape != v.shape or k.shape[1] != self.kv_heads:
+        seqs, starts, n = self._batch(seqs, starts)
+        rows, heads, kt, kh = self._rows("k", k)
+        vrows, vheads, vt, vh = self._rows("v", v)
+        if heads != self.kv_heads or vheads != heads or vrows != rows:
             raise ValueError(f"k and v must both be [rows, {self.kv_heads}, {self.head_dim}]")
-        check(lib().moe_kv_append(self._h, layer, k.data_ptr(), v.data_ptr(),
-                                  _PAIR(*_strides(k)[:2]), _PAIR(*_strides(v)[:2]),
-                                  seqs.data_ptr(), starts.data_ptr(), seqs.shape[0], k.shape[0],
-                                  self._stream()))
+        check(self._lib.moe_kv_append(self._h, layer, k.data_ptr(), v.data_ptr(), kt, kh, vt, vh,
+                                      seqs.data_ptr(), starts.data_ptr(), n, rows, self._stream()))
 
     @_on_stream
     def attend(self, q: Any, seqs: Any, starts: Any, layer: int = 0, scale: float | None = None,
@@ -225,36 +234,35 @@ class PagedKVCache:
         """Causal attention of the batch's rows ``q`` ``[rows, heads, head_dim]`` over all
         tokens of their sequences; returns ``out``, shaped as ``q``.  ``lse``: an fp32
         ``[rows, heads]`` tensor that receives the log of the sum of the exponentials."""
-        torch = _torch()
-        seqs, starts = self._batch(seqs, starts)
-        q = self._rows("q", q)
-        heads = q.shape[1]
+        seqs, starts, n = self._batch(seqs, starts)
+        rows, heads, qt, qh = self._rows("q", q)
         if heads == 0 or heads % self.kv_heads:
             raise ValueError(f"heads must be a multiple of {self.kv_heads}")
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        elif self._rows("out", out).shape != q.shape:
-            raise ValueError("out must have the shape of q")
-        if lse is not None and (lse.dtype != torch.float32 or lse.device != self.device
-                                or lse.shape != q.shape[:2]):
-            raise ValueError("lse must be a float32 [rows, heads] tensor on the cache's device")
-        rows, n = q.shape[0], seqs.shape[0]
+            out = self._empty((rows, heads, self.head_dim), dtype=self.dtype, device=self.device)
+            ot, oh = heads * self.head_dim, self.head_dim
+        else:
+            orows, oheads, ot, oh = self._rows("out", out)
+            if orows != rows or oheads != heads:
+                raise ValueError("out must have the shape of q")
+        lp, lt, lh = None, 0, 0
+        if lse is not None:
+            if lse.dtype is not self._f32 or lse.get_device() != self._dev or lse.shape != q.shape[:2]:
+                raise ValueError("lse must be a float32 [rows, heads] tensor on the cache's device")
+            lp, (lt, lh) = lse.data_ptr(), _strides(lse)
         if rows == 0 or n == 0:
             return out
-        args = _lib.MoeKvAttendArgsC(
-            q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
-            _PAIR(*_strides(q)[:2]), _PAIR(*_strides(out)[:2]),
-            _PAIR() if lse is None else _PAIR(*_strides(lse)), seqs.data_ptr(), starts.data_ptr(),
-            n, rows, heads, layer,
-            1.0 / math.sqrt(self.head_dim) if scale is None else scale)
         # the scratch of one call: torch's allocator keeps it apart from other streams' and
         # graphs' scratch
-        need = lib().moe_kv_attend_workspace_bytes(self._h, heads, rows, n)
-        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-        check(lib().moe_kv_attend(self._h, byref(args), ws.data_ptr(), need, self._stream()))
+        need = self._lib.moe_kv_attend_workspace_bytes(self._h, heads, rows, n)
+        ws = self._empty(need, dtype=self._u8, device=self.device)
+        args = _lib.MoeKvAttendArgsC(q.data_ptr(), out.data_ptr(), lp, qt, qh, ot, oh, lt, lh,
+                                     seqs.data_ptr(), starts.data_ptr(), n, rows, heads, layer,
+                                     self._scale if scale is None else scale)
+        check(self._lib.moe_kv_attend(self._h, byref(args), ws.data_ptr(), need, self._stream()))
         return out
 
     @_on_stream
     def status(self) -> None:
         """Wait for the stream and raise what the cache's kernels reported, if anything."""
-        check(lib().moe_kv_status(self._h, self._stream()))
+        check(self._lib.moe_kv_status(self._h, self._stream()))

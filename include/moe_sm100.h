@@ -424,8 +424,8 @@ int moe_kv_compact(MoeKvCache* cache, MoeKvCache* into, void* stream);
  * lengths[seqs[i]] - (q_start[i+1] - r).  Reserve first.  k, v: [rows][kv_heads][head_dim] in
  * the cache's dtype, token and head strides in elements (multiples of 8).  Rows from
  * q_start[n_seqs] on are ignored.  The same sequence twice: the rows of one entry win. */
-int moe_kv_append(MoeKvCache* cache, int32_t layer, const void* k, const void* v,
-                  const int64_t* k_strides, const int64_t* v_strides, const int32_t* seqs,
+int moe_kv_append(MoeKvCache* cache, int32_t layer, const void* k, const void* v, int64_t k_token,
+                  int64_t k_head, int64_t v_token, int64_t v_head, const int32_t* seqs,
                   const int32_t* q_start, int32_t n_seqs, int32_t rows, void* stream);
 /* out = softmax(scale * q k^T, causal) v of each new row over all tokens of its sequence up
  * to its own position; fp32 softmax and accumulation, probabilities rounded to the cache's

@@ -105,7 +105,6 @@ def test_create_refuses(built_lib: str, bad: dict, code: int) -> None:
 
 def test_null_arguments_are_errors(built_lib: str) -> None:
     lib = _lib.lib()
-    pair = (c_int64 * 2)()
     assert lib.moe_kv_create(None, None) == _lib.MOE_ERR_INVALID
     assert lib.moe_kv_scratch_bytes(None) == 0
     assert lib.moe_kv_scratch_bytes(byref(_cfg(pages=0))) == 0
@@ -116,7 +115,7 @@ def test_null_arguments_are_errors(built_lib: str) -> None:
     assert lib.moe_kv_truncate(None, None, None, 1, None) == _lib.MOE_ERR_INVALID
     assert lib.moe_kv_copy_pages(None, None, None, 1, None) == _lib.MOE_ERR_INVALID
     assert lib.moe_kv_compact(None, None, None) == _lib.MOE_ERR_INVALID
-    assert lib.moe_kv_append(None, 0, None, None, pair, pair, None, None, 1, 1, None) == \
+    assert lib.moe_kv_append(None, 0, None, None, 0, 0, 0, 0, None, None, 1, 1, None) == \
         _lib.MOE_ERR_INVALID
     assert lib.moe_kv_attend(None, None, None, 0, None) == _lib.MOE_ERR_INVALID
     assert lib.moe_kv_attend_workspace_bytes(None, 8, 1, 1) == 0
