@@ -34,12 +34,12 @@
 namespace moe {
 
 #ifndef KA_LF
-#define KA_LF 4
+#define KA_LF 2
 #define KA_LP 4
 #endif
 constexpr int kTile = 128;       // keys of a tile, rows of a warpgroup
 constexpr int kPlanT = 1024;     // threads of the plan kernel
-constexpr int kPlanSmem = 1024;  // units of a list whose prefix sums fit its shared memory
+constexpr int kPlanSmem = 512;   // units of a list whose prefix sums fit its shared memory
 
 // Rows [r0, r0 + rows) of an entry, for every kv head.
 struct KaUnit {
@@ -58,10 +58,10 @@ static_assert(sizeof(KaUnit) == 32, "two 16-byte loads");
 struct KaStart {
   int item, head, tile, count;
 };
-// 16 rows of a unit that the ends of shares cut: its pieces lie in shares first .. last.
+// A unit that the ends of shares cut: its pieces lie in shares first .. last.
 struct KaMerge {
-  int kind, first, last, row;
-  int item, head, pad[2];
+  int kind, first, last, head;
+  int row0, r0, rows, pad;  // of the unit
 };
 static_assert(sizeof(KaStart) == 16 && sizeof(KaMerge) == 32, "16-byte loads");
 constexpr int kMergeRows = 16;
@@ -103,7 +103,7 @@ static KaWs ka_ws(const KvView& c, int heads, int rows, int n, int num_sms) {
     w.pre[k] = take((static_cast<size_t>(w.cap[k]) + 1) * 8);
     w.o[k] = take(prow * c.hd * 4);
     w.ml[k] = take(prow * 8);
-    merges += shares * (kind_rows(k) / kMergeRows);
+    merges += shares;
   }
   w.merge = take(merges * sizeof(KaMerge));
   w.n_merge = take(4);
@@ -131,38 +131,40 @@ struct KaPtrs {
 };
 
 // ------------------------------------------------------------------ plan
-// Inclusive sums of three numbers over the plan CTA, in place; total gets the whole sums.
-MOE_DEV void plan_scan(long long (&v)[3], long long (&total)[3]) {
-  __shared__ long long part[3][32];
+// Inclusive sum over the plan CTA; *total gets the whole sum.  `busy`: the warps that may
+// hold anything but zero.
+MOE_DEV long long plan_scan(long long v, int busy, long long* total) {
+  __shared__ long long part[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (warp < busy) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-#pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      const long long u = __shfl_up_sync(0xffffffffu, v[k], o);
-      if (lane >= o) v[k] += u;
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
     }
+    if (lane == 31) part[warp] = v;
   }
-#pragma unroll
-  for (int k = 0; k < 3; ++k)
-    if (lane == 31) part[k][warp] = v[k];
   __syncthreads();
-  if (warp < 3) {
-    long long p = part[warp][lane];
+  long long before = 0, all = 0;
+  if (busy <= 4) {
+    for (int i = 0; i < busy; ++i) {
+      const long long p = part[i];
+      if (i < warp) before += p;
+      all += p;
+    }
+  } else {
+    long long p = lane < busy ? part[lane] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long u = __shfl_up_sync(0xffffffffu, p, o);
       if (lane >= o) p += u;
     }
-    part[warp][lane] = p;
+    all = __shfl_sync(0xffffffffu, p, 31);
+    before = warp ? __shfl_sync(0xffffffffu, p, warp - 1) : 0;
   }
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    total[k] = part[k][31];
-    if (warp) v[k] += part[k][warp - 1];
-  }
-  __syncthreads();
+  *total = all;
+  __syncthreads();  // part is written again by the next call
+  return v + before;
 }
 
 MOE_DEV int key_tiles(int base, int last_token, int keys) {
@@ -202,23 +204,26 @@ MOE_DEV KaPlace plan_place(const long long* pre, int n, T w0, int heads, int ext
 }
 
 // (1) entries -> units and the prefix sums of their costs, (2) each share's first tile and
-// the units that the shares' ends cut.  One CTA, a chain of two dependent loads, one
-// scan and a search: about 4 us, the price of shares of equal work for any mix.
+// the units that the shares' ends cut.  One CTA: two dependent loads, two scans, a search.
 __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const KvBatch b,
                                                          const int group, const int num_sms,
                                                          const KaPtrs w, const int cap0) {
   pdl_enter();
   __shared__ long long spre[kKinds][kPlanSmem + 1];
-  __shared__ long long stiles[5 * kKvMaxSms + kKinds];
-  const int tid = threadIdx.x, lane = tid & 31;
+  __shared__ long long stiles[kPlanT + 1];
   __shared__ int s_merges;
+  __shared__ int4 s_entry[kPlanT];       // the chunk's entries: seq, row0, m, len
+  __shared__ int s_pairs[kPlanT + 1];    // pairs before each of them
+  const int tid = threadIdx.x;
   if (tid == 0) s_merges = 0;
   // (1)
-  int n_list[kKinds] = {0, 0, 0};
-  long long work[kKinds] = {0, 0, 0};  // of one kv head
-  long long* pre[kKinds] = {spre[0], b.n <= kPlanSmem ? spre[1] : w.single.pre, b.n <= kPlanSmem ? spre[2] : w.few.pre};
+  int n_pair = 0, n_single = 0, n_few = 0;
+  long long work_pair = 0, work_single = 0, work_few = 0;  // of one kv head
+  long long* pre_pair = cap0 <= kPlanSmem ? spre[0] : w.pair.pre;
+  long long* pre_single = b.n <= kPlanSmem ? spre[1] : w.single.pre;
+  long long* pre_few = b.n <= kPlanSmem ? spre[2] : w.few.pre;
   for (int i0 = 0; i0 < b.n; i0 += kPlanT) {
-    const int i = i0 + tid;
+    const int i = i0 + tid, busy = min((b.n - i0 + 31) / 32, 32);
     int seq = -1, row0 = 0, m = 0, len = 0;
     if (i < b.n) {
       seq = b.seqs[i];
@@ -245,106 +250,100 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
     const int na = rows / (2 * kTile) + (rem > kTile ? 1 : 0);
     const bool single = rem > kFewRows && rem <= kTile, few = rem > 0 && rem <= kFewRows;
     const int tiles = key_tiles(len - m, m - 1, kind_keys(few ? kFew : kSingle));
-    // [0] pairs in the low 40 bits, the other two (at most one a thread) above
-    long long at[3] = {na | (single ? 1ll << 40 : 0) | (few ? 1ll << 52 : 0),
-                       single ? tiles + kind_extra(kSingle) : 0, few ? tiles + kind_extra(kFew) : 0};
-    const long long mine = at[0];
-    long long total[3];
-    plan_scan(at, total);
-    const long long before = at[0] - mine;
-    const int at_a = n_list[0] + static_cast<int>(before & 0xffffffffff);
+    // counts (at most 1024 each) in the high bits, cost of a chunk's units in the low 44
     const KaUnit rest{seq, row0, rows - rem, rem, len - m, len, tiles, 0};
-    if (single) {
-      const int j = n_list[1] + (static_cast<int>(before >> 40) & 0xfff);
-      w.single.list[j] = rest;
-      pre[1][j + 1] = work[1] + at[1];
-    }
+    long long total, mine = few ? (1ll << 44) + tiles + kind_extra(kFew) : 0;
+    long long at = plan_scan(mine, busy, &total);
+    constexpr long long kLow = (1ll << 44) - 1;
     if (few) {
-      const int j = n_list[2] + static_cast<int>(before >> 52);
+      const int j = n_few + static_cast<int>(at >> 44) - 1;
       w.few.list[j] = rest;
-      pre[2][j + 1] = work[2] + at[2];
+      pre_few[j + 1] = work_few + (at & kLow);
     }
-    // pairs of one entry: the warp's lanes side by side
-    for (uint32_t todo = __ballot_sync(0xffffffffu, na > 0); todo; todo &= todo - 1) {
-      const int l = __ffs(todo) - 1;
-      const int k = __shfl_sync(0xffffffffu, na, l), to = __shfl_sync(0xffffffffu, at_a, l);
-      const int rs = __shfl_sync(0xffffffffu, rows, l), q0 = __shfl_sync(0xffffffffu, row0, l);
-      const int sq = __shfl_sync(0xffffffffu, seq, l), ln = __shfl_sync(0xffffffffu, len, l);
-      const int mm = __shfl_sync(0xffffffffu, m, l);
-      for (int j = lane; j < k && to + j < cap0; j += 32) {
-        const int r0 = j * 2 * kTile, r1 = min(r0 + 2 * kTile, rs);
-        w.pair.list[to + j] = KaUnit{sq, q0, r0, r1 - r0, ln - mm, ln, key_tiles(ln - mm, (r1 - 1) / group, kTile), 0};
-      }
+    n_few += static_cast<int>(total >> 44);
+    work_few += total & kLow;
+    if (!__syncthreads_or(single || na > 0)) continue;
+    mine = single ? (1ll << 44) + tiles + kind_extra(kSingle) : 0;
+    at = plan_scan(mine, busy, &total);
+    if (single) {
+      const int j = n_single + static_cast<int>(at >> 44) - 1;
+      w.single.list[j] = rest;
+      pre_single[j + 1] = work_single + (at & kLow);
     }
-    n_list[0] += static_cast<int>(total[0] & 0xffffffffff);
-    n_list[1] += static_cast<int>(total[0] >> 40) & 0xfff;
-    n_list[2] += static_cast<int>(total[0] >> 52);
-    work[1] += total[1];
-    work[2] += total[2];
-  }
-  n_list[0] = min(n_list[0], cap0);
-  if (n_list[0] > kPlanSmem) pre[0] = w.pair.pre;
-  if (n_list[0] > 0) {
+    n_single += static_cast<int>(total >> 44);
+    work_single += total & kLow;
+    at = plan_scan(na, busy, &total);
+    s_entry[tid] = make_int4(seq, row0, m, len);
+    s_pairs[tid + 1] = static_cast<int>(at);
+    if (tid == 0) s_pairs[0] = 0;
     __syncthreads();
-    for (int i0 = 0; i0 < n_list[0]; i0 += kPlanT) {
-      const int i = i0 + tid;
-      long long at[3] = {i < n_list[0] ? w.pair.list[i].tiles + kind_extra(kPair) : 0, 0, 0}, total[3];
-      plan_scan(at, total);
-      if (i < n_list[0]) pre[0][i + 1] = work[0] + at[0];
-      work[0] += total[0];
+    const int pairs = min(static_cast<int>(total), cap0 - n_pair);
+    for (int j0 = 0; j0 < pairs; j0 += kPlanT) {  // a thread a pair
+      const int j = j0 + tid;
+      long long mine = 0, all;
+      KaUnit u{};
+      if (j < pairs) {
+        int lo = 0, hi = min(b.n - i0, kPlanT);  // s_pairs[lo] <= j < s_pairs[hi]
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (s_pairs[mid] <= j) lo = mid;
+          else hi = mid;
+        }
+        const int4 e = s_entry[lo];
+        const int r0 = (j - s_pairs[lo]) * 2 * kTile, r1 = min(r0 + 2 * kTile, e.z * group);
+        u = KaUnit{e.x, e.y, r0, r1 - r0, e.w - e.z, e.w, key_tiles(e.w - e.z, (r1 - 1) / group, kTile), 0};
+        w.pair.list[n_pair + j] = u;
+        mine = u.tiles + kind_extra(kPair);
+      }
+      const long long sum = plan_scan(mine, min((pairs - j0 + 31) / 32, 32), &all);
+      if (j < pairs) pre_pair[n_pair + j + 1] = work_pair + sum;
+      work_pair += all;
+    }
+    n_pair += pairs;
+  }
+  if (tid == 0) pre_pair[0] = pre_single[0] = pre_few[0] = 0;
+  __syncthreads();
+  // (2) a thread for each share of each kind, and one past the last of each
+  int k = kPair, s = tid;
+  while (k < kKinds && s > num_sms * kind_shares(k)) s -= num_sms * kind_shares(k++) + 1;
+  const int shares = num_sms * kind_shares(k), extra = kind_extra(k);
+  const int n = k == kPair ? n_pair : k == kSingle ? n_single : n_few;
+  const long long* pre = k == kPair ? pre_pair : k == kSingle ? pre_single : pre_few;
+  const long long all = (k == kPair ? work_pair : k == kSingle ? work_single : work_few) * c.heads;
+  const bool small = all < 0x40000000;
+  long long per = 1, w0 = 0;
+  KaPlace p{};
+  if (k < kKinds && all > 0) {
+    if (small) {
+      const uint32_t per32 = max((static_cast<uint32_t>(all) + shares - 1) / static_cast<uint32_t>(shares),
+                                 static_cast<uint32_t>(kind_least(k)));
+      per = per32;
+      w0 = static_cast<long long>(s) * per32;
+      if (w0 < all) p = plan_place<uint32_t>(pre, n, static_cast<uint32_t>(w0), c.heads, extra);
+    } else {
+      per = (all + shares - 1) / shares;
+      w0 = s * per;
+      if (w0 < all) p = plan_place<unsigned long long>(pre, n, static_cast<unsigned long long>(w0), c.heads, extra);
     }
   }
-  __shared__ long long s_work[kKinds];
-  __shared__ const long long* s_pre[kKinds];
-  __shared__ int s_n[kKinds];
-  if (tid == 0) {
-#pragma unroll
-    for (int k = 0; k < kKinds; ++k) {
-      pre[k][0] = 0;
-      s_pre[k] = pre[k];
-      s_work[k] = work[k];
-      s_n[k] = n_list[k];
+  const bool in = k < kKinds && w0 < all;
+  stiles[tid] = in ? p.tiles : all - static_cast<long long>(n) * extra * c.heads;
+  __syncthreads();
+  if (k < kKinds) {
+    const KaList l = w.kind(k);
+    if (s < shares) l.start[s] = KaStart{p.item, p.head, p.tile, in ? static_cast<int>(stiles[tid + 1] - stiles[tid]) : 0};
+    // a unit that begins in the share before and is cut here first
+    if (p.tile > 0 && p.unit + extra >= w0 - per) {
+      const int last = small ? static_cast<uint32_t>(p.unit + p.cost - 1) / static_cast<uint32_t>(per)
+                             : static_cast<int>((p.unit + p.cost - 1) / per);
+      const KaUnit u = l.list[p.item];
+      w.merge[atomicAdd(&s_merges, 1)] = KaMerge{k, s - 1, last, p.head, u.row0, u.r0, u.rows, 0};
     }
   }
   __syncthreads();
-  // (2) a thread for each share of each kind, and one past the last
-  const int counts = 5 * num_sms + kKinds;
-#pragma unroll 1
-  for (int phase = 0; phase < 2; ++phase) {
-    for (int j = tid; j < counts; j += kPlanT) {
-      int k = kPair, s = j;
-      while (s > num_sms * kind_shares(k)) s -= num_sms * kind_shares(k++) + 1;
-      const int shares = num_sms * kind_shares(k), extra = kind_extra(k), n = s_n[k];
-      const long long all = s_work[k] * c.heads;
-      const bool small = all < 0x40000000;
-      const long long per = small ? max((static_cast<int>(all) + shares - 1) / shares, kind_least(k)) : (all + shares - 1) / shares;
-      const long long w0 = s * per;
-      const KaList l = w.kind(k);
-      KaPlace p{};
-      if (w0 < all)
-        p = small ? plan_place<uint32_t>(s_pre[k], n, static_cast<uint32_t>(w0), c.heads, extra)
-                  : plan_place<unsigned long long>(s_pre[k], n, static_cast<unsigned long long>(w0), c.heads, extra);
-      if (phase == 0) {
-        stiles[j] = w0 < all ? p.tiles : all - static_cast<long long>(n) * extra * c.heads;
-        continue;
-      }
-      if (s < shares) {
-        const int count = w0 < all ? static_cast<int>(stiles[j + 1] - stiles[j]) : 0;
-        l.start[s] = KaStart{p.item, p.head, p.tile, count};
-      }
-      // a unit that begins in the share before and is cut here first
-      if (p.tile > 0 && p.unit + extra >= w0 - per) {
-        const int last = small ? static_cast<uint32_t>(p.unit + p.cost - 1) / static_cast<uint32_t>(per)
-                               : static_cast<int>((p.unit + p.cost - 1) / per);
-        const int rows = l.list[p.item].rows;
-        const int nb = (rows + kMergeRows - 1) / kMergeRows, at = atomicAdd(&s_merges, nb);
-        for (int i = 0; i < nb; ++i) w.merge[at + i] = KaMerge{k, s - 1, last, i * kMergeRows, p.item, p.head, {0, 0}};
-      }
-    }
-    __syncthreads();
-  }
   if (tid == 0) *w.n_merge = s_merges;
 }
+static_assert(5 * kKvMaxSms + kKinds <= kPlanT, "a thread for each share");
 
 // ------------------------------------------------------------------ the kernel
 template <int HD>
@@ -361,7 +360,7 @@ struct KaCfg {
 static_assert(KaCfg<128>::kSmem <= 227 * 1024 && KaCfg<64>::kSmem > 114 * 1024,
               "one CTA, and with it all of TMEM, an SM");
 
-// Twelve warps (8: K / V, 9: MMA, 10 and 11 idle), so that each third is a warpgroup and
+// Twelve warps (8: K / V, 9: MMA, 10 and 11: Q), so that each third is a warpgroup and
 // registers can move between them: 384 * 168 at launch = 2 * 128 * 208 + 128 * 80 + rest.
 constexpr int kAttThreads = 384;
 constexpr int kRegsSoftmax = 208, kRegsOther = 80;
@@ -418,10 +417,11 @@ struct KaCursor {
     u.seq = a.x; u.row0 = a.y; u.r0 = a.z; u.rows = a.w;
     u.base = b.x; u.len = b.y; u.tiles = b.z;
   }
-  MOE_DEV void init(const KaPtrs& w, int kind, int share, int kv_heads) {
-    const KaList l = w.kind(kind);
-    const int4 s = *reinterpret_cast<const int4*>(l.start + share);
-    list = l.list;
+  MOE_DEV static int4 start(const KaPtrs& w, int kind, int share) {
+    return *reinterpret_cast<const int4*>(w.kind(kind).start + share);
+  }
+  MOE_DEV void init(const KaPtrs& w, int kind, const int4 s, int kv_heads) {
+    list = w.kind(kind).list;
     item = s.x;
     head = s.y;
     tile = s.z;
@@ -431,9 +431,12 @@ struct KaCursor {
   }
   // this share's last tile of the unit
   MOE_DEV bool ends_unit() const { return tile + 1 == u.tiles || left == 1; }
-  MOE_DEV void next() {
-    --left;
-    if (++tile == u.tiles) {
+  MOE_DEV void next() { skip(1); }
+  // the next n tiles, all of this unit
+  MOE_DEV void skip(int n) {
+    left -= n;
+    tile += n;
+    if (tile == u.tiles) {
       tile = 0;
       if (++head == heads) {
         head = 0;
@@ -620,6 +623,12 @@ MOE_DEV uint64_t add_pair(uint64_t a, uint64_t b) {
 // (the unit began in an earlier share) or 1 (it goes on in a later one).
 MOE_DEV long long piece_slot(int kind, int share, bool tail, int row) {
   return (2ll * share + (tail ? 1 : 0)) * kind_rows(kind) + row;
+}
+
+MOE_DEV void store32(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 
 // Results of one packed row: lane's HD / 32 values, the log of the sum.
@@ -901,7 +910,8 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   uint64_t* few_empty = few_full + 2 * C::kHalves;  // [2][kHalves]
   uint64_t* joined = few_empty + 2 * C::kHalves;    // [2][2] 4 warps: parts read, parts written
   uint64_t* ring_free = joined + 4;                 // the MMAs have let all stages go
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ring_free + 1);
+  uint64_t* q_free = ring_free + 1;                 // [2] every S of a unit done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_free + 2);
   float2* s_ml = reinterpret_cast<float2*>(bars + 80);  // [2][4][16]
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -919,7 +929,8 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&joined[i], 4);
       mbar_init(&joined[i + 2], 4);
-      mbar_init(&q_full[i], 4);
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_free[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
       mbar_init(&p_half[i], 4);
@@ -953,9 +964,11 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     auto put = [&](const KaUnit& u, int head, int tile, KaPages& pg, bool val) {
       ok = ring.put(u, head, tile, pg, val, n);
     };
+    const int4 st_pair = KaCursor::start(w, kPair, cta), st0 = KaCursor::start(w, kSingle, cta),
+               st1 = KaCursor::start(w, kSingle, cta + ctas);
     KaCursor x;
     KaPages px;
-    x.init(w, kPair, cta, c.heads);
+    x.init(w, kPair, st_pair, c.heads);
     while (ok && x.left > 0) {
       put(x.u, x.head, x.tile, px, false);
       if (ok) put(x.u, x.head, x.tile, px, true);
@@ -963,8 +976,8 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     }
     KaCursor y;
     KaPages py;
-    x.init(w, kSingle, cta, c.heads);
-    y.init(w, kSingle, cta + ctas, c.heads);
+    x.init(w, kSingle, st0, c.heads);
+    y.init(w, kSingle, st1, c.heads);
     if (ok && x.left > 0) put(x.u, x.head, x.tile, px, false);
     if (ok && y.left > 0) put(y.u, y.head, y.tile, py, false);
     while (ok && (x.left > 0 || y.left > 0)) {
@@ -992,12 +1005,65 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     __syncwarp();
     if (ok && lane == 0) mbar_arrive(ring_free);
   }
+  if (warp >= 10) {
+    // ------------------------------------------------------------ Q tiles of a stream
+    // 128 rows, swizzled as the MMA reads them, as soon as the S products of the unit
+    // before are done: under its last softmax and its epilogue
+    const int s = warp - 10;
+    const __half* q16 = static_cast<const __half*>(a.q);
+    constexpr int ch = HD / 8, step = 32 / ch;  // 16-byte chunks of a row, rows at a time
+    const int row_in = lane / ch, chunk = lane - row_in * ch;
+    const uint32_t to = smem_u32(sQ) + s * C::kQ + (chunk >> 3) * 16384;
+    const int dtok = step / group, dhg = step - dtok * group;
+    const int4 st_pair = KaCursor::start(w, kPair, cta), st_single = KaCursor::start(w, kSingle, cta + s * ctas);
+    bool ok = true;
+    int units = 0;  // begun so far
+#pragma unroll 1
+    for (int kind = kPair; kind <= kSingle && ok; ++kind) {
+      const int part = kind ? 0 : s;
+      KaCursor x;
+      x.init(w, kind, kind ? st_single : st_pair, c.heads);
+      while (ok && x.left > 0) {
+        if (units > 0 && !warp_wait(&q_free[s], (units - 1) & 1, abort_flag)) {
+          ok = false;
+          break;
+        }
+        const KaUnit& u = x.u;
+        int row = row_in, packed = u.r0 + part * kTile + row;
+        int tok = packed / group, hg = packed - tok * group;
+        const __half* src = q16 + static_cast<long long>(u.row0) * a.qs[0] +
+                            static_cast<long long>(x.head) * group * a.qs[1] + chunk * 8;
+        const int rows = min(u.rows - part * kTile, kTile);
+#pragma unroll 8
+        for (; row < rows; row += step) {
+          cp_async16(to + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), src + tok * a.qs[0] + hg * a.qs[1]);
+          tok += dtok;
+          hg += dhg;
+          if (hg >= group) {
+            hg -= group;
+            ++tok;
+          }
+        }
+        cp_async_wait();
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[s]);
+        ++units;
+        x.skip(min(x.left, x.u.tiles - x.tile));
+      }
+    }
+    if (!ok) {
+      *abort_flag = 1;
+      if (lane == 0) record_error(c.err, DEV_TIMEOUT_FULL);
+    }
+    __syncwarp();
+  }
   if (warp == 8 || warp == 10) {
     // ------------------------------------------------------------ few rows: 64-key tiles
     // a ring and a producer warp for each of the two warpgroups
     const int r = warp == 10;
     KaCursor x;
-    x.init(w, kFew, cta + r * ctas, c.heads);
+    x.init(w, kFew, KaCursor::start(w, kFew, cta + r * ctas), c.heads);
     if (x.left > 0) {
       // the other kinds may run for long: a limit of about two minutes
       bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(ring_free, 0, abort_flag, 128 * kWaitLimitCycles));
@@ -1034,8 +1100,8 @@ __global__ void __launch_bounds__(kAttThreads, 1)
       ++n;
       return st;
     };
-    // S of stream s from Q tile s and ring stage st
-    auto issue_s = [&](int s, int st, bool begins) {
+    // S of stream s from Q tile s and ring stage st; begins / ends: the unit's first / last
+    auto issue_s = [&](int s, int st, bool begins, bool ends) {
       if (begins) {
         if (!warp_wait(&q_full[s], nq[s] & 1, abort_flag)) ok = false;
         ++nq[s];
@@ -1049,6 +1115,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
           tc_mma_f16(tm + s * kTile, dq + off, dk + off, id_s, k > 0 ? 1u : 0u);
         }
         tc_commit(&s_full[s]);
+        if (ends) tc_commit(&q_free[s]);
       }
       __syncwarp();
     };
@@ -1089,12 +1156,15 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     };
     // pairs: both streams read the same K and V tiles.  At a unit's end the next S (which
     // waits for the next Q) comes after both products with V.
+    const int4 st_pair = KaCursor::start(w, kPair, cta);
+    const int4 st_single[2] = {KaCursor::start(w, kSingle, cta), KaCursor::start(w, kSingle, cta + ctas)};
     KaCursor x;
-    x.init(w, kPair, cta, c.heads);
+    x.init(w, kPair, st_pair, c.heads);
     if (x.left > 0) {
       int kst = take();
-      if (ok) issue_s(0, kst, true);
-      if (ok) issue_s(1, kst, true);
+      const bool one = x.ends_unit();
+      if (ok) issue_s(0, kst, true, one);
+      if (ok) issue_s(1, kst, true, one);
       if (ok) release(kst);
       bool first = true;
       while (ok) {
@@ -1109,16 +1179,16 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         issue_o(0, vst, first);
         if (ok && more && !ends) {
           kst = take();
-          if (ok) issue_s(0, kst, false);
+          if (ok) issue_s(0, kst, false, x.ends_unit());
         }
         if (ok) issue_o(1, vst, first);
         if (ok) release(vst);
         if (ok && more && ends) {
           kst = take();
-          if (ok) issue_s(0, kst, true);
+          if (ok) issue_s(0, kst, true, x.ends_unit());
         }
         if (ok && more) {
-          issue_s(1, kst, ends);
+          issue_s(1, kst, ends, x.ends_unit());
           if (ok) release(kst);
         }
         first = ends;
@@ -1129,12 +1199,12 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     KaCursor y[2];
     bool first[2] = {true, true};
 #pragma unroll
-    for (int s = 0; s < 2; ++s) y[s].init(w, kSingle, cta + s * ctas, c.heads);
+    for (int s = 0; s < 2; ++s) y[s].init(w, kSingle, st_single[s], c.heads);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       if (ok && y[s].left > 0) {
         const int st = take();
-        if (ok) issue_s(s, st, true);
+        if (ok) issue_s(s, st, true, y[s].ends_unit());
         if (ok) release(st);
       }
     }
@@ -1152,7 +1222,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         y[s].next();
         if (ok && y[s].left > 0) {
           const int kst = take();
-          if (ok) issue_s(s, kst, ends);
+          if (ok) issue_s(s, kst, ends, y[s].ends_unit());
           if (ok) release(kst);
         }
       }
@@ -1178,42 +1248,18 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     // P is scaled by 2^shift: f16 keeps probabilities down to 2^-31 of the largest
     // (the reference maximum may lag by 2^8: 2^15 at most, below f16's 65504)
     constexpr float shift = BF16 ? 0.f : 7.f;
-    const __half* q16 = static_cast<const __half*>(a.q);
     __half* out16 = static_cast<__half*>(a.out);
     bool ok = true;
     int nt = 0;  // tiles of this stream so far
-    // this warp's 32 rows of a unit's Q, swizzled as the MMA reads them; two rows a step
-    auto load_q = [&](const KaUnit& u, int head, int part) {
-      constexpr int ch = HD / 8;       // 16-byte chunks of a row
-      const int row_in = lane / ch, chunk = lane - row_in * ch;
-      const uint32_t base = smem_u32(sQ) + s * C::kQ + (chunk >> 3) * 16384;
-      for (int r = row_in; r < 32; r += 32 / ch) {
-        const int row = quad * 32 + r;
-        const int pr = part * kTile + row;
-        if (pr < u.rows) {
-          const int packed = u.r0 + pr;
-          const int tok = packed / group, hg = packed - tok * group;
-          const __half* src = q16 + (static_cast<long long>(u.row0) + tok) * a.qs[0] +
-                              (static_cast<long long>(head) * group + hg) * a.qs[1] + chunk * 8;
-          cp_async16(base + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), src);
-        }
-      }
-    };
-    auto q_ready = [&]() {
-      cp_async_wait();
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full[s]);
-    };
+    const int4 st_pair = KaCursor::start(w, kPair, cta), st_single = KaCursor::start(w, kSingle, cta + s * ctas),
+               st_few = KaCursor::start(w, kFew, cta + s * ctas);
 #pragma unroll 1
     for (int kind = kPair; kind <= kSingle && ok; ++kind) {
       const int share = kind ? cta + s * ctas : cta;
       const int part = kind ? 0 : s;  // the unit's rows of this warpgroup: part * 128 ..
       KaCursor x;
-      x.init(w, kind, share, c.heads);
+      x.init(w, kind, kind ? st_single : st_pair, c.heads);
       if (x.left <= 0) continue;
-      load_q(x.u, x.head, part);
-      q_ready();
       bool cut_front = x.tile > 0;  // the unit began in an earlier share
       while (x.left > 0 && ok) {
         const KaUnit u = x.u;
@@ -1237,8 +1283,6 @@ __global__ void __launch_bounds__(kAttThreads, 1)
             break;
           }
           tc_fence_after();
-          const bool load_next = ends && x.left > 0;
-          if (load_next) load_q(x.u, x.head, part);  // S of this unit is done: Q is free
           if (any) {
             float sc[kTile];
             load_s(t_s, sc);
@@ -1312,7 +1356,6 @@ __global__ void __launch_bounds__(kAttThreads, 1)
               mbar_arrive(&p_full[s]);
             }
           }
-          if (load_next) q_ready();
           ++nt;
         }
         if (!ok) break;
@@ -1326,18 +1369,27 @@ __global__ void __launch_bounds__(kAttThreads, 1)
             const long long row = static_cast<long long>(u.row0) + tok;
             const int h = head * group + hg;
             const float inv = l > 0.f ? 1.f / l : 0.f;
-            uint4* dst = reinterpret_cast<uint4*>(out16 + row * a.os[0] + h * a.os[1]);
+            // a thread writes its own row: its 32 lanes meet 32 lines in every store, so
+            // the stores are as wide as they can be
+            __half* dst = out16 + row * a.os[0] + h * a.os[1];
+            const bool wide = !((reinterpret_cast<uintptr_t>(out16) | (a.os[0] * 2) | (a.os[1] * 2)) & 31);
 #pragma unroll
             for (int i = 0; i < HD / 32; ++i) {
               float o[32];
               tmem_ld32(t_o + i * 32, o);
-              uint32_t pk[16];
 #pragma unroll
-              for (int j = 0; j < 16; ++j)
-                pk[j] = l > 0.f ? pack2<BF16>(o[2 * j] * inv, o[2 * j + 1] * inv) : 0u;
-              if (valid) {
+              for (int k = 0; k < 2; ++k) {
+                uint32_t pk[8];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) dst[i * 4 + j] = make_uint4(pk[4 * j], pk[4 * j + 1], pk[4 * j + 2], pk[4 * j + 3]);
+                for (int j = 0; j < 8; ++j)
+                  pk[j] = l > 0.f ? pack2<BF16>(o[k * 16 + 2 * j] * inv, o[k * 16 + 2 * j + 1] * inv) : 0u;
+                if (valid && wide) {
+                  store32(dst + i * 32 + k * 16, pk);
+                } else if (valid) {
+                  uint4* d4 = reinterpret_cast<uint4*>(dst + i * 32 + k * 16);
+                  d4[0] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                  d4[1] = make_uint4(pk[4], pk[5], pk[6], pk[7]);
+                }
               }
             }
             if (valid && a.lse)
@@ -1347,15 +1399,19 @@ __global__ void __launch_bounds__(kAttThreads, 1)
             // a piece: unnormalised, to the share's slot 0 (its first unit) or 1 (its last)
             const KaList l_k = w.kind(kind);
             const long long slot = piece_slot(kind, share, !cut_front, pr);
-            float4* dst = reinterpret_cast<float4*>(l_k.o + slot * HD);
+            float* dst = l_k.o + slot * HD;
 #pragma unroll
             for (int i = 0; i < HD / 32; ++i) {
               float o[32];
               tmem_ld32(t_o + i * 32, o);
               if (valid) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                  dst[i * 8 + j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                for (int k = 0; k < 4; ++k) {
+                  uint32_t v[8];
+#pragma unroll
+                  for (int j = 0; j < 8; ++j) v[j] = __float_as_uint(o[k * 8 + j]);
+                  store32(dst + i * 32 + k * 8, v);
+                }
               }
             }
             if (valid) l_k.ml[slot] = make_float2(l > 0.f ? m - shift : -INFINITY, l);
@@ -1372,7 +1428,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
                         abort_flag};
       const int share = cta + s * ctas;
       KaCursor x;
-      x.init(w, kFew, share, c.heads);
+      x.init(w, kFew, st_few, c.heads);
       if (x.left > 0) f.fetch_q(x);
       while (ok && x.left > 0) {
         const int rows = x.u.rows;
@@ -1382,7 +1438,6 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     if (!ok) {
       *abort_flag = 1;
       if (lane == 0) record_error(c.err, DEV_TIMEOUT_TMEM_FULL);
-      cp_async_wait();
     }
   }
   pdl_release();
@@ -1397,42 +1452,35 @@ __global__ void __launch_bounds__(kAttThreads, 1)
 // ------------------------------------------------------------------ merge
 // Joins the pieces of cut units, in share order: 16 rows a CTA and step, two rows a warp.
 // A kernel of its own, since its reading (two or more fp32 pieces a row) wants the whole
-// GPU: joined by the last warp of a unit inside the attention kernel, 64 mixed chunks took
+// GPU: joined by the last warp of a unit inside the attention kernel, 33 mixed chunks took
 // 293 us instead of 241.
 template <int HD, bool BF16>
 __global__ void __launch_bounds__(256) kv_merge_kernel(const KvAttend a, const KaPtrs w, const int group) {
   pdl_enter();
   constexpr int V = HD / 32;
-  const int n = *w.n_merge;
   const int lane = threadIdx.x & 31;
+  const int r0 = blockIdx.y * kMergeRows + 2 * (threadIdx.x >> 5);
+  const int n = *w.n_merge;
   for (int i = blockIdx.x; i < n; i += gridDim.x) {
-    const int4 e = *reinterpret_cast<const int4*>(w.merge + i);
-    const int2 at = *reinterpret_cast<const int2*>(&w.merge[i].item);
+    const int4 e = reinterpret_cast<const int4*>(w.merge + i)[0], f = reinterpret_cast<const int4*>(w.merge + i)[1];
     const int kind = e.x, first = e.y, last = e.z;
-    const KaList l = w.kind(kind);
-    const KaUnit u = l.list[at.x];
-    const int r0 = e.w + 2 * (threadIdx.x >> 5);
+    KaUnit u;
+    u.row0 = f.x;
+    u.r0 = f.y;
+    u.rows = f.z;
     if (r0 >= u.rows) continue;
-    const bool two = r0 + 1 < u.rows;
+    const KaList l = w.kind(kind);
+    const int two = r0 + 1 < u.rows ? 1 : 0;  // or the same row again, not written
     float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, acc[2][V] = {};
-    for (int s = first + lane; s <= last; s += 32) {
-      const long long slot = piece_slot(kind, s, s == first, r0);
-      top[0] = fmaxf(top[0], l.ml[slot].x);
-      if (two) top[1] = fmaxf(top[1], l.ml[slot + 1].x);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], o));
-      top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], o));
-    }
+    // the running maximum of the pieces moves with them: one pass, loads of four pieces
+    // in flight
 #pragma unroll 4
     for (int s = first; s <= last; ++s) {
       const long long slot = piece_slot(kind, s, s == first, r0);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        if (j && !two) continue;
-        const float2 ml = l.ml[slot + j];
-        const float* src = l.o + (slot + j) * HD + lane * V;
+        const float2 ml = l.ml[slot + j * two];
+        const float* src = l.o + (slot + j * two) * HD + lane * V;
         float v[V];
         if constexpr (V == 4) {
           const float4 t = *reinterpret_cast<const float4*>(src);
@@ -1441,14 +1489,17 @@ __global__ void __launch_bounds__(256) kv_merge_kernel(const KvAttend a, const K
           const float2 t = *reinterpret_cast<const float2*>(src);
           v[0] = t.x; v[1] = t.y;
         }
-        const float f = ml.y > 0.f ? exp2_ftz(ml.x - top[j]) : 0.f;
-        sum[j] += f * ml.y;
+        const float up = fmaxf(top[j], ml.x);
+        const float keep = top[j] == -INFINITY ? 0.f : exp2_ftz(top[j] - up);
+        const float f2 = ml.x == -INFINITY ? 0.f : exp2_ftz(ml.x - up);
+        top[j] = up;
+        sum[j] = sum[j] * keep + f2 * ml.y;
 #pragma unroll
-        for (int e2 = 0; e2 < V; ++e2) acc[j][e2] = fmaf(f, v[e2], acc[j][e2]);
+        for (int x = 0; x < V; ++x) acc[j][x] = fmaf(f2, v[x], acc[j][x] * keep);
       }
     }
-    write_row<HD, BF16>(a, u, at.y, group, r0, acc[0], top[0], sum[0]);
-    if (two) write_row<HD, BF16>(a, u, at.y, group, r0 + 1, acc[1], top[1], sum[1]);
+    write_row<HD, BF16>(a, u, e.w, group, r0, acc[0], top[0], sum[0]);
+    if (two) write_row<HD, BF16>(a, u, e.w, group, r0 + 1, acc[1], top[1], sum[1]);
   }
 }
 
@@ -1482,7 +1533,9 @@ static cudaError_t ka_launch(const KvView& c, const CUtensorMap& tk, const CUten
   MOE_PDL(kv_plan_kernel, dim3(1), dim3(kPlanT), 0, s, c, b, group, num_sms, w, l.cap[0]);
   MOE_PDL(kv_attend_kernel<HD, BF16>, dim3(num_sms), dim3(kAttThreads), smem, s, tk, tv, c, a, w, group,
           static_cast<float>(a.scale * 1.4426950408889634));
-  MOE_PDL(kv_merge_kernel<HD, BF16>, dim3(num_sms * 4), dim3(256), 0, s, a, w, group);
+  const int64_t most = std::min<int64_t>(static_cast<int64_t>(b.rows) * group, 2 * kTile);
+  MOE_PDL(kv_merge_kernel<HD, BF16>, dim3(num_sms, static_cast<int>((most + kMergeRows - 1) / kMergeRows)),
+          dim3(256), 0, s, a, w, group);
   return cudaSuccess;
 }
 
