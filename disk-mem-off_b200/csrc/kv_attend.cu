@@ -12,17 +12,19 @@
 // Work.  kv_plan_kernel (one CTA) cuts the entries into units: 256 rows that two
 // warpgroups work on against the same keys ("pair"), or up to 128 rows that one
 // warpgroup works on alone ("single": decode steps and the ends of chunks).  A unit of
-// one kv head costs its number of 128-key tiles.  All tiles are numbered in a row and
+// one kv head costs its number of 64-key tiles and a constant.  All tiles are numbered in a row and
 // cut into equal shares, pairs for 148 CTAs and singles for 2 * 148 warpgroups, so the
 // load is even for any mix of lengths; a unit cut by a share's border leaves fp32
 // partial results that kv_merge_kernel joins in share order (same bits every time).
 //
-// kv_attend_kernel (one CTA an SM, 320 threads): warps 0-3 and 4-7 are the two softmax
+// kv_attend_kernel (one CTA an SM, 384 threads): warps 0-3 and 4-7 are the two softmax
 // warpgroups, a thread a row; warp 8 fetches K and V tiles page by page (TMA, 128-byte
-// swizzle) into one ring; warp 9 issues S = Q K^T (both operands in shared memory, K
-// major) and O += P V (P from TMEM, V as an N-major operand, so that V needs no
-// transposed copy).  TMEM: S0, S1 (128 columns each; P overwrites its S), O0, O1.  While
-// one warpgroup is in its softmax, the tensor cores work for the other.
+// swizzle) into one ring, warp 11 the Q tiles; warps 9 and 10 issue S = Q K^T (both
+// operands in shared memory, K major) and O += P V (P from TMEM, V as an N-major operand,
+// so that V needs no transposed copy), one for each softmax warpgroup: a single issuing
+// warp took 2,590 cycles for a tile of both, most of them between the products.  TMEM: two S buffers of 64 keys for each
+// warpgroup (P overwrites its S) and its O, 512 columns in all.  S runs two tiles ahead
+// of the product with V, so the softmax finds its next S ready.
 #include <cuda_bf16.h>
 #include <math.h>
 
@@ -37,7 +39,8 @@ namespace moe {
 #define KA_LF 2
 #define KA_LP 4
 #endif
-constexpr int kTile = 128;       // keys of a tile, rows of a warpgroup
+constexpr int kTile = 128;       // rows of a warpgroup
+constexpr int kKeys = 64;        // keys of a tile
 constexpr int kPlanT = 1024;     // threads of the plan kernel
 constexpr int kPlanSmem = 512;   // units of a list whose prefix sums fit its shared memory
 
@@ -70,12 +73,11 @@ constexpr int kMergeRows = 16;
 constexpr int kPair = 0, kSingle = 1, kFew = 2, kKinds = 3;
 constexpr int kFewRows = 64;
 // What beginning and ending a unit costs, in tiles of its kind.
-__host__ __device__ constexpr int kind_extra(int k) { return k == kFew ? 3 : 1; }
+__host__ __device__ constexpr int kind_extra(int k) { return 3; }
 // The least share worth a CTA or warpgroup of its own, in cost.
 __host__ __device__ constexpr int kind_least(int k) { return k == kFew ? KA_LF : KA_LP; }
 __host__ __device__ constexpr int kind_rows(int k) { return k == kPair ? 2 * kTile : k == kSingle ? kTile : kFewRows; }
 __host__ __device__ constexpr int kind_shares(int k) { return k == kPair ? 1 : 2; }
-__host__ __device__ constexpr int kind_keys(int k) { return k == kFew ? 64 : kTile; }  // of a tile
 
 struct KaWs {
   size_t start[kKinds], list[kKinds], pre[kKinds], o[kKinds], ml[kKinds], merge, n_merge, total;
@@ -167,11 +169,11 @@ MOE_DEV long long plan_scan(long long v, int busy, long long* total) {
   return v + before;
 }
 
-MOE_DEV int key_tiles(int base, int last_token, int keys) {
+MOE_DEV int key_tiles(int base, int last_token) {
   // tokens visible to the unit's last row, at least one tile (rows that see nothing
   // still have to be written); beyond the table they read as zeros and are masked
   const long long vis = static_cast<long long>(max(base, 0)) + last_token + 1;
-  return static_cast<int>((vis + keys - 1) / keys);
+  return static_cast<int>((vis + kKeys - 1) / kKeys);
 }
 
 // Where the cost w0 lies in a list whose prefix sums (of one kv head) are pre[0 .. n]; T:
@@ -249,7 +251,7 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
     const int rem = rows & (2 * kTile - 1);
     const int na = rows / (2 * kTile) + (rem > kTile ? 1 : 0);
     const bool single = rem > kFewRows && rem <= kTile, few = rem > 0 && rem <= kFewRows;
-    const int tiles = key_tiles(len - m, m - 1, kind_keys(few ? kFew : kSingle));
+    const int tiles = key_tiles(len - m, m - 1);
     // counts (at most 1024 each) in the high bits, cost of a chunk's units in the low 44
     const KaUnit rest{seq, row0, rows - rem, rem, len - m, len, tiles, 0};
     long long total, mine = few ? (1ll << 44) + tiles + kind_extra(kFew) : 0;
@@ -291,7 +293,7 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
         }
         const int4 e = s_entry[lo];
         const int r0 = (j - s_pairs[lo]) * 2 * kTile, r1 = min(r0 + 2 * kTile, e.z * group);
-        u = KaUnit{e.x, e.y, r0, r1 - r0, e.w - e.z, e.w, key_tiles(e.w - e.z, (r1 - 1) / group, kTile), 0};
+        u = KaUnit{e.x, e.y, r0, r1 - r0, e.w - e.z, e.w, key_tiles(e.w - e.z, (r1 - 1) / group), 0};
         w.pair.list[n_pair + j] = u;
         mine = u.tiles + kind_extra(kPair);
       }
@@ -349,18 +351,17 @@ static_assert(5 * kKvMaxSms + kKinds <= kPlanT, "a thread for each share");
 template <int HD>
 struct KaCfg {
   static constexpr int kQ = kTile * HD * 2;      // one warpgroup's Q tile
-  static constexpr int kStage = kTile * HD * 2;  // one K or V tile
-  static constexpr int kStages = HD == 128 ? 5 : 8;
-  static constexpr int kLoads = HD / 64;         // 64-dim blocks of a tile
-  static constexpr int kHalf = kStage / 2;       // 64 keys: a tile of the few-row units,
-  static constexpr int kHalves = kStages;        // whose two rings share the same memory
+  static constexpr int kStage = kKeys * HD * 2;  // one K or V tile
+  static constexpr int kStages = HD == 128 ? 10 : 16;
+  static constexpr int kHalf = kStages / 2;  // of each of the two rings of the other kinds
+  static constexpr int kLoads = HD / 64;          // 64-dim blocks of a tile
   // barriers, and the 8 warps' (max, sum) of 16 rows each
-  static constexpr size_t kSmem = 1024 + 2 * kQ + kStages * kStage + 640 + 1024;
+  static constexpr size_t kSmem = 1024 + 2 * kQ + kStages * kStage + 768 + 1024;
 };
 static_assert(KaCfg<128>::kSmem <= 227 * 1024 && KaCfg<64>::kSmem > 114 * 1024,
               "one CTA, and with it all of TMEM, an SM");
 
-// Twelve warps (8: K / V, 9: MMA, 10 and 11: Q), so that each third is a warpgroup and
+// Twelve warps (8: K / V, 9 and 10: MMA, 11: Q, then K / V), so that each third is a warpgroup and
 // registers can move between them: 384 * 168 at launch = 2 * 128 * 208 + 128 * 80 + rest.
 constexpr int kAttThreads = 384;
 constexpr int kRegsSoftmax = 208, kRegsOther = 80;
@@ -369,7 +370,7 @@ template <int N>
 MOE_DEV void regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 MOE_DEV void regs_fewer() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-constexpr uint32_t kOCols = 2 * kTile;  // TMEM: S0 S1 at 0, 128; O0 O1 at 256, 384
+constexpr uint32_t kOCols = 256;  // TMEM: S of stream s, buffer b at s * 128 + b * 64; O at 256 + s * 128
 
 // Five-dimensional tiled load (dim, row, head, page, layer); a page past the end reads
 // as zeros.
@@ -395,11 +396,11 @@ __host__ __device__ constexpr uint32_t ka_idesc(uint32_t fmt, int n, uint32_t nm
 }
 
 // Descriptor of a V tile as the N-major B operand: rows of a key with 64 dims (128
-// bytes, 128-byte swizzle), 8 keys every 1024 bytes (SBO), the next 64 dims 16 KiB on (LBO).
+// bytes, 128-byte swizzle), 8 keys every 1024 bytes (SBO), the next 64 dims 8 KiB on (LBO).
 MOE_DEV uint64_t nmajor_desc(uint32_t smem_addr) {
   uint64_t d = 0;
   d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFF);
-  d |= static_cast<uint64_t>(16384 >> 4) << 16;
+  d |= static_cast<uint64_t>(kKeys * 128 >> 4) << 16;
   d |= static_cast<uint64_t>(1024 >> 4) << 32;
   d |= static_cast<uint64_t>(1) << 46;
   d |= static_cast<uint64_t>(2) << 61;
@@ -474,35 +475,96 @@ struct KaRing {
   const int layer;
   uint64_t *full, *empty;
   const uint32_t smem;
-  const int stages, keys, bytes, loads;
+  const int stages, bytes, loads;
   volatile int* abort_flag;
+  int st = 0, n = 0;  // next stage, tiles put
+  uint32_t ph = 1;    // parity of the wait for it
   // Tile `tile` of the unit's keys or values into the next stage: boxes of up to 64 rows by
   // 64 dims, a lane each.
-  MOE_DEV bool put(const KaUnit& u, int head, int tile, KaPages& pg, bool val, int& n) {
+  MOE_DEV bool put(const KaUnit& u, int head, int tile, KaPages& pg, bool val) {
     const int lane = threadIdx.x & 31;
-    const int st = n % stages;
-    if (!__all_sync(0xffffffffu, mbar_wait_bounded(&empty[st], ((n / stages) & 1) ^ 1, abort_flag))) return false;
-    const int box = min(c.page, 64);
+    if (!__all_sync(0xffffffffu, mbar_wait_bounded(&empty[st], ph, abort_flag))) return false;
+    const int box = min(c.page, kKeys);
     const int p = lane / loads, kb = lane - p * loads;
-    const int key = tile * keys + p * box;
-    pg.at(c, u, (tile * keys) >> c.page_shift);
+    const int key = tile * kKeys + p * box;
+    pg.at(c, u, (tile * kKeys) >> c.page_shift);
     if (lane == 0) mbar_arrive_expect_tx(&full[st], bytes);
     __syncwarp();
     const int blk = key >> c.page_shift;
     int id = __shfl_sync(0xffffffffu, pg.ids, blk & 31);
-    if (p * box < keys) {
+    if (p * box < kKeys) {
       if (id < 0 || id >= c.pages) {
         // past the sequence's last page: zeros; before it: a hole in the table
         if (key < u.len) record_error(c.err, DEV_BAD_PAGE);
         id = c.pages;
       }
-      tma_load_5d(smem + st * bytes + kb * (keys * 128) + p * box * 128, val ? &tv : &tk, kb * 64,
+      tma_load_5d(smem + st * bytes + kb * (kKeys * 128) + p * box * 128, val ? &tv : &tk, kb * 64,
                   key & (c.page - 1), head, id, layer, &full[st]);
     }
     ++n;
+    if (++st == stages) {
+      st = 0;
+      ph ^= 1;
+    }
     return true;
   }
+  // This share's tiles of the cursor's unit, K two tiles ahead of V as the MMAs take them.
+  MOE_DEV bool put_unit(KaCursor& x, KaPages& pg) {
+    const int nt = min(x.left, x.u.tiles - x.tile);
+    for (int j = -2; j < nt; ++j) {
+      if (j >= 0 && !put(x.u, x.head, x.tile + j, pg, true)) return false;
+      if (j + 2 < nt && !put(x.u, x.head, x.tile + j + 2, pg, false)) return false;
+    }
+    x.skip(nt);
+    return true;
+  }
+  // All copies have landed; with `read` also waits until all stages have been let go.
+  MOE_DEV void drain(bool& read) {
+    const int k = min(n, stages);
+    for (int i = 0; i < k; ++i) {
+      if (st-- == 0) {
+        st = stages - 1;
+        ph ^= 1;
+      }
+      mbar_wait_drain(&full[st], ph ^ 1);
+      if (read) read = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[st], ph ^ 1, abort_flag));
+    }
+    __syncwarp();
+  }
+  MOE_DEV void drain(bool&& read) {
+    bool r = read;
+    drain(r);
+  }
 };
+
+// Up to 128 rows of a unit's Q from packed row `first` on, by a warp, swizzled as the MMA
+// reads them.
+template <int HD>
+MOE_DEV void fetch_q(const KvAttend& a, const KaUnit& u, int head, int group, int first, uint32_t smem) {
+  constexpr int ch = HD / 8, step = 32 / ch;  // 16-byte chunks of a row, rows at a time
+  const int lane = threadIdx.x & 31;
+  int row = lane / ch;
+  const int chunk = lane - row * ch;
+  const int rows = min(u.rows - first, kTile);
+  const uint32_t to = smem + (chunk >> 3) * (kTile * 128);
+  const int dtok = step / group, dhg = step - dtok * group;
+  const int packed = u.r0 + first + row;
+  const int tok = packed / group;
+  int hg = packed - tok * group;
+  const int64_t dwrap = a.qs[0] - group * a.qs[1], dsrc = dtok * a.qs[0] + dhg * a.qs[1];
+  const __half* src = static_cast<const __half*>(a.q) + (u.row0 + static_cast<int64_t>(tok)) * a.qs[0] +
+                      (static_cast<int64_t>(head) * group + hg) * a.qs[1] + chunk * 8;
+#pragma unroll 8
+  for (; row < rows; row += step) {
+    cp_async16(to + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), src);
+    src += dsrc;
+    hg += dhg;
+    if (hg >= group) {
+      hg -= group;
+      src += dwrap;
+    }
+  }
+}
 
 // One lane of a converged warp, the same one every time.
 MOE_DEV bool elect_one() {
@@ -561,10 +623,10 @@ MOE_DEV void tmem_landed(float* v, int n) {
 #pragma unroll
   for (int i = 0; i < n; ++i) asm volatile("" : "+f"(v[i]));
 }
-MOE_DEV void load_s(uint32_t taddr, float (&sc)[kTile]) {
+MOE_DEV void load_s(uint32_t taddr, float (&sc)[kKeys]) {
 #pragma unroll
-  for (int i = 0; i < kTile / 32; ++i) tmem_ld32_start(taddr + i * 32, sc + i * 32);
-  tmem_landed(sc, kTile);
+  for (int i = 0; i < kKeys / 32; ++i) tmem_ld32_start(taddr + i * 32, sc + i * 32);
+  tmem_landed(sc, kKeys);
 }
 
 // ------------------------------------------------------------------ few rows
@@ -719,9 +781,9 @@ struct KaFew {
       if (ends) whole = x.tile + 1 == u.tiles;
       x.next();
       // S = Q K^T of this warp's slice
-      int st = n % C::kHalves;
-      if (!warp_wait(&full[st], (n / C::kHalves) & 1, abort_flag)) return false;
-      uint32_t base = smem_u32(sR) + st * C::kHalf + krow * 128;
+      int st = n % C::kHalf;
+      if (!warp_wait(&full[st], (n / C::kHalf) & 1, abort_flag)) return false;
+      uint32_t base = smem_u32(sR) + st * C::kStage + krow * 128;
       float sc[MT][2][4];
 #pragma unroll
       for (int kg = 0; kg < MT; ++kg) {
@@ -792,18 +854,18 @@ struct KaFew {
       }
       if (ends && x.left > 0) fetch_q(x);  // lands while this unit ends
       // O += P V
-      st = n % C::kHalves;
-      if (!warp_wait(&full[st], (n / C::kHalves) & 1, abort_flag)) return false;
+      st = n % C::kHalf;
+      if (!warp_wait(&full[st], (n / C::kHalf) & 1, abort_flag)) return false;
       if (u.len < slice_end) {
         // keys past the sequence's end: P is zero there, V must be (0 * NaN is not)
         for (int row = max(u.len - key0, slice * kKeys); row < (slice + 1) * kKeys; ++row)
           if (lane < HD / 8)
-            *reinterpret_cast<uint4*>(sR + st * C::kHalf + (lane >> 3) * 8192 + row * 128 + (lane & 7) * 16) =
+            *reinterpret_cast<uint4*>(sR + st * C::kStage + (lane >> 3) * 8192 + row * 128 + (lane & 7) * 16) =
                 make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();
         __syncwarp();
       }
-      base = smem_u32(sR) + st * C::kHalf + vrow * 128;
+      base = smem_u32(sR) + st * C::kStage + vrow * 128;
 #pragma unroll
       for (int kg = 0; kg < MT; ++kg) {
         const uint32_t p[4] = {pack2<BF16>(sc[kg][0][0], sc[kg][0][1]), pack2<BF16>(sc[kg][0][2], sc[kg][0][3]),
@@ -898,45 +960,43 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   uint8_t* sQ = smem;
   uint8_t* sR = sQ + 2 * C::kQ;  // the K / V ring
   uint64_t* bars = reinterpret_cast<uint64_t*>(sR + C::kStages * C::kStage);
-  uint64_t* full = bars;                   // [kStages]
-  uint64_t* empty = bars + C::kStages;     // [kStages]
-  uint64_t* q_full = bars + 2 * C::kStages;  // [2] Q tile of the next unit written
-  uint64_t* s_full = q_full + 2;           // [2] S of a tile done (and every MMA before it)
-  uint64_t* p_full = q_full + 4;           // [2] P of a tile written
-  uint64_t* o_done = q_full + 6;           // [2] P V of a tile done
-  uint64_t* p_half = q_full + 8;           // [2] its first 64 keys
-  uint64_t* mma_done = q_full + 10;
-  uint64_t* few_full = q_full + 11;                 // [2][kHalves] the few-row units' rings
-  uint64_t* few_empty = few_full + 2 * C::kHalves;  // [2][kHalves]
-  uint64_t* joined = few_empty + 2 * C::kHalves;    // [2][2] 4 warps: parts read, parts written
-  uint64_t* ring_free = joined + 4;                 // the MMAs have let all stages go
-  uint64_t* q_free = ring_free + 1;                 // [2] every S of a unit done
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_free + 2);
-  float2* s_ml = reinterpret_cast<float2*>(bars + 80);  // [2][4][16]
+  uint64_t* full = bars;                       // [kStages]
+  uint64_t* empty = full + C::kStages;         // [kStages]
+  uint64_t* half_full = empty + C::kStages;     // [2][kFewStages] the few-row units' rings
+  uint64_t* half_empty = half_full + C::kStages;  // [2][kFewStages]
+  uint64_t* s_full = half_empty + C::kStages;   // [stream][buffer] S of a tile done
+  uint64_t* p_full = s_full + 4;               // [stream][buffer] P of a tile written
+  uint64_t* o_done = s_full + 8;               // [stream][buffer] P V of a tile done
+  uint64_t* joined = s_full + 12;              // [stream][2] 4 warps: parts read, parts written
+  uint64_t* ring_free = s_full + 16;           // the MMAs have let all stages go
+  uint64_t* mma_done = s_full + 17;
+  uint64_t* q_full = s_full + 18;              // [stream] Q tile of a pair written
+  uint64_t* q_free = s_full + 20;              // [stream] every S of a pair done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 22);
+  static_assert((4 * C::kStages + 23) * 8 <= 768, "barriers");
+  float2* s_ml = reinterpret_cast<float2*>(bars + 96);  // [2][4][16]
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kStages; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
+      mbar_init(&empty[i], 2);
+      mbar_init(&half_full[i], 1);
+      mbar_init(&half_empty[i], 4);
     }
-    for (int i = 0; i < 2 * C::kHalves; ++i) {
-      mbar_init(&few_full[i], 1);
-      mbar_init(&few_empty[i], 4);
-    }
-    mbar_init(ring_free, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&joined[i], 4);
-      mbar_init(&joined[i + 2], 4);
-      mbar_init(&q_full[i], 1);
-      mbar_init(&q_free[i], 1);
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
-      mbar_init(&p_half[i], 4);
       mbar_init(&o_done[i], 1);
+      mbar_init(&joined[i], 4);
     }
-    mbar_init(mma_done, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_free[i], 1);
+    }
+    mbar_init(ring_free, 1);
+    mbar_init(mma_done, 2);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -957,100 +1017,41 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   if (warp >= 8) {
   regs_fewer<kRegsOther>();
   if (warp == 8) {
-    // ------------------------------------------------------------ K / V tiles
-    int n = 0;  // tiles put into the ring so far
-    bool ok = true;
-    KaRing ring{c, tk, tv, a.layer, full, empty, smem_u32(sR), C::kStages, kTile, C::kStage, C::kLoads, abort_flag};
-    auto put = [&](const KaUnit& u, int head, int tile, KaPages& pg, bool val) {
-      ok = ring.put(u, head, tile, pg, val, n);
-    };
-    const int4 st_pair = KaCursor::start(w, kPair, cta), st0 = KaCursor::start(w, kSingle, cta),
-               st1 = KaCursor::start(w, kSingle, cta + ctas);
+    // ------------------------------------------------------------ K / V tiles of pairs
     KaCursor x;
-    KaPages px;
-    x.init(w, kPair, st_pair, c.heads);
-    while (ok && x.left > 0) {
-      put(x.u, x.head, x.tile, px, false);
-      if (ok) put(x.u, x.head, x.tile, px, true);
-      x.next();
-    }
-    KaCursor y;
-    KaPages py;
-    x.init(w, kSingle, st0, c.heads);
-    y.init(w, kSingle, st1, c.heads);
-    if (ok && x.left > 0) put(x.u, x.head, x.tile, px, false);
-    if (ok && y.left > 0) put(y.u, y.head, y.tile, py, false);
-    while (ok && (x.left > 0 || y.left > 0)) {
-      if (x.left > 0) {
-        put(x.u, x.head, x.tile, px, true);
-        x.next();
-        if (ok && x.left > 0) put(x.u, x.head, x.tile, px, false);
-      }
-      if (ok && y.left > 0) {
-        put(y.u, y.head, y.tile, py, true);
-        y.next();
-        if (ok && y.left > 0) put(y.u, y.head, y.tile, py, false);
-      }
-    }
+    x.init(w, kPair, KaCursor::start(w, kPair, cta), c.heads);
+    KaRing ring{c, tk, tv, a.layer, full, empty, smem_u32(sR), C::kStages, C::kStage, C::kLoads, abort_flag};
+    KaPages pg;
+    bool ok = true;
+    while (ok && x.left > 0) ok = ring.put_unit(x, pg);
     if (!ok) {
       *abort_flag = 1;
       if (lane == 0) record_error(c.err, DEV_TIMEOUT_EMPTY);
     }
     // every copy must land before the CTA exits, and every MMA have read its stage before
-    // the few-row units use it
-    for (int j = max(n - C::kStages, 0); j < n; ++j) {
-      if (ok) ok = warp_wait(&empty[j % C::kStages], (j / C::kStages) & 1, abort_flag);
-      mbar_wait_drain(&full[j % C::kStages], (j / C::kStages) & 1);
-    }
-    __syncwarp();
+    // the other kinds use it
+    ring.drain(ok);
     if (ok && lane == 0) mbar_arrive(ring_free);
   }
-  if (warp >= 10) {
-    // ------------------------------------------------------------ Q tiles of a stream
-    // 128 rows, swizzled as the MMA reads them, as soon as the S products of the unit
-    // before are done: under its last softmax and its epilogue
-    const int s = warp - 10;
-    const __half* q16 = static_cast<const __half*>(a.q);
-    constexpr int ch = HD / 8, step = 32 / ch;  // 16-byte chunks of a row, rows at a time
-    const int row_in = lane / ch, chunk = lane - row_in * ch;
-    const uint32_t to = smem_u32(sQ) + s * C::kQ + (chunk >> 3) * 16384;
-    const int dtok = step / group, dhg = step - dtok * group;
-    const int4 st_pair = KaCursor::start(w, kPair, cta), st_single = KaCursor::start(w, kSingle, cta + s * ctas);
+  if (warp == 11) {
+    // ------------------------------------------------------------ Q tiles of pairs
+    // as soon as every S of the unit before is done: under its last softmax and epilogue
+    KaCursor x;
+    x.init(w, kPair, KaCursor::start(w, kPair, cta), c.heads);
     bool ok = true;
-    int units = 0;  // begun so far
-#pragma unroll 1
-    for (int kind = kPair; kind <= kSingle && ok; ++kind) {
-      const int part = kind ? 0 : s;
-      KaCursor x;
-      x.init(w, kind, kind ? st_single : st_pair, c.heads);
-      while (ok && x.left > 0) {
-        if (units > 0 && !warp_wait(&q_free[s], (units - 1) & 1, abort_flag)) {
-          ok = false;
-          break;
+    for (int n = 0; ok && x.left > 0; ++n) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if (ok && n > 0) ok = warp_wait(&q_free[s], (n - 1) & 1, abort_flag);
+        if (ok) {
+          fetch_q<HD>(a, x.u, x.head, group, s * kTile, smem_u32(sQ) + s * C::kQ);
+          cp_async_wait();
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&q_full[s]);
         }
-        const KaUnit& u = x.u;
-        int row = row_in, packed = u.r0 + part * kTile + row;
-        int tok = packed / group, hg = packed - tok * group;
-        const __half* src = q16 + static_cast<long long>(u.row0) * a.qs[0] +
-                            static_cast<long long>(x.head) * group * a.qs[1] + chunk * 8;
-        const int rows = min(u.rows - part * kTile, kTile);
-#pragma unroll 8
-        for (; row < rows; row += step) {
-          cp_async16(to + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), src + tok * a.qs[0] + hg * a.qs[1]);
-          tok += dtok;
-          hg += dhg;
-          if (hg >= group) {
-            hg -= group;
-            ++tok;
-          }
-        }
-        cp_async_wait();
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&q_full[s]);
-        ++units;
-        x.skip(min(x.left, x.u.tiles - x.tile));
       }
+      x.skip(min(x.left, x.u.tiles - x.tile));
     }
     if (!ok) {
       *abort_flag = 1;
@@ -1058,183 +1059,155 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     }
     __syncwarp();
   }
-  if (warp == 8 || warp == 10) {
-    // ------------------------------------------------------------ few rows: 64-key tiles
+  if (warp == 8 || warp == 11) {
+    // ------------------------------------------------------------ K / V tiles of singles, few rows
     // a ring and a producer warp for each of the two warpgroups
-    const int r = warp == 10;
-    KaCursor x;
-    x.init(w, kFew, KaCursor::start(w, kFew, cta + r * ctas), c.heads);
-    if (x.left > 0) {
-      // the other kinds may run for long: a limit of about two minutes
+    const int r = warp == 11;
+    KaCursor x, y;
+    x.init(w, kSingle, KaCursor::start(w, kSingle, cta + r * ctas), c.heads);
+    y.init(w, kFew, KaCursor::start(w, kFew, cta + r * ctas), c.heads);
+    if (x.left > 0 || y.left > 0) {
+      // the pairs may run for long: a limit of about two minutes
       bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(ring_free, 0, abort_flag, 128 * kWaitLimitCycles));
-      KaRing ring{c, tk, tv, a.layer, few_full + r * C::kHalves, few_empty + r * C::kHalves,
-                  smem_u32(sR) + r * C::kHalves * C::kHalf, C::kHalves, 64, C::kHalf, C::kLoads, abort_flag};
-      KaPages px;
-      int n = 0;
-      while (ok && x.left > 0) {
-        ok = ring.put(x.u, x.head, x.tile, px, false, n);
-        if (ok) ok = ring.put(x.u, x.head, x.tile, px, true, n);
-        x.next();
+      KaRing ring{c, tk, tv, a.layer, half_full + r * C::kHalf, half_empty + r * C::kHalf,
+                  smem_u32(sR) + r * C::kHalf * C::kStage, C::kHalf, C::kStage, C::kLoads, abort_flag};
+      KaPages pg;
+      while (ok && x.left > 0) ok = ring.put_unit(x, pg);
+      while (ok && y.left > 0) {
+        ok = ring.put(y.u, y.head, y.tile, pg, false) && ring.put(y.u, y.head, y.tile, pg, true);
+        y.next();
       }
       if (!ok) {
         *abort_flag = 1;
         if (lane == 0) record_error(c.err, DEV_TIMEOUT_EMPTY);
       }
-      for (int j = max(n - C::kHalves, 0); j < n; ++j)
-        mbar_wait_drain(&ring.full[j % C::kHalves], (j / C::kHalves) & 1);
-      __syncwarp();
+      ring.drain(false);
     }
-  } else if (warp == 9) {
-    // ------------------------------------------------------------ MMA issue
+  } else if (warp == 9 || warp == 10) {
+    // ------------------------------------------------------------ Q and MMAs of a stream
+    const int s = warp - 9;
     constexpr uint32_t fmt = BF16 ? 1 : 0;
-    constexpr uint32_t id_s = ka_idesc(fmt, kTile, 0), id_o = ka_idesc(fmt, HD, 1);
-    const uint32_t aq = uniform(smem_u32(sQ)), ar = uniform(smem_u32(sR)), tm = uniform(tmem);
+    constexpr uint32_t id_s = ka_idesc(fmt, kKeys, 0), id_o = ka_idesc(fmt, HD, 1);
+    const bool lead = elect_one();
+    const int leader = __ffs(__ballot_sync(0xffffffffu, lead)) - 1;
+    const uint32_t t_s = uniform(tmem + s * kTile), t_o = t_s + kOCols;
+    const uint32_t q_smem = smem_u32(sQ) + s * C::kQ;
+    const uint64_t dq = sw128_desc(q_smem);
+    const int4 start_pair = KaCursor::start(w, kPair, cta), start_single = KaCursor::start(w, kSingle, cta + s * ctas);
     bool ok = true;
-    int n = 0;             // ring tiles taken
-    int np[2] = {0, 0};    // P tiles taken, by stream
-    int nq[2] = {0, 0};    // units begun
-    // the next ring tile has landed
-    auto take = [&]() -> int {
-      const int st = n % C::kStages;
-      if (!warp_wait(&full[st], (n / C::kStages) & 1, abort_flag)) ok = false;
-      ++n;
-      return st;
-    };
-    // S of stream s from Q tile s and ring stage st; begins / ends: the unit's first / last
-    auto issue_s = [&](int s, int st, bool begins, bool ends) {
-      if (begins) {
-        if (!warp_wait(&q_full[s], nq[s] & 1, abort_flag)) ok = false;
-        ++nq[s];
-      }
-      tc_fence_after();
-      const uint64_t dq = sw128_desc(aq + s * C::kQ), dk = sw128_desc(ar + uniform(st) * C::kStage);
-      if (ok && elect_one()) {
-#pragma unroll
-        for (int k = 0; k < HD / 16; ++k) {
-          const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;  // in the descriptors' units
-          tc_mma_f16(tm + s * kTile, dq + off, dk + off, id_s, k > 0 ? 1u : 0u);
+    int ns = 0, np = 0, nq = 0;  // S tiles, P tiles, units so far
+    // The units of a cursor from a ring.  One lane waits and issues: S two tiles ahead of
+    // P V, P V of the unit's last two tiles apart, with rows of V past the sequence's end
+    // cleared first (by the whole warp).  Q comes from warp 11 for pairs; singles, whose
+    // streams do not wait for each other, fetch their own.
+    auto units = [&](KaCursor x, bool own_q, uint64_t* fullb, uint64_t* emptyb, uint8_t* ring, int stages,
+                     int extra_arrivals) {
+      const uint64_t dk0 = sw128_desc(smem_u32(ring)), dv0 = nmajor_desc(smem_u32(ring));
+      int st = 0;
+      uint32_t ph = 0;
+      auto let_go = [&](int at) {
+        for (int i = 0; i < extra_arrivals; ++i) mbar_arrive(&emptyb[at]);
+        tc_commit(&emptyb[at]);
+      };
+      auto pass = [&]() {
+        if (++st == stages) {
+          st = 0;
+          ph ^= 1;
         }
-        tc_commit(&s_full[s]);
-        if (ends) tc_commit(&q_free[s]);
-      }
-      __syncwarp();
-    };
-    // keys past the sequence's end hold whatever was in the page: their rows of V are
-    // zeroed, since P is zero there but 0 * NaN is not
-    auto clear_v = [&](int st, const KaUnit& u, int tile) {
-      const int valid = u.len - tile * kTile;
-      if (valid >= kTile) return;
-      const int from = max(valid, 0) * 128;
-      for (int kb = 0; kb < C::kLoads; ++kb)
-        for (int o = from + lane * 16; o < 16384; o += 512)
-          *reinterpret_cast<uint4*>(sR + st * C::kStage + kb * 16384 + o) = make_uint4(0, 0, 0, 0);
-      fence_proxy_async_smem();
-      __syncwarp();
-    };
-    auto issue_o = [&](int s, int st, bool first) {
-      const uint64_t dv = nmajor_desc(ar + uniform(st) * C::kStage);
-      const uint32_t add = uniform(first ? 0u : 1u);
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        if (ok && !warp_wait(half ? &p_full[s] : &p_half[s], np[s] & 1, abort_flag)) ok = false;
+      };
+      auto product = [&](bool first) -> bool {  // O += P V
+        const int buf = np & 1;
+        if (!mbar_wait_bounded(&fullb[st], ph, abort_flag) ||
+            !mbar_wait_bounded(&p_full[2 * s + buf], (np >> 1) & 1, abort_flag))
+          return false;
         tc_fence_after();
-        if (ok && elect_one()) {
+        const uint64_t dv = dv0 + static_cast<uint32_t>(st * (C::kStage >> 4));
 #pragma unroll
-          for (int k = half * 4; k < half * 4 + 4; ++k)
-            tc_mma_f16_ts(tm + kOCols + s * kTile, tm + s * kTile + k * 8, dv + k * (2048 >> 4), id_o,
-                          k > 0 ? 1u : add);
-          if (half) tc_commit(&o_done[s]);
+        for (int k = 0; k < kKeys / 16; ++k)
+          tc_mma_f16_ts(t_o, t_s + buf * kKeys + k * 8, dv + k * (2048 >> 4), id_o, first && k == 0 ? 0u : 1u);
+        tc_commit(&o_done[2 * s + buf]);
+        let_go(st);
+        ++np;
+        pass();
+        return true;
+      };
+      while (ok && x.left > 0) {
+        const int nt = min(x.left, x.u.tiles - x.tile);
+        const int behind = max(nt - 2, 0);
+        if (own_q) {
+          if (ns > 0 && !warp_wait(&s_full[2 * s + ((ns - 1) & 1)], ((ns - 1) >> 1) & 1, abort_flag)) ok = false;
+          fetch_q<HD>(a, x.u, x.head, group, 0, q_smem);
+          cp_async_wait();
+          fence_proxy_async_smem();
+          __syncwarp();
+        } else {
+          if (!warp_wait(&q_full[s], nq & 1, abort_flag)) ok = false;
+          ++nq;
+        }
+        if (lead) {
+          for (int j = -2; ok && j < behind; ++j) {
+            if (j >= 0) ok = product(j == 0);
+            if (ok && j + 2 < nt) {  // S into buffer ns & 1, which P of two tiles before has left
+              ok = mbar_wait_bounded(&fullb[st], ph, abort_flag);
+              if (!ok) break;
+              tc_fence_after();
+              const int buf = ns & 1;
+              const uint64_t dk = dk0 + static_cast<uint32_t>(st * (C::kStage >> 4));
+#pragma unroll
+              for (int k = 0; k < HD / 16; ++k)  // offsets in the descriptors' units of 16 bytes
+                tc_mma_f16(t_s + buf * kKeys, dq + (((k >> 2) * 16384 + (k & 3) * 32) >> 4),
+                           dk + (((k >> 2) * kKeys * 128 + (k & 3) * 32) >> 4), id_s, k > 0 ? 1u : 0u);
+              tc_commit(&s_full[2 * s + buf]);
+              if (j + 3 == nt && !own_q) tc_commit(&q_free[s]);
+              let_go(st);
+              ++ns;
+              pass();
+            }
+          }
         }
         __syncwarp();
+        // what the one lane counted
+        ok = __shfl_sync(0xffffffffu, ok, leader);
+        st = __shfl_sync(0xffffffffu, st, leader);
+        ph = __shfl_sync(0xffffffffu, ph, leader);
+        ns = __shfl_sync(0xffffffffu, ns, leader);
+        np = __shfl_sync(0xffffffffu, np, leader);
+        for (int j = behind; ok && j < nt; ++j) {
+          // keys past the sequence's end hold whatever was in the page: their rows of V
+          // are zeroed, since P is zero there but 0 * NaN is not
+          const int valid = x.u.len - (x.tile + j) * kKeys;
+          if (valid < kKeys) {
+            if (!warp_wait(&fullb[st], ph, abort_flag)) {
+              ok = false;
+              break;
+            }
+            for (int kb = 0; kb < C::kLoads; ++kb)
+              for (int o = max(valid, 0) * 128 + lane * 16; o < kKeys * 128; o += 512)
+                *reinterpret_cast<uint4*>(ring + st * C::kStage + kb * kKeys * 128 + o) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          if (lead) ok = product(j == 0);
+          __syncwarp();
+          ok = __shfl_sync(0xffffffffu, ok, leader);
+          st = __shfl_sync(0xffffffffu, st, leader);
+          ph = __shfl_sync(0xffffffffu, ph, leader);
+          np = __shfl_sync(0xffffffffu, np, leader);
+        }
+        x.skip(nt);
       }
-      ++np[s];
     };
-    auto release = [&](int st) {
-      uint64_t* bar = &empty[uniform(st)];
-      if (ok && elect_one()) tc_commit(bar);
-      __syncwarp();
-    };
-    // pairs: both streams read the same K and V tiles.  At a unit's end the next S (which
-    // waits for the next Q) comes after both products with V.
-    const int4 st_pair = KaCursor::start(w, kPair, cta);
-    const int4 st_single[2] = {KaCursor::start(w, kSingle, cta), KaCursor::start(w, kSingle, cta + ctas)};
     KaCursor x;
-    x.init(w, kPair, st_pair, c.heads);
-    if (x.left > 0) {
-      int kst = take();
-      const bool one = x.ends_unit();
-      if (ok) issue_s(0, kst, true, one);
-      if (ok) issue_s(1, kst, true, one);
-      if (ok) release(kst);
-      bool first = true;
-      while (ok) {
-        const KaUnit u = x.u;
-        const int tile = x.tile;
-        const bool ends = x.ends_unit();
-        x.next();
-        const bool more = x.left > 0;
-        const int vst = take();
-        if (!ok) break;
-        clear_v(vst, u, tile);
-        issue_o(0, vst, first);
-        if (ok && more && !ends) {
-          kst = take();
-          if (ok) issue_s(0, kst, false, x.ends_unit());
-        }
-        if (ok) issue_o(1, vst, first);
-        if (ok) release(vst);
-        if (ok && more && ends) {
-          kst = take();
-          if (ok) issue_s(0, kst, true, x.ends_unit());
-        }
-        if (ok && more) {
-          issue_s(1, kst, ends, x.ends_unit());
-          if (ok) release(kst);
-        }
-        first = ends;
-        if (!more) break;
-      }
-    }
-    // singles: each stream has its own units
-    KaCursor y[2];
-    bool first[2] = {true, true};
-#pragma unroll
-    for (int s = 0; s < 2; ++s) y[s].init(w, kSingle, st_single[s], c.heads);
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      if (ok && y[s].left > 0) {
-        const int st = take();
-        if (ok) issue_s(s, st, true, y[s].ends_unit());
-        if (ok) release(st);
-      }
-    }
-    while (ok && (y[0].left > 0 || y[1].left > 0)) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        if (!ok || y[s].left <= 0) continue;
-        const bool ends = y[s].ends_unit();
-        const int vst = take();
-        if (!ok) break;
-        clear_v(vst, y[s].u, y[s].tile);
-        issue_o(s, vst, first[s]);
-        if (ok) release(vst);
-        first[s] = ends;
-        y[s].next();
-        if (ok && y[s].left > 0) {
-          const int kst = take();
-          if (ok) issue_s(s, kst, ends, y[s].ends_unit());
-          if (ok) release(kst);
-        }
-      }
-    }
+    x.init(w, kPair, start_pair, c.heads);
+    units(x, false, full, empty, sR, C::kStages, 0);
+    x.init(w, kSingle, start_single, c.heads);
+    if (ok) units(x, true, half_full + s * C::kHalf, half_empty + s * C::kHalf, sR + s * C::kHalf * C::kStage, C::kHalf, 3);
     if (!ok) {
       *abort_flag = 1;
       if (lane == 0) record_error(c.err, DEV_TIMEOUT_FULL);
     }
-    if (elect_one()) {
-      tc_commit(mma_done);  // no MMA may still write TMEM when it is released
-      mbar_wait_drain(mma_done, 0);
-    }
+    if (lead) tc_commit(mma_done);  // no MMA may still write TMEM when it is released
+    mbar_wait_drain(mma_done, 0);
     __syncwarp();
   }
   } else {
@@ -1275,27 +1248,35 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         bool first = true, whole = true;
         for (bool ends = false; !ends; first = false) {
           ends = x.ends_unit();
-          const int key0 = x.tile * kTile;
+          const int key0 = x.tile * kKeys;
           if (ends) whole = x.tile + 1 == u.tiles;
           x.next();
-          if (!warp_wait(&s_full[s], nt & 1, abort_flag)) {
+          const int buf = nt & 1;
+          const uint32_t t_sb = t_s + buf * kKeys;
+          if (!warp_wait(&s_full[2 * s + buf], (nt >> 1) & 1, abort_flag)) {
             ok = false;
             break;
           }
           tc_fence_after();
           if (any) {
-            float sc[kTile];
-            load_s(t_s, sc);
+            float sc[kKeys];
+            load_s(t_sb, sc);
             const int lim = seen - key0;
-            if (__any_sync(0xffffffffu, lim < kTile)) {
+            if (__any_sync(0xffffffffu, lim < kKeys)) {
 #pragma unroll
-              for (int j = 0; j < kTile; ++j)
+              for (int j = 0; j < kKeys; ++j)
                 if (j >= lim) sc[j] = -INFINITY;
             }
-            float mx[4] = {sc[0], sc[1], sc[2], sc[3]};
+            float mx[8];
 #pragma unroll
-            for (int j = 4; j < kTile; ++j) mx[j & 3] = fmaxf(mx[j & 3], sc[j]);
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;
+            for (int j = 0; j < 8; ++j) mx[j] = fmaxf(sc[j], fmaxf(sc[j + 8], sc[j + 16]));
+#pragma unroll
+            for (int j = 24; j < kKeys; j += 16)
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                mx[k] = j + 8 < kKeys ? fmaxf(mx[k], fmaxf(sc[j + k], sc[j + 8 + k])) : fmaxf(mx[k], sc[j + k]);
+            const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
+                                    fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]))) * scale_log2;
             // m, the maximum that P, l and O refer to, moves (and l and O are rescaled)
             // only when it grows by more than 2^8
             const bool grow = valid && top - m > 8.f;
@@ -1305,7 +1286,12 @@ __global__ void __launch_bounds__(kAttThreads, 1)
               m = top;
             }
             if (!first && __any_sync(0xffffffffu, grow)) {
-              // s_full of this tile also says that O is complete up to the one before
+              // O must be complete up to the tile before (s_full says so up to two before)
+              if (!warp_wait(&o_done[2 * s + (buf ^ 1)], ((nt - 1) >> 1) & 1, abort_flag)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
 #pragma unroll
               for (int i = 0; i < HD / 16; ++i) {
                 float o[16];
@@ -1315,13 +1301,12 @@ __global__ void __launch_bounds__(kAttThreads, 1)
                 tmem_st16(t_o + i * 16, o);
               }
             }
-            // P in four chunks of 32 keys: the conversions and TMEM stores of one run
-            // under the exponentials of the next, and the first 64 keys are handed to
-            // the MMA warp while the rest is computed
+            // P in chunks of 32 keys: the conversions and TMEM stores of one run under the
+            // exponentials of the next
             const float ref = m == -INFINITY ? 0.f : m - shift;
             const uint64_t scale2 = pair_of(scale_log2, scale_log2), nref2 = pair_of(-ref, -ref);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < kKeys / 32; ++i) {
               uint32_t pk[16];
 #pragma unroll
               for (int j = 0; j < 16; ++j) {
@@ -1331,35 +1316,26 @@ __global__ void __launch_bounds__(kAttThreads, 1)
                 e[1] = exp2_ftz(x2.y);
                 pk[j] = pack2<BF16>(e[0], e[1]);
               }
-              if (i == 2) {
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_half[s]);
-              }
-              tmem_st16_start(t_s + i * 16, pk);
+              tmem_st16_start(t_sb + i * 16, pk);
             }
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[s]);
-            // the row sum, off the path to the next product
+            if (lane == 0) mbar_arrive(&p_full[2 * s + buf]);
+            // the row sum, off the path to the product with V
             uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
-            for (int j = 0; j < kTile / 2; ++j) sum[j & 3] = add_pair(sum[j & 3], pair_of(sc[2 * j], sc[2 * j + 1]));
+            for (int j = 0; j < kKeys / 2; ++j) sum[j & 3] = add_pair(sum[j & 3], pair_of(sc[2 * j], sc[2 * j + 1]));
             const float2 sum2 = split_pair(add_pair(add_pair(sum[0], sum[1]), add_pair(sum[2], sum[3])));
             l = l * alpha + (sum2.x + sum2.y);
           } else {
             tc_fence_before();
-            if (lane == 0) {
-              mbar_arrive(&p_half[s]);
-              mbar_arrive(&p_full[s]);
-            }
+            if (lane == 0) mbar_arrive(&p_full[2 * s + buf]);
           }
           ++nt;
         }
         if (!ok) break;
-        if (!warp_wait(&o_done[s], (nt - 1) & 1, abort_flag)) {
+        if (!warp_wait(&o_done[2 * s + ((nt - 1) & 1)], ((nt - 1) >> 1) & 1, abort_flag)) {
           ok = false;
           break;
         }
@@ -1368,7 +1344,8 @@ __global__ void __launch_bounds__(kAttThreads, 1)
           if (whole && !cut_front) {
             const long long row = static_cast<long long>(u.row0) + tok;
             const int h = head * group + hg;
-            const float inv = l > 0.f ? 1.f / l : 0.f;
+            const bool saw = m != -INFINITY;  // else the row sees no token
+            const float inv = saw ? 1.f / l : 0.f;
             // a thread writes its own row: its 32 lanes meet 32 lines in every store, so
             // the stores are as wide as they can be
             __half* dst = out16 + row * a.os[0] + h * a.os[1];
@@ -1382,7 +1359,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
                 uint32_t pk[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                  pk[j] = l > 0.f ? pack2<BF16>(o[k * 16 + 2 * j] * inv, o[k * 16 + 2 * j + 1] * inv) : 0u;
+                  pk[j] = saw ? pack2<BF16>(o[k * 16 + 2 * j] * inv, o[k * 16 + 2 * j + 1] * inv) : 0u;
                 if (valid && wide) {
                   store32(dst + i * 32 + k * 16, pk);
                 } else if (valid) {
@@ -1394,7 +1371,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
             }
             if (valid && a.lse)
               a.lse[row * a.ls[0] + h * a.ls[1]] =
-                  l > 0.f ? (m - shift + log2f(l)) * 0.6931471805599453f : -INFINITY;
+                  saw ? (m - shift + log2f(l)) * 0.6931471805599453f : -INFINITY;
           } else {
             // a piece: unnormalised, to the share's slot 0 (its first unit) or 1 (its last)
             const KaList l_k = w.kind(kind);
@@ -1414,7 +1391,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
                 }
               }
             }
-            if (valid) l_k.ml[slot] = make_float2(l > 0.f ? m - shift : -INFINITY, l);
+            if (valid) l_k.ml[slot] = m == -INFINITY ? make_float2(-INFINITY, 0.f) : make_float2(m - shift, l);
           }
         }
         tc_fence_before();  // O is read: the next unit's first product may overwrite it
@@ -1423,9 +1400,10 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     }
     // few rows: this warpgroup's share
     if (ok) {
-      KaFew<HD, BF16> f{c, a, w, group, scale_log2, sQ + s * C::kQ, sR + s * C::kHalves * C::kHalf,
-                        few_full + s * C::kHalves, few_empty + s * C::kHalves, joined + 2 * s, s_ml + s * 64,
+      KaFew<HD, BF16> f{c, a, w, group, scale_log2, sQ + s * C::kQ, sR + s * C::kHalf * C::kStage,
+                        half_full + s * C::kHalf, half_empty + s * C::kHalf, joined + 2 * s, s_ml + s * 64,
                         abort_flag};
+      f.n = 2 * st_single.w;  // the ring has gone round for the singles
       const int share = cta + s * ctas;
       KaCursor x;
       x.init(w, kFew, st_few, c.heads);
