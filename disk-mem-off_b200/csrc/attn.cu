@@ -26,6 +26,7 @@
 #include <string>
 
 #include "common.cuh"
+#include "kv_internal.h"
 #include "moe_internal.h"
 
 namespace moe {
@@ -63,6 +64,32 @@ struct AttnWs {
 };
 
 static size_t a256(size_t v) { return (v + 255) & ~size_t(255); }
+
+// Workspace of a forward over the paged cache: q and o rows by token, the place of each
+// token's keys and values, and the attention's own scratch.
+struct AttnCachedWs {
+  size_t rms, h16, qkv, rope, slot, q, o16, oplanes, attend, total;
+  int s1, s2;
+};
+
+static AttnCachedWs attn_cached_ws(const AttnPlan& a, const MoeKvCache& c, int T, int n_seqs) {
+  AttnCachedWs w{};
+  w.s1 = dense_gemm_splits(a.nqkv, T, a.H, a.num_sms);
+  w.s2 = dense_gemm_splits(a.H, T, a.nout, a.num_sms);
+  size_t o = 0;
+  auto take = [&](size_t b) { const size_t at = o; o = a256(o + b); return at; };
+  w.rms = take(static_cast<size_t>(T) * 4);
+  w.h16 = take(static_cast<size_t>(T) * a.H * 2);
+  w.qkv = take(static_cast<size_t>(w.s1) * T * a.nqkv * 4);
+  w.rope = take(static_cast<size_t>(T) * (a.hd / 2) * 8);
+  w.slot = take(static_cast<size_t>(T) * 8);
+  w.q = take(static_cast<size_t>(T) * a.nout * 2);
+  w.o16 = take(static_cast<size_t>(T) * a.nout * 2);
+  w.oplanes = take(static_cast<size_t>(w.s2) * T * a.H * 4);
+  w.attend = take(kv_attend_workspace(c.v, a.nh, T, n_seqs, c.num_sms));
+  w.total = o;
+  return w;
+}
 
 static AttnWs attn_ws(const AttnPlan& a, int T) {
   AttnWs w{};
@@ -105,12 +132,15 @@ MOE_DEV void load_vec(const float* __restrict__ p, float (&out)[V]) {
 // in float64, angles rounded to float32) to their first `rot` dims, then writes
 // q and k as f16 rows [head][tpad][hd] and v transposed [kv head][hd][tpad] (the
 // K-major B operand of O += P V).  Rows past T are written as zeros.
-template <int HD>
+// CACHED: q rows [token][head][hd] instead, k and v into the paged cache at slot[token] =
+// (page, place in the page), page < 0: nowhere; no rows past T.
+template <int HD, bool CACHED>
 __global__ void __launch_bounds__(256) attn_qkv_kernel(
     const float* __restrict__ planes, int nsplit, int T, int tpad, int nh, int nkv,
     const float* __restrict__ bias, const float* __restrict__ qn, const float* __restrict__ kn,
     int rot, const float2* __restrict__ rope, float eps, __half* __restrict__ q16,
-    __half* __restrict__ k16, __half* __restrict__ v16) {
+    __half* __restrict__ k16, __half* __restrict__ v16, const KvView cache, int layer,
+    const int2* __restrict__ slot) {
   pdl_enter();
   constexpr int V = HD / 32;
   __shared__ float sh[8][HD];
@@ -218,6 +248,20 @@ __global__ void __launch_bounds__(256) attn_qkv_kernel(
       __half* dst = kind == 0 ? q16 + (static_cast<size_t>(hh) * tpad + t) * HD
                   : kind == 1 ? k16 + (static_cast<size_t>(hh - nh) * tpad + t) * HD
                               : v16 + (static_cast<size_t>(hh - nh - nkv) * tpad + t) * HD;
+      if constexpr (CACHED) {
+        const int2 at = slot[t];
+        if (kind == 0) {
+          dst = q16 + (static_cast<size_t>(t) * nh + hh) * HD;
+        } else if (at.x < 0) {
+          continue;
+        } else if (kind == 1) {
+          dst = reinterpret_cast<__half*>(cache.k + layer * cache.ks[0] + at.x * cache.ks[1] +
+                                          (hh - nh) * cache.ks[2] + at.y * cache.ks[3]);
+        } else {
+          dst = reinterpret_cast<__half*>(cache.v + layer * cache.vs[0] + at.x * cache.vs[1] +
+                                          (hh - nh - nkv) * cache.vs[2] + at.y * cache.vs[3]);
+        }
+      }
       __half2 h2[V / 2];
   #pragma unroll
       for (int i = 0; i < V / 2; ++i) h2[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
@@ -241,6 +285,40 @@ __global__ void __launch_bounds__(256) attn_rope_kernel(float2* __restrict__ rop
   const float ang = static_cast<float>(static_cast<double>(t) * freq);
   rope[i] = make_float2(static_cast<float>(cos(static_cast<double>(ang))),
                         static_cast<float>(sin(static_cast<double>(ang))));
+}
+
+// The same for rows of the paged cache, at their own positions, and the place of each
+// row's keys and values.  A warp per row; rows that belong to no sequence (or whose page is
+// missing) get position 0 and no place.
+__global__ void __launch_bounds__(128) attn_place_kernel(const KvView c, const KvBatch b, float2* __restrict__ rope,
+                                                         int2* __restrict__ slot, int half, float theta) {
+  pdl_enter();
+  const int lane = threadIdx.x & 31;
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (r >= b.rows) return;
+  const int e = r < b.q_start[b.n] ? entry_of_row(b.q_start, b.n, r) : -1;
+  int64_t pos = 0;
+  int2 at = make_int2(-1, 0);
+  if (e >= 0) {
+    const int s = b.seqs[e];
+    if (s >= 0 && s < c.nseq) {
+      pos = static_cast<int64_t>(c.len[s]) - (b.q_start[e + 1] - r);
+      const int64_t blk = pos >> c.page_shift;
+      if (pos >= 0 && blk < c.max_blocks)
+        at = make_int2(c.table[static_cast<int64_t>(s) * c.max_blocks + blk], static_cast<int>(pos & (c.page - 1)));
+      if (at.x >= c.pages) at.x = -1;
+    }
+    if (at.x < 0 && lane == 0)
+      record_error(c.err, s < 0 || s >= c.nseq ? DEV_BAD_SEQ : pos < 0 ? DEV_BAD_LENGTH : DEV_BAD_PAGE);
+    if (pos < 0) pos = 0;
+  }
+  if (lane == 0) slot[r] = at;
+  for (int j = lane; j < half; j += 32) {
+    const double freq = 1.0 / pow(static_cast<double>(theta), static_cast<double>(j) / static_cast<double>(half));
+    const float ang = static_cast<float>(static_cast<double>(pos) * freq);
+    rope[static_cast<int64_t>(r) * half + j] = make_float2(static_cast<float>(cos(static_cast<double>(ang))),
+                                                           static_cast<float>(sin(static_cast<double>(ang))));
+  }
 }
 
 // v [kv head][tpad][HD] -> vt [kv head][HD][tpad] (the K-major B operand of P V),
@@ -629,10 +707,12 @@ __global__ void __launch_bounds__(kFaThreads, 1) attn_fwd_kernel(const __grid_co
 // out = x + sum_s planes[s] (the o_proj K-split planes, added in split order)
 __global__ void __launch_bounds__(256) attn_out_kernel(const float* __restrict__ x,
                                                        const float* __restrict__ planes, int nsplit,
-                                                       size_t n, float* __restrict__ out) {
+                                                       size_t n, float* __restrict__ out,
+                                                       const int* __restrict__ rows, int H) {
   pdl_enter();
-  // n is a multiple of 4 (H is a multiple of 64): float4 at a time, planes in order
-  const size_t n4 = n / 4;
+  // n is a multiple of 4 (H is a multiple of 64): float4 at a time, planes in order; with
+  // rows only its first *rows rows
+  const size_t n4 = (rows ? min(n, static_cast<size_t>(max(*rows, 0)) * H) : n) / 4;
   for (size_t i = blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x; i < n4;
        i += static_cast<size_t>(gridDim.x) * blockDim.x) {
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -665,12 +745,12 @@ static cudaError_t attn_launch(const AttnPlan& a, const AttnWs& w, char* ws, con
   // token's heads in groups of 8 across CTAs at short ones
   const int groups = (a.nh + 2 * a.nkv + 7) / 8;
   const int gy = std::max(1, std::min(groups, (8 * a.num_sms + w.tpad - 1) / w.tpad));
-  MOE_PDL(attn_qkv_kernel<HD>, dim3(w.tpad, gy), dim3(256), 0, s, reinterpret_cast<const float*>(ws + w.qkv),
+  MOE_PDL((attn_qkv_kernel<HD, false>), dim3(w.tpad, gy), dim3(256), 0, s, reinterpret_cast<const float*>(ws + w.qkv),
           w.s1, T, w.tpad, a.nh, a.nkv, a.bqkv, a.has_qk_norm ? a.qn : nullptr,
           a.has_qk_norm ? a.kn : nullptr, a.rot, reinterpret_cast<const float2*>(ws + w.rope),
           a.cfg.rms_norm_eps,
           reinterpret_cast<__half*>(ws + w.q), reinterpret_cast<__half*>(ws + w.k),
-          reinterpret_cast<__half*>(ws + w.v));
+          reinterpret_cast<__half*>(ws + w.v), KvView{}, 0, static_cast<const int2*>(nullptr));
   MOE_PDL(attn_vt_kernel, dim3(w.tpad / 64, HD / 64, a.nkv), dim3(256), 0, s,
           reinterpret_cast<const __half*>(ws + w.v), reinterpret_cast<__half*>(ws + w.vt), w.tpad, HD);
   FaArgs fa{};
@@ -709,7 +789,44 @@ static cudaError_t attn_launch(const AttnPlan& a, const AttnWs& w, char* ws, con
   const size_t n = static_cast<size_t>(T) * a.H;
   const int grid = static_cast<int>(std::min<size_t>((n + 255) / 256, static_cast<size_t>(a.num_sms) * 8));
   MOE_PDL(attn_out_kernel, dim3(grid), dim3(256), 0, s, x, reinterpret_cast<const float*>(ws + w.oplanes),
-          w.s2, n, out);
+          w.s2, n, out, static_cast<const int*>(nullptr), a.H);
+  return cudaSuccess;
+}
+
+// The block over the paged cache: the new tokens' keys and values go to their pages, the
+// attention reads all cached tokens.
+template <int HD>
+static cudaError_t attn_cached_launch(const AttnPlan& a, const MoeKvCache& c, const AttnCachedWs& w, char* ws,
+                                      const float* x, float* out, int layer, const KvBatch& b, cudaStream_t s) {
+  const int T = b.rows;
+  MOE_CUDA_RET(launch_norm_rows(x, a.win, a.H, a.cfg.rms_norm_eps, T, reinterpret_cast<float*>(ws + w.rms),
+                                reinterpret_cast<__half*>(ws + w.h16), a.d_err, s));
+  MOE_CUDA_RET(launch_dense_gemm(a.tm_qkv, a.nqkv, a.H, reinterpret_cast<const __half*>(ws + w.h16), T,
+                                 reinterpret_cast<float*>(ws + w.qkv), w.s1, a.d_err, a.num_sms, s));
+  MOE_PDL(attn_place_kernel, dim3((T + 3) / 4), dim3(128), 0, s, c.v, b, reinterpret_cast<float2*>(ws + w.rope),
+          reinterpret_cast<int2*>(ws + w.slot), a.rot / 2, a.cfg.rope_theta);
+  const int groups = (a.nh + 2 * a.nkv + 7) / 8;
+  const int gy = std::max(1, std::min(groups, (8 * a.num_sms + T - 1) / T));
+  MOE_PDL((attn_qkv_kernel<HD, true>), dim3(T, gy), dim3(256), 0, s, reinterpret_cast<const float*>(ws + w.qkv), w.s1,
+          T, T, a.nh, a.nkv, a.bqkv, a.has_qk_norm ? a.qn : nullptr, a.has_qk_norm ? a.kn : nullptr, a.rot,
+          reinterpret_cast<const float2*>(ws + w.rope), a.cfg.rms_norm_eps, reinterpret_cast<__half*>(ws + w.q),
+          static_cast<__half*>(nullptr), static_cast<__half*>(nullptr), c.v, layer,
+          reinterpret_cast<const int2*>(ws + w.slot));
+  KvAttend k{};
+  k.q = ws + w.q;
+  k.out = ws + w.o16;
+  k.qs[0] = k.os[0] = a.nout;
+  k.qs[1] = k.os[1] = a.hd;
+  k.heads = a.nh;
+  k.layer = layer;
+  k.scale = static_cast<float>(1.0 / sqrt(static_cast<double>(HD)));
+  MOE_CUDA_RET(kv_launch_attend(c.v, c.tk, c.tv, c.bf16, b, k, ws + w.attend, c.num_sms, s));
+  MOE_CUDA_RET(launch_dense_gemm(a.tm_o, a.H, a.nout, reinterpret_cast<const __half*>(ws + w.o16), T,
+                                 reinterpret_cast<float*>(ws + w.oplanes), w.s2, a.d_err, a.num_sms, s));
+  const size_t n = static_cast<size_t>(T) * a.H;
+  const int grid = static_cast<int>(std::min<size_t>((n + 255) / 256, static_cast<size_t>(a.num_sms) * 8));
+  MOE_PDL(attn_out_kernel, dim3(grid), dim3(256), 0, s, x, reinterpret_cast<const float*>(ws + w.oplanes), w.s2, n,
+          out, b.q_start + b.n, a.H);
   return cudaSuccess;
 }
 
@@ -928,6 +1045,51 @@ int moe_attn_forward(MoeAttn* h, const float* x_dev, float* out_dev, int32_t T, 
   char* ws = static_cast<char*>(workspace);
   const cudaError_t st = a.hd == 128 ? attn_launch<128>(a, w, ws, x_dev, out_dev, T, s)
                                      : attn_launch<64>(a, w, ws, x_dev, out_dev, T, s);
+  if (st != cudaSuccess) return afail(MOE_ERR_CUDA, std::string("attention launch: ") + cudaGetErrorString(st));
+  return MOE_OK;
+}
+
+static const char* cached_mismatch(const AttnPlan& a, const MoeKvCache& c) {
+  if (c.bf16) return "the attention block needs an f16 cache";
+  if (c.v.heads != a.nkv || c.v.hd != a.hd) return "the cache's kv_heads or head_dim differ from the plan's";
+  if (c.device != a.cfg.device) return "the cache is on another device than the plan";
+  return nullptr;
+}
+
+uint64_t moe_attn_cached_workspace_bytes(const MoeAttn* h, const MoeKvCache* cache, int32_t T, int32_t n_seqs) {
+  if (!h || !cache || T <= 0 || n_seqs <= 0 || cached_mismatch(h->a, *cache)) return 0;
+  return attn_cached_ws(h->a, *cache, T, n_seqs).total;
+}
+
+int moe_attn_forward_cached(MoeAttn* h, MoeKvCache* cache, int32_t layer, const float* x_dev, float* out_dev,
+                            const int32_t* seqs, const int32_t* q_start, int32_t n_seqs, int32_t T,
+                            void* workspace, uint64_t workspace_bytes, void* stream) {
+  if (!h) return afail(MOE_ERR_INVALID, "null attention plan");
+  if (!cache) return afail(MOE_ERR_INVALID, "null cache");
+  AttnPlan& a = h->a;
+  if (!a.bound) return afail(MOE_ERR_NOT_BOUND, "moe_attn_bind has not been called");
+  if (const char* why = cached_mismatch(a, *cache)) return afail(MOE_ERR_INVALID, why);
+  if (layer < 0 || layer >= cache->v.layers) return afail(MOE_ERR_INVALID, "layer outside the cache");
+  if (T < 0 || T > a.cfg.max_tokens) return afail(MOE_ERR_INVALID, "T outside [0, max_tokens]");
+  if (n_seqs < 0) return afail(MOE_ERR_INVALID, "negative n_seqs");
+  if (T == 0 || n_seqs == 0) return MOE_OK;
+  if (!x_dev || !out_dev || !seqs || !q_start) return afail(MOE_ERR_INVALID, "null x / out / seqs / q_start");
+  if (x_dev == out_dev) return afail(MOE_ERR_INVALID, "x and out may not alias");
+  if (misaligned16(x_dev) || misaligned16(out_dev))
+    return afail(MOE_ERR_INVALID, "x and out must be 16-byte aligned");
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255))
+    return afail(MOE_ERR_WORKSPACE, "workspace must be a 256-byte aligned device pointer");
+  const AttnCachedWs w = attn_cached_ws(a, *cache, T, n_seqs);
+  if (workspace_bytes < w.total) return afail(MOE_ERR_WORKSPACE, "workspace too small");
+  int before = -1;
+  MOE_ATT_CUDA(cudaGetDevice(&before));
+  if (before != a.cfg.device) MOE_ATT_CUDA(cudaSetDevice(a.cfg.device));
+  const KvBatch b{seqs, q_start, n_seqs, T};
+  char* ws = static_cast<char*>(workspace);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t st = a.hd == 128 ? attn_cached_launch<128>(a, *cache, w, ws, x_dev, out_dev, layer, b, s)
+                                     : attn_cached_launch<64>(a, *cache, w, ws, x_dev, out_dev, layer, b, s);
+  if (before != a.cfg.device) cudaSetDevice(before);
   if (st != cudaSuccess) return afail(MOE_ERR_CUDA, std::string("attention launch: ") + cudaGetErrorString(st));
   return MOE_OK;
 }

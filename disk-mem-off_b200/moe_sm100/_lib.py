@@ -161,6 +161,9 @@ _PROTOTYPES: dict[str, tuple] = {
     "moe_kv_attend_workspace_bytes": (c_uint64, [c_void_p, c_int32, c_int32, c_int32]),
     "moe_kv_attend": (c_int32, [c_void_p, POINTER(MoeKvAttendArgsC), c_void_p, c_uint64, c_void_p]),
     "moe_kv_status": (c_int32, [c_void_p, c_void_p]),
+    "moe_attn_cached_workspace_bytes": (c_uint64, [c_void_p, c_void_p, c_int32, c_int32]),
+    "moe_attn_forward_cached": (c_int32, [c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_void_p,
+                                          c_void_p, c_int32, c_int32, c_void_p, c_uint64, c_void_p]),
     "moe_wait_probe": (c_int32, [c_void_p, c_int64, c_void_p]),
     "moe_last_error": (c_char_p, []),
     "moe_version": (c_char_p, []),

@@ -4,7 +4,8 @@
 ``GLM4MoeExecutor._attention_block(x, t)`` (offload_runtime/executors/glm4_moe.py:112-162):
 ``x + o_proj(causal softmax attention(rms_norm(x)))`` with the reference's q/k/v
 biases, per-head q/k RMS norms, partial rotate-half RoPE and grouped-query heads,
-over the whole sequence at positions 0..T-1.  PyTorch provides only buffers and
+over the whole sequence at positions 0..T-1.  ``forward_cached`` is the same block on the
+new tokens of many sequences over a ``paged.PagedKVCache``.  PyTorch provides only buffers and
 the current stream; the kernels are the library's (tcgen05 projections and a
 tcgen05 flash-attention kernel).
 """
@@ -17,6 +18,7 @@ from typing import Any, Iterable
 from . import _lib
 from ._lib import check, lib
 from .layer import _descs, _stream_handle, _torch
+from .paged import PagedKVCache
 
 
 @dataclass
@@ -113,6 +115,39 @@ class AttentionLayer:
         check(lib().moe_attn_forward(self._h, c_void_p(x.data_ptr()), c_void_p(out.data_ptr()), t,
                                      c_void_p(self._ws.data_ptr()), self._ws.numel(),
                                      c_void_p(_stream_handle(stream))))
+        return out
+
+    def forward_cached(self, x: Any, cache: PagedKVCache, seqs: Any, starts: Any, layer: int = 0,
+                       out: Any = None, stream: Any = None) -> Any:
+        """``x + attention(x)`` for the new tokens of a batch of cached sequences: rows
+        ``starts[i] .. starts[i + 1] - 1`` of ``x`` (CUDA fp32 [T, H]) are the last tokens of
+        sequence ``seqs[i]`` of ``cache``, reserved beforehand.  Their keys and values go to
+        ``layer`` of the cache; errors of the sequences are raised by ``cache.status()``."""
+        torch = _torch()
+        if stream is not None:
+            if not isinstance(stream, torch.cuda.Stream):
+                stream = torch.cuda.ExternalStream(_stream_handle(stream), device=cache.device)
+            with torch.cuda.stream(stream):
+                return self.forward_cached(x, cache, seqs, starts, layer, out)
+        if not (isinstance(x, torch.Tensor) and x.device == cache.device and x.dtype == torch.float32):
+            raise TypeError(f"x must be a float32 tensor on {cache.device}")
+        if x.dim() != 2 or x.shape[1] != self.cfg.hidden:
+            raise ValueError(f"x must be [T, {self.cfg.hidden}]")
+        seqs, starts, n = cache._batch(seqs, starts)
+        x = x.contiguous()
+        if out is None:
+            out = torch.empty_like(x)
+        elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device \
+                or not out.is_contiguous():
+            raise ValueError("out must be a contiguous tensor like x")
+        t = x.shape[0]
+        if t == 0 or n == 0:
+            return out
+        need = int(lib().moe_attn_cached_workspace_bytes(self._h, cache._h, t, n))
+        ws = torch.empty(max(need, 256), dtype=torch.uint8, device=x.device)  # this call's own
+        check(lib().moe_attn_forward_cached(
+            self._h, cache._h, layer, x.data_ptr(), out.data_ptr(), seqs.data_ptr(),
+            starts.data_ptr(), n, t, ws.data_ptr(), need, cache._stream()))
         return out
 
     def status(self, stream: Any = None) -> None:

@@ -456,6 +456,19 @@ int moe_kv_attend(MoeKvCache* cache, const MoeKvAttendArgs* args, void* workspac
 /* As moe_status, for the cache's error word (in its scratch). */
 int moe_kv_status(MoeKvCache* cache, void* stream);
 
+/* The GLM-4 attention block (moe_attn_forward) on the new tokens of a batch of sequences of
+ * a paged cache: out = x + attention(x) for the T rows of x, each at its own position; the
+ * rows' keys and values are written to layer `layer` of the cache, whose older tokens they
+ * attend to.  Reserve first (once for all layers); seqs, q_start, n_seqs as moe_kv_append;
+ * the cache is f16 with the plan's kv_heads and head_dim.  Rows of out from q_start[n_seqs]
+ * on are left as they were.  Errors of the sequences are reported by moe_kv_status. */
+uint64_t moe_attn_cached_workspace_bytes(const MoeAttn* attn, const MoeKvCache* cache, int32_t T,
+                                         int32_t n_seqs);
+int moe_attn_forward_cached(MoeAttn* attn, MoeKvCache* cache, int32_t layer, const float* x_dev,
+                            float* out_dev, const int32_t* seqs, const int32_t* q_start,
+                            int32_t n_seqs, int32_t T, void* workspace, uint64_t workspace_bytes,
+                            void* stream);
+
 /* ------------------------------------------- runtime (CUDABackend, ctypes) */
 int moe_rt_device_count(int32_t* count);
 int moe_rt_set_device(int32_t device);
