@@ -159,7 +159,7 @@ _PROTOTYPES: dict[str, tuple] = {
     "moe_kv_append": (c_int32, [c_void_p, c_int32, c_void_p, c_void_p, c_int64, c_int64, c_int64,
                                 c_int64, c_void_p, c_void_p, c_int32, c_int32, c_void_p]),
     "moe_kv_attend_workspace_bytes": (c_uint64, [c_void_p, c_int32, c_int32, c_int32]),
-    "moe_kv_attend": (c_int32, [c_void_p, POINTER(MoeKvAttendArgsC), c_void_p, c_uint64, c_void_p]),
+    "moe_kv_attend": (c_int32, [c_void_p, c_char_p, c_void_p, c_uint64, c_void_p]),  # MoeKvAttendArgs
     "moe_kv_status": (c_int32, [c_void_p, c_void_p]),
     "moe_attn_cached_workspace_bytes": (c_uint64, [c_void_p, c_void_p, c_int32, c_int32]),
     "moe_attn_forward_cached": (c_int32, [c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_void_p,

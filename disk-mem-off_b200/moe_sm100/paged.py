@@ -21,8 +21,8 @@ in their values are found on the device and raised by ``status()``.  Every call 
 """
 from __future__ import annotations
 
-import functools
 import math
+import struct
 from ctypes import byref, c_int64, c_void_p
 from typing import Any
 
@@ -31,24 +31,13 @@ from ._lib import check, lib
 from .layer import _stream_handle, _torch
 
 
+# MoeKvAttendArgs as bytes: cheaper to fill on every call than a ctypes structure
+_ATTEND_ARGS = struct.Struct("@QQQqqqqqqQQiiiif4x")
+
+
 def _strides(t: Any) -> list[int]:
     """Element strides; a dimension of one entry gets 0 (torch leaves it arbitrary)."""
     return [st if n > 1 else 0 for n, st in zip(t.shape, t.stride())]
-
-
-def _on_stream(method: Any) -> Any:
-    """With ``stream=`` the call runs as if that stream were current, so that the buffers
-    it allocates belong to that stream too."""
-    @functools.wraps(method)
-    def call(self: Any, *args: Any, stream: Any = None, **kw: Any) -> Any:
-        if stream is None:
-            return method(self, *args, **kw)
-        torch = _torch()
-        if not isinstance(stream, torch.cuda.Stream):
-            stream = torch.cuda.ExternalStream(_stream_handle(stream), device=self.device)
-        with torch.cuda.stream(stream):
-            return method(self, *args, **kw)
-    return call
 
 
 class PagedKVCache:
@@ -88,7 +77,10 @@ class PagedKVCache:
         self._dev = k.get_device()
         self._lib = lib()
         self._i32, self._f32, self._u8 = torch.int32, torch.float32, torch.uint8
-        self._empty, self._current_stream = torch.empty, torch.cuda.current_stream
+        self._empty = torch.empty
+        # the handle of the current stream without a Stream object around it
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+            (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
         self._scale = 1.0 / math.sqrt(head_dim)
         cfg = _lib.MoeKvConfigC(
             k=k.data_ptr(), v=v.data_ptr(), k_strides=(c_int64 * 4)(*_strides(k)[:4]),
@@ -134,26 +126,27 @@ class PagedKVCache:
 
     # -- arguments ----------------------------------------------------------------
     # A decode step makes these calls once a layer, and its kernels take some
-    # microseconds: the checks compare the devices' numbers and dtype objects.
+    # microseconds: the checks read the tensors as little as they can.
     def _index(self, name: str, t: Any) -> Any:
-        if not hasattr(t, "data_ptr"):
-            torch = _torch()
-            t = torch.tensor(list(t), dtype=torch.int32).to(self.device)
-        if t.dtype is not self._i32 or t.dim() != 1 or t.get_device() != self._dev:
-            raise TypeError(f"{name} must be a 1-D int32 tensor on {self.device}")
-        return t if t.is_contiguous() else t.contiguous()
+        """``t`` as a contiguous 1-D int32 tensor on the cache's device."""
+        try:
+            if t.dtype is self._i32 and t.get_device() == self._dev and t.dim() == 1:
+                return t if t.is_contiguous() else t.contiguous()
+        except AttributeError:
+            return _torch().tensor(list(t), dtype=self._i32).to(self.device)
+        raise TypeError(f"{name} must be a 1-D int32 tensor on {self.device}")
 
     def _indices(self, a: str, x: Any, b: str, y: Any) -> tuple[Any, Any, int]:
         x, y = self._index(a, x), self._index(b, y)
-        n = x.shape[0]
-        if y.shape[0] != n:
+        n = len(x)
+        if len(y) != n:
             raise ValueError(f"{a} and {b} must have one entry each")
         return x, y, n
 
     def _batch(self, seqs: Any, starts: Any) -> tuple[Any, Any, int]:
         seqs, starts = self._index("seqs", seqs), self._index("starts", starts)
-        n = seqs.shape[0]
-        if starts.shape[0] != n + 1:
+        n = len(seqs)
+        if len(starts) != n + 1:
             raise ValueError("starts must have one entry more than seqs")
         return seqs, starts, n
 
@@ -171,55 +164,71 @@ class PagedKVCache:
         return rows, heads, token if rows > 1 else 0, head if heads > 1 else 0
 
     def _stream(self) -> int:
-        return self._current_stream(self._dev).cuda_stream
+        return self._raw_stream(self._dev)
+
+    def _on(self, stream: Any, method: Any, *args: Any) -> Any:
+        """The call as if ``stream`` were current, so that the buffers it allocates belong
+        to that stream too."""
+        torch = _torch()
+        if not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(_stream_handle(stream), device=self.device)
+        with torch.cuda.stream(stream):
+            return method(*args)
 
     # -- pages --------------------------------------------------------------------
-    @_on_stream
-    def reserve(self, seqs: Any, counts: Any) -> None:
+    def reserve(self, seqs: Any, counts: Any, stream: Any = None) -> None:
         """Lengthen ``seqs[i]`` by ``counts[i]`` tokens, with pages for them."""
+        if stream is not None:
+            return self._on(stream, self.reserve, seqs, counts)
         seqs, counts, n = self._indices("seqs", seqs, "counts", counts)
         check(self._lib.moe_kv_reserve(self._h, seqs.data_ptr(), counts.data_ptr(), n, self._stream()))
 
-    @_on_stream
-    def fork(self, parents: Any, children: Any) -> None:
+    def fork(self, parents: Any, children: Any, stream: Any = None) -> None:
         """Make the empty sequence ``children[i]`` a copy of ``parents[i]`` that shares
         its pages; a page is copied when one of its holders next writes to it."""
+        if stream is not None:
+            return self._on(stream, self.fork, parents, children)
         parents, children, n = self._indices("parents", parents, "children", children)
         check(self._lib.moe_kv_fork(self._h, parents.data_ptr(), children.data_ptr(), n,
                                     self._stream()))
 
-    @_on_stream
-    def truncate(self, seqs: Any, lengths: Any) -> None:
+    def truncate(self, seqs: Any, lengths: Any, stream: Any = None) -> None:
         """Shorten ``seqs[i]`` to ``lengths[i]`` tokens and let its other pages go."""
+        if stream is not None:
+            return self._on(stream, self.truncate, seqs, lengths)
         seqs, lengths, n = self._indices("seqs", seqs, "lengths", lengths)
         check(self._lib.moe_kv_truncate(self._h, seqs.data_ptr(), lengths.data_ptr(), n,
                                         self._stream()))
 
-    @_on_stream
-    def free(self, seqs: Any) -> None:
+    def free(self, seqs: Any, stream: Any = None) -> None:
         """Empty the sequences: ``truncate`` to no tokens."""
+        if stream is not None:
+            return self._on(stream, self.free, seqs)
         seqs = self._index("seqs", seqs)
         self.truncate(seqs, _torch().zeros_like(seqs))
 
-    @_on_stream
-    def copy_pages(self, src: Any, dst: Any) -> None:
+    def copy_pages(self, src: Any, dst: Any, stream: Any = None) -> None:
         """Copy pages ``src[i]`` to ``dst[i]`` in every layer; tables and refs stay."""
+        if stream is not None:
+            return self._on(stream, self.copy_pages, src, dst)
         src, dst, n = self._indices("src", src, "dst", dst)
         check(self._lib.moe_kv_copy_pages(self._h, src.data_ptr(), dst.data_ptr(), n,
                                           self._stream()))
 
-    @_on_stream
-    def compact(self, into: "PagedKVCache | None" = None) -> None:
+    def compact(self, into: "PagedKVCache | None" = None, stream: Any = None) -> None:
         """Move the live pages to the lowest numbers, or, dense and in order, ``into``
         another cache (whose sequences are overwritten): how a pool changes its size."""
-        check(self._lib.moe_kv_compact(self._h, into._h if into is not None else None,
-                                       self._stream()))
+        if stream is not None:
+            return self._on(stream, self.compact, into)
+        check(self._lib.moe_kv_compact(self._h, None if into is None else into._h, self._stream()))
 
     # -- tokens -------------------------------------------------------------------
-    @_on_stream
-    def append(self, k: Any, v: Any, seqs: Any, starts: Any, layer: int = 0) -> None:
+    def append(self, k: Any, v: Any, seqs: Any, starts: Any, layer: int = 0,
+               stream: Any = None) -> None:
         """Write the batch's keys and values ``[rows, kv_heads, head_dim]`` to the last
         places of their sequences (after ``reserve``)."""
+        if stream is not None:
+            return self._on(stream, self.append, k, v, seqs, starts, layer)
         seqs, starts, n = self._batch(seqs, starts)
         rows, heads, kt, kh = self._rows("k", k)
         vrows, vheads, vt, vh = self._rows("v", v)
@@ -228,12 +237,13 @@ class PagedKVCache:
         check(self._lib.moe_kv_append(self._h, layer, k.data_ptr(), v.data_ptr(), kt, kh, vt, vh,
                                       seqs.data_ptr(), starts.data_ptr(), n, rows, self._stream()))
 
-    @_on_stream
     def attend(self, q: Any, seqs: Any, starts: Any, layer: int = 0, scale: float | None = None,
-               out: Any = None, lse: Any = None) -> Any:
+               out: Any = None, lse: Any = None, stream: Any = None) -> Any:
         """Causal attention of the batch's rows ``q`` ``[rows, heads, head_dim]`` over all
         tokens of their sequences; returns ``out``, shaped as ``q``.  ``lse``: an fp32
         ``[rows, heads]`` tensor that receives the log of the sum of the exponentials."""
+        if stream is not None:
+            return self._on(stream, self.attend, q, seqs, starts, layer, scale, out, lse)
         seqs, starts, n = self._batch(seqs, starts)
         rows, heads, qt, qh = self._rows("q", q)
         if heads == 0 or heads % self.kv_heads:
@@ -245,7 +255,7 @@ class PagedKVCache:
             orows, oheads, ot, oh = self._rows("out", out)
             if orows != rows or oheads != heads:
                 raise ValueError("out must have the shape of q")
-        lp, lt, lh = None, 0, 0
+        lp, lt, lh = 0, 0, 0
         if lse is not None:
             if lse.dtype is not self._f32 or lse.get_device() != self._dev or lse.shape != q.shape[:2]:
                 raise ValueError("lse must be a float32 [rows, heads] tensor on the cache's device")
@@ -256,13 +266,14 @@ class PagedKVCache:
         # graphs' scratch
         need = self._lib.moe_kv_attend_workspace_bytes(self._h, heads, rows, n)
         ws = self._empty(need, dtype=self._u8, device=self.device)
-        args = _lib.MoeKvAttendArgsC(q.data_ptr(), out.data_ptr(), lp, qt, qh, ot, oh, lt, lh,
-                                     seqs.data_ptr(), starts.data_ptr(), n, rows, heads, layer,
-                                     self._scale if scale is None else scale)
-        check(self._lib.moe_kv_attend(self._h, byref(args), ws.data_ptr(), need, self._stream()))
+        args = _ATTEND_ARGS.pack(q.data_ptr(), out.data_ptr(), lp, qt, qh, ot, oh, lt, lh,
+                                 seqs.data_ptr(), starts.data_ptr(), n, rows, heads, layer,
+                                 self._scale if scale is None else scale)
+        check(self._lib.moe_kv_attend(self._h, args, ws.data_ptr(), need, self._stream()))
         return out
 
-    @_on_stream
-    def status(self) -> None:
+    def status(self, stream: Any = None) -> None:
         """Wait for the stream and raise what the cache's kernels reported, if anything."""
+        if stream is not None:
+            return self._on(stream, self.status)
         check(self._lib.moe_kv_status(self._h, self._stream()))

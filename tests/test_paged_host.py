@@ -11,7 +11,7 @@ import pytest
 import torch
 
 from moe_sm100 import _lib
-from moe_sm100.paged import PagedKVCache
+from moe_sm100.paged import _ATTEND_ARGS, PagedKVCache
 from oracle.paged_oracle import OracleError, PagedOracle, attend_chunk
 
 
@@ -137,6 +137,9 @@ def test_struct_sizes_match_the_header() -> None:
     # natural alignment of the C declarations
     assert ctypes.sizeof(_lib.MoeKvConfigC) == 2 * 8 + 8 * 8 + 4 * 8 + 9 * 4 + 4
     assert ctypes.sizeof(_lib.MoeKvAttendArgsC) == 3 * 8 + 6 * 8 + 2 * 8 + 4 * 4 + 4 + 4
+    # the packed form that calls pass has the structure's bytes
+    values = list(range(1, 16)) + [0.5]
+    assert _ATTEND_ARGS.pack(*values) == bytes(_lib.MoeKvAttendArgsC(*values))
 
 
 def test_error_code_of_an_exhausted_pool_is_a_runtime_error() -> None:
