@@ -10,12 +10,13 @@
 // of each kv head.  128 rows fill the M of one tcgen05.mma.
 //
 // Work.  kv_plan_kernel (one CTA) cuts the entries into units: 256 rows that two
-// warpgroups work on against the same keys ("pair"), or up to 128 rows that one
-// warpgroup works on alone ("single": decode steps and the ends of chunks).  A unit of
-// one kv head costs its number of 64-key tiles and a constant.  All tiles are numbered in a row and
-// cut into equal shares, pairs for 148 CTAs and singles for 2 * 148 warpgroups, so the
-// load is even for any mix of lengths; a unit cut by a share's border leaves fp32
-// partial results that kv_merge_kernel joins in share order (same bits every time).
+// warpgroups work on against the same keys ("pair"), 33 to 128 rows that one warpgroup
+// works on alone ("single": the ends of chunks), or up to 32 ("few": decode steps).  A
+// unit of one kv head costs its number of 64-key tiles and a constant.  All units, pairs
+// first and counted twice since they take both warpgroups, are laid on one line that is
+// cut into equal shares, one for each SM, so the load is even for any mix of lengths and
+// an SM meets one or two kinds; a unit cut by a share's border leaves fp32 partial
+// results that kv_merge_kernel joins in share order (same bits every time).
 //
 // kv_attend_kernel (one CTA an SM, 384 threads): warps 0-3 and 4-7 are the two softmax
 // warpgroups, a thread a row; warp 8 fetches K and V tiles page by page (TMA, 128-byte
@@ -35,9 +36,11 @@
 
 namespace moe {
 
-#ifndef KA_LF
-#define KA_LF 2
-#define KA_LP 4
+#ifndef KA_EXTRA
+#define KA_EXTRA 3
+#endif
+#ifndef KA_LEAST
+#define KA_LEAST 2
 #endif
 constexpr int kTile = 128;       // rows of a warpgroup
 constexpr int kKeys = 64;        // keys of a tile
@@ -71,11 +74,11 @@ constexpr int kMergeRows = 16;
 
 // Kinds of units: rows of a unit, shares an SM.
 constexpr int kPair = 0, kSingle = 1, kFew = 2, kKinds = 3;
-constexpr int kFewRows = 64;
-// What beginning and ending a unit costs, in tiles of its kind.
-__host__ __device__ constexpr int kind_extra(int k) { return 3; }
-// The least share worth a CTA or warpgroup of its own, in cost.
-__host__ __device__ constexpr int kind_least(int k) { return k == kFew ? KA_LF : KA_LP; }
+constexpr int kFewRows = 32;
+// What beginning and ending a unit costs, in tiles.
+constexpr int kUnitExtra = KA_EXTRA;
+// The least cost worth a warpgroup of its own.
+constexpr int kLeastShare = KA_LEAST;
 __host__ __device__ constexpr int kind_rows(int k) { return k == kPair ? 2 * kTile : k == kSingle ? kTile : kFewRows; }
 __host__ __device__ constexpr int kind_shares(int k) { return k == kPair ? 1 : 2; }
 
@@ -185,6 +188,35 @@ struct KaPlace {
   long long cost;   // and is this
   long long tiles;  // tiles before w0
 };
+// One kind's part of the line: pairs from 0 on, the others after `before`.  CTA c has
+// [2 per c, 2 per (c + 1)) of the line; a pair unit takes two of it for one of cost, and the
+// other kinds' part of a CTA is halved between its warpgroups.
+struct KaLine {
+  long long per, before, all;
+  bool small, pair;
+  MOE_DEV void range(int share, long long* w0, long long* w1) const {
+    if (pair) {
+      *w0 = min(share * per, all);
+      *w1 = min((share + 1) * per, all);
+      return;
+    }
+    const long long at = 2 * per * (share >> 1) - before;
+    const long long lo = min(max(at, 0ll), all), hi = min(max(at + 2 * per, 0ll), all);
+    const long long mid = lo + ((hi - lo + 1) >> 1);
+    *w0 = share & 1 ? mid : lo;
+    *w1 = share & 1 ? hi : mid;
+  }
+  MOE_DEV int share_of(long long pos) const {
+    const long long at = pair ? pos : pos + before, len = pair ? per : 2 * per;
+    const int c = small ? static_cast<int>(static_cast<uint32_t>(at) / static_cast<uint32_t>(len))
+                        : static_cast<int>(at / len);
+    if (pair) return c;
+    long long w0, w1;
+    range(2 * c, &w0, &w1);
+    return 2 * c + (pos >= w1 ? 1 : 0);
+  }
+};
+
 template <typename T>
 MOE_DEV KaPlace plan_place(const long long* pre, int n, T w0, int heads, int extra) {
   int lo = 0, hi = n;  // heads * pre[lo] <= w0 < heads * pre[hi]
@@ -212,7 +244,6 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
                                                          const KaPtrs w, const int cap0) {
   pdl_enter();
   __shared__ long long spre[kKinds][kPlanSmem + 1];
-  __shared__ long long stiles[kPlanT + 1];
   __shared__ int s_merges;
   __shared__ int4 s_entry[kPlanT];       // the chunk's entries: seq, row0, m, len
   __shared__ int s_pairs[kPlanT + 1];    // pairs before each of them
@@ -254,7 +285,7 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
     const int tiles = key_tiles(len - m, m - 1);
     // counts (at most 1024 each) in the high bits, cost of a chunk's units in the low 44
     const KaUnit rest{seq, row0, rows - rem, rem, len - m, len, tiles, 0};
-    long long total, mine = few ? (1ll << 44) + tiles + kind_extra(kFew) : 0;
+    long long total, mine = few ? (1ll << 44) + tiles + kUnitExtra : 0;
     long long at = plan_scan(mine, busy, &total);
     constexpr long long kLow = (1ll << 44) - 1;
     if (few) {
@@ -265,7 +296,7 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
     n_few += static_cast<int>(total >> 44);
     work_few += total & kLow;
     if (!__syncthreads_or(single || na > 0)) continue;
-    mine = single ? (1ll << 44) + tiles + kind_extra(kSingle) : 0;
+    mine = single ? (1ll << 44) + tiles + kUnitExtra : 0;
     at = plan_scan(mine, busy, &total);
     if (single) {
       const int j = n_single + static_cast<int>(at >> 44) - 1;
@@ -295,7 +326,7 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
         const int r0 = (j - s_pairs[lo]) * 2 * kTile, r1 = min(r0 + 2 * kTile, e.z * group);
         u = KaUnit{e.x, e.y, r0, r1 - r0, e.w - e.z, e.w, key_tiles(e.w - e.z, (r1 - 1) / group), 0};
         w.pair.list[n_pair + j] = u;
-        mine = u.tiles + kind_extra(kPair);
+        mine = u.tiles + kUnitExtra;
       }
       const long long sum = plan_scan(mine, min((pairs - j0 + 31) / 32, 32), &all);
       if (j < pairs) pre_pair[n_pair + j + 1] = work_pair + sum;
@@ -305,47 +336,53 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
   }
   if (tid == 0) pre_pair[0] = pre_single[0] = pre_few[0] = 0;
   __syncthreads();
-  // (2) a thread for each share of each kind, and one past the last of each
-  int k = kPair, s = tid;
-  while (k < kKinds && s > num_sms * kind_shares(k)) s -= num_sms * kind_shares(k++) + 1;
-  const int shares = num_sms * kind_shares(k), extra = kind_extra(k);
-  const int n = k == kPair ? n_pair : k == kSingle ? n_single : n_few;
-  const long long* pre = k == kPair ? pre_pair : k == kSingle ? pre_single : pre_few;
-  const long long all = (k == kPair ? work_pair : k == kSingle ? work_single : work_few) * c.heads;
-  const bool small = all < 0x40000000;
-  long long per = 1, w0 = 0;
-  KaPlace p{};
-  if (k < kKinds && all > 0) {
-    if (small) {
-      const uint32_t per32 = max((static_cast<uint32_t>(all) + shares - 1) / static_cast<uint32_t>(shares),
-                                 static_cast<uint32_t>(kind_least(k)));
-      per = per32;
-      w0 = static_cast<long long>(s) * per32;
-      if (w0 < all) p = plan_place<uint32_t>(pre, n, static_cast<uint32_t>(w0), c.heads, extra);
-    } else {
-      per = (all + shares - 1) / shares;
-      w0 = s * per;
-      if (w0 < all) p = plan_place<unsigned long long>(pre, n, static_cast<unsigned long long>(w0), c.heads, extra);
+  // (2) a thread for each share of each kind
+  const int k = tid < num_sms ? kPair : tid < 3 * num_sms ? kSingle : kFew;
+  const int share = tid - (k == kPair ? 0 : k == kSingle ? num_sms : 3 * num_sms);
+  if (share < num_sms * kind_shares(k)) {
+    const long long cost_pair = work_pair * c.heads, cost_single = work_single * c.heads, cost_few = work_few * c.heads;
+    const long long line = 2 * cost_pair + cost_single + cost_few;
+    const bool small = line < 0x40000000;
+    const int halves = 2 * num_sms;
+    KaLine l;
+    l.per = max(small ? (static_cast<int>(line) + halves - 1) / halves : (line + halves - 1) / halves,
+                static_cast<long long>(kLeastShare));
+    l.small = small;
+    l.pair = k == kPair;
+    l.before = k == kPair ? 0 : k == kSingle ? 2 * cost_pair : 2 * cost_pair + cost_single;
+    l.all = k == kPair ? cost_pair : k == kSingle ? cost_single : cost_few;
+    const int n = k == kPair ? n_pair : k == kSingle ? n_single : n_few;
+    const long long* pre = k == kPair ? pre_pair : k == kSingle ? pre_single : pre_few;
+    const KaList list = w.kind(k);
+    long long w0, w1;
+    l.range(share, &w0, &w1);
+    KaStart st{0, 0, 0, 0};
+    if (w0 < w1) {
+      const KaPlace p = small ? plan_place<uint32_t>(pre, n, static_cast<uint32_t>(w0), c.heads, kUnitExtra)
+                              : plan_place<unsigned long long>(pre, n, static_cast<unsigned long long>(w0), c.heads, kUnitExtra);
+      long long end = l.all - static_cast<long long>(n) * kUnitExtra * c.heads;
+      if (w1 < l.all)
+        end = (small ? plan_place<uint32_t>(pre, n, static_cast<uint32_t>(w1), c.heads, kUnitExtra)
+                     : plan_place<unsigned long long>(pre, n, static_cast<unsigned long long>(w1), c.heads, kUnitExtra)).tiles;
+      st = KaStart{p.item, p.head, p.tile, static_cast<int>(end - p.tiles)};
+      // a unit that is cut here first: its first tile lies in the share that ends here
+      if (p.tile > 0) {
+        const int first = l.share_of(p.unit + kUnitExtra);
+        long long f0, f1;
+        l.range(first, &f0, &f1);
+        if (f1 == w0) {
+          const KaUnit u = list.list[p.item];
+          w.merge[atomicAdd(&s_merges, 1)] =
+              KaMerge{k, first, l.share_of(p.unit + p.cost - 1), p.head, u.row0, u.r0, u.rows, 0};
+        }
+      }
     }
-  }
-  const bool in = k < kKinds && w0 < all;
-  stiles[tid] = in ? p.tiles : all - static_cast<long long>(n) * extra * c.heads;
-  __syncthreads();
-  if (k < kKinds) {
-    const KaList l = w.kind(k);
-    if (s < shares) l.start[s] = KaStart{p.item, p.head, p.tile, in ? static_cast<int>(stiles[tid + 1] - stiles[tid]) : 0};
-    // a unit that begins in the share before and is cut here first
-    if (p.tile > 0 && p.unit + extra >= w0 - per) {
-      const int last = small ? static_cast<uint32_t>(p.unit + p.cost - 1) / static_cast<uint32_t>(per)
-                             : static_cast<int>((p.unit + p.cost - 1) / per);
-      const KaUnit u = l.list[p.item];
-      w.merge[atomicAdd(&s_merges, 1)] = KaMerge{k, s - 1, last, p.head, u.row0, u.r0, u.rows, 0};
-    }
+    list.start[share] = st;
   }
   __syncthreads();
   if (tid == 0) *w.n_merge = s_merges;
 }
-static_assert(5 * kKvMaxSms + kKinds <= kPlanT, "a thread for each share");
+static_assert(5 * kKvMaxSms <= kPlanT, "a thread for each share");
 
 // ------------------------------------------------------------------ the kernel
 template <int HD>
@@ -630,7 +667,7 @@ MOE_DEV void load_s(uint32_t taddr, float (&sc)[kKeys]) {
 }
 
 // ------------------------------------------------------------------ few rows
-// Units of at most 64 rows (decode steps).  They are bound by the reading of K and V, and
+// Units of at most 32 rows (decode steps).  They are bound by the reading of K and V, and
 // a tcgen05.mma of 128 rows would spend its time, and its softmax warps theirs, on padding.
 // So each warpgroup works alone on 64-key tiles of its own ring: MT 16-row blocks times
 // 4 / MT slices of 16 * MT keys, mma.sync m16n8k16 from the same swizzled tiles.  A warp
@@ -731,7 +768,7 @@ struct KaFew {
   MOE_DEV void fetch_q(const KaCursor& x) {
     const KaUnit& u = x.u;
     const int warp = (threadIdx.x >> 5) & 3, g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
-    const int mi = u.rows <= 16 ? 0 : u.rows <= 32 ? warp >> 1 : warp;
+    const int mi = u.rows <= 16 ? 0 : warp >> 1;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int pr = mi * 16 + g + 8 * r;
@@ -754,7 +791,7 @@ struct KaFew {
   template <int MT>
   MOE_DEV bool unit(KaCursor& x, int share) {
     constexpr float shift = BF16 ? 0.f : 7.f;  // as in the softmax warpgroups
-    constexpr int kSlices = 4 / MT, kKeys = 16 * MT;
+    constexpr int kSlices = 4 / MT, kKeysW = 16 * MT;  // keys of a warp
     const int warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
     const int slice = warp % kSlices;  // of 16-row block warp / kSlices
     const int g = lane >> 2, t = lane & 3;
@@ -774,10 +811,10 @@ struct KaFew {
     bool whole = true;
     // lane addresses inside a 16-key group: K rows (lane >> 4) * 8 + (lane & 7), chunk
     // (lane >> 3 & 1); V rows lane & 15, chunk lane >> 4
-    const int krow = slice * kKeys + ((lane >> 4) << 3) + (lane & 7), vrow = slice * kKeys + (lane & 15);
+    const int krow = slice * kKeysW + ((lane >> 4) << 3) + (lane & 7), vrow = slice * kKeysW + (lane & 15);
     for (bool ends = false; !ends;) {
       ends = x.ends_unit();
-      const int key0 = x.tile * 64;
+      const int key0 = x.tile * kKeys;
       if (ends) whole = x.tile + 1 == u.tiles;
       x.next();
       // S = Q K^T of this warp's slice
@@ -802,9 +839,9 @@ struct KaFew {
       if (lane == 0) mbar_arrive(&empty[st]);
       ++n;
       // softmax of the slice
-      const int slice_end = key0 + (slice + 1) * kKeys;
+      const int slice_end = key0 + (slice + 1) * kKeysW;
       if (__any_sync(0xffffffffu, min(seen[0], seen[1]) < slice_end)) {
-        const int col0 = key0 + slice * kKeys + 2 * t;
+        const int col0 = key0 + slice * kKeysW + 2 * t;
 #pragma unroll
         for (int kg = 0; kg < MT; ++kg)
 #pragma unroll
@@ -856,27 +893,23 @@ struct KaFew {
       // O += P V
       st = n % C::kHalf;
       if (!warp_wait(&full[st], (n / C::kHalf) & 1, abort_flag)) return false;
-      if (u.len < slice_end) {
-        // keys past the sequence's end: P is zero there, V must be (0 * NaN is not)
-        for (int row = max(u.len - key0, slice * kKeys); row < (slice + 1) * kKeys; ++row)
-          if (lane < HD / 8)
-            *reinterpret_cast<uint4*>(sR + st * C::kStage + (lane >> 3) * 8192 + row * 128 + (lane & 7) * 16) =
-                make_uint4(0, 0, 0, 0);
-        fence_proxy_async_smem();
-        __syncwarp();
-      }
       base = smem_u32(sR) + st * C::kStage + vrow * 128;
 #pragma unroll
       for (int kg = 0; kg < MT; ++kg) {
         const uint32_t p[4] = {pack2<BF16>(sc[kg][0][0], sc[kg][0][1]), pack2<BF16>(sc[kg][0][2], sc[kg][0][3]),
                                pack2<BF16>(sc[kg][1][0], sc[kg][1][1]), pack2<BF16>(sc[kg][1][2], sc[kg][1][3])};
+        // keys past the sequence's end hold whatever was in the page: P is zero there, and
+        // so must V be (0 * NaN is not).  A register has the keys 2 t and 2 t + 1 (+ 8).
+        const int left = u.len - (key0 + slice * kKeysW + kg * 16 + 2 * t);
+        const uint32_t keep0 = left >= 2 ? ~0u : left == 1 ? 0xffffu : 0u;
+        const uint32_t keep1 = left >= 10 ? ~0u : left == 9 ? 0xffffu : 0u;
 #pragma unroll
         for (int i = 0; i < HD / 16; ++i) {
           const int chunk = (i & 3) * 2 + (lane >> 4);
           uint32_t b[4];
           ldsm4_t(base + kg * 2048 + (i >> 2) * 8192 + ((chunk ^ (vrow & 7)) << 4), b);
-          mma16816<BF16>(o[2 * i], p, b[0], b[1]);
-          mma16816<BF16>(o[2 * i + 1], p, b[2], b[3]);
+          mma16816<BF16>(o[2 * i], p, b[0] & keep0, b[1] & keep1);
+          mma16816<BF16>(o[2 * i + 1], p, b[2] & keep0, b[3] & keep1);
         }
       }
       __syncwarp();
@@ -904,33 +937,45 @@ struct KaFew {
     ++units;
     constexpr int V = HD / 32;
     const bool direct = whole && !cut_front;
-#pragma unroll 4
-    for (int pr = warp; pr < u.rows; pr += 4) {
-      const int r = pr & 15, first = (pr >> 4) * kSlices;
-      float2 ml[kSlices];
-      float top = -INFINITY;
+    // a warp has rows warp, warp + 4, ..: four of them at a time, side by side
+#pragma unroll 1
+    for (int p0 = warp; p0 < u.rows; p0 += 16) {
+      float acc[4][V], top[4], sum[4];
 #pragma unroll
-      for (int i = 0; i < kSlices; ++i) {
-        ml[i] = s_ml[(first + i) * 16 + r];
-        top = fmaxf(top, ml[i].x);
+      for (int j = 0; j < 4; ++j) {
+        const int pr = min(p0 + 4 * j, u.rows - 1), r = pr & 15, first = (pr >> 4) * kSlices;
+        float2 ml[kSlices];
+        top[j] = -INFINITY;
+        sum[j] = 0.f;
+#pragma unroll
+        for (int i = 0; i < kSlices; ++i) {
+          ml[i] = s_ml[(first + i) * 16 + r];
+          top[j] = fmaxf(top[j], ml[i].x);
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[j][e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < kSlices; ++i) {
+          const float f = ml[i].y > 0.f ? exp2_ftz(ml[i].x - top[j]) : 0.f;
+          const float* src = part + ((first + i) * 16 + r) * HD + (((lane * V / 2) ^ ((r & 7) << 2)) << 1);
+          sum[j] += f * ml[i].y;
+#pragma unroll
+          for (int e = 0; e < V; ++e) acc[j][e] = fmaf(f, src[e], acc[j][e]);
+        }
       }
-      float acc[V] = {}, sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < kSlices; ++i) {
-        const float f = ml[i].y > 0.f ? exp2_ftz(ml[i].x - top) : 0.f;
-        const float* src = part + ((first + i) * 16 + r) * HD + (((lane * V / 2) ^ ((r & 7) << 2)) << 1);
-        sum += f * ml[i].y;
+      for (int j = 0; j < 4; ++j) {
+        const int pr = p0 + 4 * j;
+        if (pr >= u.rows) break;
+        if (direct) {
+          write_row<HD, BF16>(a, u, head, group, pr, acc[j], top[j], sum[j]);
+        } else {
+          const long long slot = piece_slot(kFew, share, !cut_front, pr);
+          float* dst = w.few.o + slot * HD + lane * V;
 #pragma unroll
-        for (int e = 0; e < V; ++e) acc[e] = fmaf(f, src[e], acc[e]);
-      }
-      if (direct) {
-        write_row<HD, BF16>(a, u, head, group, pr, acc, top, sum);
-      } else {
-        const long long slot = piece_slot(kFew, share, !cut_front, pr);
-        float* dst = w.few.o + slot * HD + lane * V;
-#pragma unroll
-        for (int e = 0; e < V; ++e) dst[e] = acc[e];
-        if (lane == 0) w.few.ml[slot] = make_float2(top, sum);
+          for (int e = 0; e < V; ++e) dst[e] = acc[j][e];
+          if (lane == 0) w.few.ml[slot] = make_float2(top[j], sum[j]);
+        }
       }
     }
     __syncwarp();
@@ -1013,7 +1058,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
 
-  const int cta = blockIdx.x, ctas = gridDim.x;
+  const int cta = blockIdx.x;
   if (warp >= 8) {
   regs_fewer<kRegsOther>();
   if (warp == 8) {
@@ -1064,8 +1109,8 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     // a ring and a producer warp for each of the two warpgroups
     const int r = warp == 11;
     KaCursor x, y;
-    x.init(w, kSingle, KaCursor::start(w, kSingle, cta + r * ctas), c.heads);
-    y.init(w, kFew, KaCursor::start(w, kFew, cta + r * ctas), c.heads);
+    x.init(w, kSingle, KaCursor::start(w, kSingle, 2 * cta + r), c.heads);
+    y.init(w, kFew, KaCursor::start(w, kFew, 2 * cta + r), c.heads);
     if (x.left > 0 || y.left > 0) {
       // the pairs may run for long: a limit of about two minutes
       bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(ring_free, 0, abort_flag, 128 * kWaitLimitCycles));
@@ -1093,7 +1138,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     const uint32_t t_s = uniform(tmem + s * kTile), t_o = t_s + kOCols;
     const uint32_t q_smem = smem_u32(sQ) + s * C::kQ;
     const uint64_t dq = sw128_desc(q_smem);
-    const int4 start_pair = KaCursor::start(w, kPair, cta), start_single = KaCursor::start(w, kSingle, cta + s * ctas);
+    const int4 start_pair = KaCursor::start(w, kPair, cta), start_single = KaCursor::start(w, kSingle, 2 * cta + s);
     bool ok = true;
     int ns = 0, np = 0, nq = 0;  // S tiles, P tiles, units so far
     // The units of a cursor from a ring.  One lane waits and issues: S two tiles ahead of
@@ -1224,11 +1269,11 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     __half* out16 = static_cast<__half*>(a.out);
     bool ok = true;
     int nt = 0;  // tiles of this stream so far
-    const int4 st_pair = KaCursor::start(w, kPair, cta), st_single = KaCursor::start(w, kSingle, cta + s * ctas),
-               st_few = KaCursor::start(w, kFew, cta + s * ctas);
+    const int4 st_pair = KaCursor::start(w, kPair, cta), st_single = KaCursor::start(w, kSingle, 2 * cta + s),
+               st_few = KaCursor::start(w, kFew, 2 * cta + s);
 #pragma unroll 1
     for (int kind = kPair; kind <= kSingle && ok; ++kind) {
-      const int share = kind ? cta + s * ctas : cta;
+      const int share = kind ? 2 * cta + s : cta;
       const int part = kind ? 0 : s;  // the unit's rows of this warpgroup: part * 128 ..
       KaCursor x;
       x.init(w, kind, kind ? st_single : st_pair, c.heads);
@@ -1404,13 +1449,13 @@ __global__ void __launch_bounds__(kAttThreads, 1)
                         half_full + s * C::kHalf, half_empty + s * C::kHalf, joined + 2 * s, s_ml + s * 64,
                         abort_flag};
       f.n = 2 * st_single.w;  // the ring has gone round for the singles
-      const int share = cta + s * ctas;
+      const int share = 2 * cta + s;
       KaCursor x;
       x.init(w, kFew, st_few, c.heads);
       if (x.left > 0) f.fetch_q(x);
       while (ok && x.left > 0) {
         const int rows = x.u.rows;
-        ok = rows <= 16 ? f.template unit<1>(x, share) : rows <= 32 ? f.template unit<2>(x, share) : f.template unit<4>(x, share);
+        ok = rows <= 16 ? f.template unit<1>(x, share) : f.template unit<2>(x, share);
       }
     }
     if (!ok) {
@@ -1454,6 +1499,7 @@ __global__ void __launch_bounds__(256) kv_merge_kernel(const KvAttend a, const K
     // in flight
 #pragma unroll 4
     for (int s = first; s <= last; ++s) {
+      if (l.start[s].count == 0) continue;  // a share without tiles
       const long long slot = piece_slot(kind, s, s == first, r0);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
