@@ -36,12 +36,6 @@
 
 namespace moe {
 
-#ifndef KA_EXTRA
-#define KA_EXTRA 3
-#endif
-#ifndef KA_LEAST
-#define KA_LEAST 2
-#endif
 constexpr int kTile = 128;       // rows of a warpgroup
 constexpr int kKeys = 64;        // keys of a tile
 constexpr int kPlanT = 1024;     // threads of the plan kernel
@@ -75,10 +69,12 @@ constexpr int kMergeRows = 16;
 // Kinds of units: rows of a unit, shares an SM.
 constexpr int kPair = 0, kSingle = 1, kFew = 2, kKinds = 3;
 constexpr int kFewRows = 32;
-// What beginning and ending a unit costs, in tiles.
-constexpr int kUnitExtra = KA_EXTRA;
+// What beginning and ending a unit costs, in tiles of its kind (64 decode contexts of
+// 1 to 8192 tokens: 64 us with 2, 58 with 3, 55 with 5; 33 mixed chunks: 170 with 3, 178
+// with 8).
+__host__ __device__ constexpr int kind_extra(int k) { return k == kPair ? 3 : k == kSingle ? 4 : 5; }
 // The least cost worth a warpgroup of its own.
-constexpr int kLeastShare = KA_LEAST;
+constexpr int kLeastShare = 2;
 __host__ __device__ constexpr int kind_rows(int k) { return k == kPair ? 2 * kTile : k == kSingle ? kTile : kFewRows; }
 __host__ __device__ constexpr int kind_shares(int k) { return k == kPair ? 1 : 2; }
 
@@ -285,7 +281,7 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
     const int tiles = key_tiles(len - m, m - 1);
     // counts (at most 1024 each) in the high bits, cost of a chunk's units in the low 44
     const KaUnit rest{seq, row0, rows - rem, rem, len - m, len, tiles, 0};
-    long long total, mine = few ? (1ll << 44) + tiles + kUnitExtra : 0;
+    long long total, mine = few ? (1ll << 44) + tiles + kind_extra(kFew) : 0;
     long long at = plan_scan(mine, busy, &total);
     constexpr long long kLow = (1ll << 44) - 1;
     if (few) {
@@ -296,7 +292,7 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
     n_few += static_cast<int>(total >> 44);
     work_few += total & kLow;
     if (!__syncthreads_or(single || na > 0)) continue;
-    mine = single ? (1ll << 44) + tiles + kUnitExtra : 0;
+    mine = single ? (1ll << 44) + tiles + kind_extra(kSingle) : 0;
     at = plan_scan(mine, busy, &total);
     if (single) {
       const int j = n_single + static_cast<int>(at >> 44) - 1;
@@ -326,7 +322,7 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
         const int r0 = (j - s_pairs[lo]) * 2 * kTile, r1 = min(r0 + 2 * kTile, e.z * group);
         u = KaUnit{e.x, e.y, r0, r1 - r0, e.w - e.z, e.w, key_tiles(e.w - e.z, (r1 - 1) / group), 0};
         w.pair.list[n_pair + j] = u;
-        mine = u.tiles + kUnitExtra;
+        mine = u.tiles + kind_extra(kPair);
       }
       const long long sum = plan_scan(mine, min((pairs - j0 + 31) / 32, 32), &all);
       if (j < pairs) pre_pair[n_pair + j + 1] = work_pair + sum;
@@ -354,20 +350,21 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
     const int n = k == kPair ? n_pair : k == kSingle ? n_single : n_few;
     const long long* pre = k == kPair ? pre_pair : k == kSingle ? pre_single : pre_few;
     const KaList list = w.kind(k);
+    const int extra = kind_extra(k);
     long long w0, w1;
     l.range(share, &w0, &w1);
     KaStart st{0, 0, 0, 0};
     if (w0 < w1) {
-      const KaPlace p = small ? plan_place<uint32_t>(pre, n, static_cast<uint32_t>(w0), c.heads, kUnitExtra)
-                              : plan_place<unsigned long long>(pre, n, static_cast<unsigned long long>(w0), c.heads, kUnitExtra);
-      long long end = l.all - static_cast<long long>(n) * kUnitExtra * c.heads;
+      const KaPlace p = small ? plan_place<uint32_t>(pre, n, static_cast<uint32_t>(w0), c.heads, extra)
+                              : plan_place<unsigned long long>(pre, n, static_cast<unsigned long long>(w0), c.heads, extra);
+      long long end = l.all - static_cast<long long>(n) * extra * c.heads;
       if (w1 < l.all)
-        end = (small ? plan_place<uint32_t>(pre, n, static_cast<uint32_t>(w1), c.heads, kUnitExtra)
-                     : plan_place<unsigned long long>(pre, n, static_cast<unsigned long long>(w1), c.heads, kUnitExtra)).tiles;
+        end = (small ? plan_place<uint32_t>(pre, n, static_cast<uint32_t>(w1), c.heads, extra)
+                     : plan_place<unsigned long long>(pre, n, static_cast<unsigned long long>(w1), c.heads, extra)).tiles;
       st = KaStart{p.item, p.head, p.tile, static_cast<int>(end - p.tiles)};
       // a unit that is cut here first: its first tile lies in the share that ends here
       if (p.tile > 0) {
-        const int first = l.share_of(p.unit + kUnitExtra);
+        const int first = l.share_of(p.unit + extra);
         long long f0, f1;
         l.range(first, &f0, &f1);
         if (f1 == w0) {
@@ -730,15 +727,11 @@ MOE_DEV void store32(void* p, const uint32_t (&v)[8]) {
                : "memory");
 }
 
-// Results of one packed row: lane's HD / 32 values, the log of the sum.
+// Results of one row and head: lane's HD / 32 values, the log of the sum.
 template <int HD, bool BF16>
-MOE_DEV void write_row(const KvAttend& a, const KaUnit& u, int head, int group, int pr, const float* v,
-                       float top, float sum) {
+MOE_DEV void write_row(const KvAttend& a, long long row, int h, const float* v, float top, float sum) {
   constexpr int V = HD / 32;
   const int lane = threadIdx.x & 31;
-  const int packed = u.r0 + pr;
-  const int tok = packed / group, h = head * group + (packed - tok * group);
-  const long long row = static_cast<long long>(u.row0) + tok;
   const float inv = sum > 0.f ? 1.f / sum : 0.f;
   uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<__half*>(a.out) + row * a.os[0] + h * a.os[1]) + lane * (V / 2);
 #pragma unroll
@@ -763,22 +756,33 @@ struct KaFew {
   int units = 0;  // joins so far
   uint32_t next_q[HD / 16][4];  // Q fragments of the next unit
   int next_seen[2];             // tokens that its rows see
+  // Row `lane` of the unit, the next one's and the current one's: token of the batch and
+  // head of its group.  A division, made once for all kv heads of an entry.
+  int rows_of = -1;  // list entry of the next unit
+  int next_tok, next_hg, next_sees;
+  int tok, hg;
 
   // Q fragments of rows mi * 16 + g and + 8 of the cursor's unit, and the tokens they see
   MOE_DEV void fetch_q(const KaCursor& x) {
     const KaUnit& u = x.u;
-    const int warp = (threadIdx.x >> 5) & 3, g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
-    const int mi = u.rows <= 16 ? 0 : warp >> 1;
+    const int warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    if (rows_of != x.item) {
+      rows_of = x.item;
+      const int packed = u.r0 + min(lane, u.rows - 1);
+      const int k = packed / group;
+      next_hg = packed - k * group;
+      next_tok = u.row0 + k;
+      next_sees = lane < u.rows ? max(min(u.base + k + 1, u.len), 0) : 0;
+    }
+    const long long at = next_tok * a.qs[0] + (static_cast<long long>(x.head) * group + next_hg) * a.qs[1];
+    const int first = u.rows <= 16 ? 0 : (warp >> 1) * 16;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int pr = mi * 16 + g + 8 * r;
+      const int pr = first + g + 8 * r;
+      next_seen[r] = __shfl_sync(0xffffffffu, next_sees, pr);
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const __half*>(a.q) +
+                                                              __shfl_sync(0xffffffffu, at, pr));
       const bool valid = pr < u.rows;
-      const int packed = u.r0 + (valid ? pr : 0);
-      const int tok = packed / group, hg = packed - tok * group;
-      next_seen[r] = valid ? max(min(u.base + tok + 1, u.len), 0) : 0;
-      const uint32_t* src = reinterpret_cast<const uint32_t*>(
-          static_cast<const __half*>(a.q) + (static_cast<long long>(u.row0) + tok) * a.qs[0] +
-          (static_cast<long long>(x.head) * group + hg) * a.qs[1]);
 #pragma unroll
       for (int k = 0; k < HD / 16; ++k) {
         next_q[k][r] = valid ? src[k * 8 + t] : 0u;
@@ -804,11 +808,13 @@ struct KaFew {
 #pragma unroll
       for (int e = 0; e < 4; ++e) q[k][e] = next_q[k][e];
     const int seen[2] = {next_seen[0], next_seen[1]};
+    tok = next_tok;
+    hg = next_hg;
     float o[HD / 8][4];
 #pragma unroll
     for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    bool whole = true;
+    bool whole = true, first = true;
     // lane addresses inside a 16-key group: K rows (lane >> 4) * 8 + (lane & 7), chunk
     // (lane >> 3 & 1); V rows lane & 15, chunk lane >> 4
     const int krow = slice * kKeysW + ((lane >> 4) << 3) + (lane & 7), vrow = slice * kKeysW + (lane & 15);
@@ -880,7 +886,7 @@ struct KaFew {
             }
         l[r] = l[r] * alpha[r] + sum;
       }
-      if (__any_sync(0xffffffffu, grow)) {
+      if (!first && __any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int i = 0; i < HD / 8; ++i) {
           o[i][0] *= alpha[0];
@@ -889,6 +895,7 @@ struct KaFew {
           o[i][3] *= alpha[1];
         }
       }
+      first = false;
       if (ends && x.left > 0) fetch_q(x);  // lands while this unit ends
       // O += P V
       st = n % C::kHalf;
@@ -937,45 +944,36 @@ struct KaFew {
     ++units;
     constexpr int V = HD / 32;
     const bool direct = whole && !cut_front;
-    // a warp has rows warp, warp + 4, ..: four of them at a time, side by side
+    // rows warp, warp + 4, ..  Not unrolled: code that a unit runs once costs more in
+    // instruction fetches than in latency (3 rows side by side: 4,000 cycles, so: 1,500)
 #pragma unroll 1
-    for (int p0 = warp; p0 < u.rows; p0 += 16) {
-      float acc[4][V], top[4], sum[4];
+    for (int pr = warp; pr < u.rows; pr += 4) {
+      const int r = pr & 15, first = (pr >> 4) * kSlices;
+      float2 ml[kSlices];
+      float top = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int pr = min(p0 + 4 * j, u.rows - 1), r = pr & 15, first = (pr >> 4) * kSlices;
-        float2 ml[kSlices];
-        top[j] = -INFINITY;
-        sum[j] = 0.f;
-#pragma unroll
-        for (int i = 0; i < kSlices; ++i) {
-          ml[i] = s_ml[(first + i) * 16 + r];
-          top[j] = fmaxf(top[j], ml[i].x);
-        }
-#pragma unroll
-        for (int e = 0; e < V; ++e) acc[j][e] = 0.f;
-#pragma unroll
-        for (int i = 0; i < kSlices; ++i) {
-          const float f = ml[i].y > 0.f ? exp2_ftz(ml[i].x - top[j]) : 0.f;
-          const float* src = part + ((first + i) * 16 + r) * HD + (((lane * V / 2) ^ ((r & 7) << 2)) << 1);
-          sum[j] += f * ml[i].y;
-#pragma unroll
-          for (int e = 0; e < V; ++e) acc[j][e] = fmaf(f, src[e], acc[j][e]);
-        }
+      for (int i = 0; i < kSlices; ++i) {
+        ml[i] = s_ml[(first + i) * 16 + r];
+        top = fmaxf(top, ml[i].x);
       }
+      float acc[V] = {}, sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int pr = p0 + 4 * j;
-        if (pr >= u.rows) break;
-        if (direct) {
-          write_row<HD, BF16>(a, u, head, group, pr, acc[j], top[j], sum[j]);
-        } else {
-          const long long slot = piece_slot(kFew, share, !cut_front, pr);
-          float* dst = w.few.o + slot * HD + lane * V;
+      for (int i = 0; i < kSlices; ++i) {
+        const float f = ml[i].y > 0.f ? exp2_ftz(ml[i].x - top) : 0.f;
+        const float* src = part + ((first + i) * 16 + r) * HD + (((lane * V / 2) ^ ((r & 7) << 2)) << 1);
+        sum += f * ml[i].y;
 #pragma unroll
-          for (int e = 0; e < V; ++e) dst[e] = acc[j][e];
-          if (lane == 0) w.few.ml[slot] = make_float2(top[j], sum[j]);
-        }
+        for (int e = 0; e < V; ++e) acc[e] = fmaf(f, src[e], acc[e]);
+      }
+      if (direct) {
+        write_row<HD, BF16>(a, __shfl_sync(0xffffffffu, tok, pr), head * group + __shfl_sync(0xffffffffu, hg, pr),
+                            acc, top, sum);
+      } else {
+        const long long slot = piece_slot(kFew, share, !cut_front, pr);
+        float* dst = w.few.o + slot * HD + lane * V;
+#pragma unroll
+        for (int e = 0; e < V; ++e) dst[e] = acc[e];
+        if (lane == 0) w.few.ml[slot] = make_float2(top, sum);
       }
     }
     __syncwarp();
@@ -1522,8 +1520,13 @@ __global__ void __launch_bounds__(256) kv_merge_kernel(const KvAttend a, const K
         for (int x = 0; x < V; ++x) acc[j][x] = fmaf(f2, v[x], acc[j][x] * keep);
       }
     }
-    write_row<HD, BF16>(a, u, e.w, group, r0, acc[0], top[0], sum[0]);
-    if (two) write_row<HD, BF16>(a, u, e.w, group, r0 + 1, acc[1], top[1], sum[1]);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int packed = u.r0 + r0 + j, tok = packed / group;
+      if (j <= two)
+        write_row<HD, BF16>(a, static_cast<long long>(u.row0) + tok, e.w * group + packed - tok * group, acc[j],
+                            top[j], sum[j]);
+    }
   }
 }
 
