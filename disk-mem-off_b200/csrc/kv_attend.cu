@@ -132,40 +132,45 @@ struct KaPtrs {
 };
 
 // ------------------------------------------------------------------ plan
-// Inclusive sum over the plan CTA; *total gets the whole sum.  `busy`: the warps that may
-// hold anything but zero.
-MOE_DEV long long plan_scan(long long v, int busy, long long* total) {
-  __shared__ long long part[32];
+// Inclusive sums of N numbers over the plan CTA, in place; total gets the whole sums.
+// `busy`: the warps that may hold anything but zero.
+template <int N>
+MOE_DEV void plan_scan(long long (&v)[N], int busy, long long (&total)[N]) {
+  __shared__ long long part[N][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (warp < busy) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long u = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += u;
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const long long u = __shfl_up_sync(0xffffffffu, v[k], o);
+        if (lane >= o) v[k] += u;
+      }
     }
-    if (lane == 31) part[warp] = v;
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (lane == 31) part[k][warp] = v[k];
   }
   __syncthreads();
-  long long before = 0, all = 0;
-  if (busy <= 4) {
-    for (int i = 0; i < busy; ++i) {
-      const long long p = part[i];
-      if (i < warp) before += p;
-      all += p;
-    }
-  } else {
-    long long p = lane < busy ? part[lane] : 0;
+  long long p[N];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long u = __shfl_up_sync(0xffffffffu, p, o);
-      if (lane >= o) p += u;
+  for (int k = 0; k < N; ++k) p[k] = lane < busy ? part[k][lane] : 0;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    if (o >= busy) break;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const long long u = __shfl_up_sync(0xffffffffu, p[k], o);
+      if (lane >= o) p[k] += u;
     }
-    all = __shfl_sync(0xffffffffu, p, 31);
-    before = warp ? __shfl_sync(0xffffffffu, p, warp - 1) : 0;
   }
-  *total = all;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    total[k] = __shfl_sync(0xffffffffu, p[k], busy - 1);
+    const long long before = __shfl_sync(0xffffffffu, p[k], max(min(warp, busy) - 1, 0));
+    if (warp) v[k] += before;
+  }
   __syncthreads();  // part is written again by the next call
-  return v + before;
 }
 
 MOE_DEV int key_tiles(int base, int last_token) {
@@ -241,6 +246,7 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
   pdl_enter();
   __shared__ long long spre[kKinds][kPlanSmem + 1];
   __shared__ int s_merges;
+  __shared__ long long s_tiles[kPlanT];
   __shared__ int4 s_entry[kPlanT];       // the chunk's entries: seq, row0, m, len
   __shared__ int s_pairs[kPlanT + 1];    // pairs before each of them
   const int tid = threadIdx.x;
@@ -279,37 +285,35 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
     const int na = rows / (2 * kTile) + (rem > kTile ? 1 : 0);
     const bool single = rem > kFewRows && rem <= kTile, few = rem > 0 && rem <= kFewRows;
     const int tiles = key_tiles(len - m, m - 1);
-    // counts (at most 1024 each) in the high bits, cost of a chunk's units in the low 44
+    // few and single: counts (at most 1024) in the high bits, costs in the low 44; pairs
     const KaUnit rest{seq, row0, rows - rem, rem, len - m, len, tiles, 0};
-    long long total, mine = few ? (1ll << 44) + tiles + kind_extra(kFew) : 0;
-    long long at = plan_scan(mine, busy, &total);
-    constexpr long long kLow = (1ll << 44) - 1;
+    constexpr long long kOne = 1ll << 44, kLow = kOne - 1;
+    long long at[3] = {few ? kOne + tiles + kind_extra(kFew) : 0, single ? kOne + tiles + kind_extra(kSingle) : 0, na};
+    long long total[3];
+    plan_scan(at, busy, total);
     if (few) {
-      const int j = n_few + static_cast<int>(at >> 44) - 1;
+      const int j = n_few + static_cast<int>(at[0] >> 44) - 1;
       w.few.list[j] = rest;
-      pre_few[j + 1] = work_few + (at & kLow);
+      pre_few[j + 1] = work_few + (at[0] & kLow);
     }
-    n_few += static_cast<int>(total >> 44);
-    work_few += total & kLow;
-    if (!__syncthreads_or(single || na > 0)) continue;
-    mine = single ? (1ll << 44) + tiles + kind_extra(kSingle) : 0;
-    at = plan_scan(mine, busy, &total);
     if (single) {
-      const int j = n_single + static_cast<int>(at >> 44) - 1;
+      const int j = n_single + static_cast<int>(at[1] >> 44) - 1;
       w.single.list[j] = rest;
-      pre_single[j + 1] = work_single + (at & kLow);
+      pre_single[j + 1] = work_single + (at[1] & kLow);
     }
-    n_single += static_cast<int>(total >> 44);
-    work_single += total & kLow;
-    at = plan_scan(na, busy, &total);
+    n_few += static_cast<int>(total[0] >> 44);
+    work_few += total[0] & kLow;
+    n_single += static_cast<int>(total[1] >> 44);
+    work_single += total[1] & kLow;
+    if (total[2] == 0) continue;
     s_entry[tid] = make_int4(seq, row0, m, len);
-    s_pairs[tid + 1] = static_cast<int>(at);
+    s_pairs[tid + 1] = static_cast<int>(at[2]);
     if (tid == 0) s_pairs[0] = 0;
     __syncthreads();
-    const int pairs = min(static_cast<int>(total), cap0 - n_pair);
+    const int pairs = min(static_cast<int>(total[2]), cap0 - n_pair);
     for (int j0 = 0; j0 < pairs; j0 += kPlanT) {  // a thread a pair
       const int j = j0 + tid;
-      long long mine = 0, all;
+      long long sum[1] = {0}, all[1];
       KaUnit u{};
       if (j < pairs) {
         int lo = 0, hi = min(b.n - i0, kPlanT);  // s_pairs[lo] <= j < s_pairs[hi]
@@ -322,11 +326,11 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
         const int r0 = (j - s_pairs[lo]) * 2 * kTile, r1 = min(r0 + 2 * kTile, e.z * group);
         u = KaUnit{e.x, e.y, r0, r1 - r0, e.w - e.z, e.w, key_tiles(e.w - e.z, (r1 - 1) / group), 0};
         w.pair.list[n_pair + j] = u;
-        mine = u.tiles + kind_extra(kPair);
+        sum[0] = u.tiles + kind_extra(kPair);
       }
-      const long long sum = plan_scan(mine, min((pairs - j0 + 31) / 32, 32), &all);
-      if (j < pairs) pre_pair[n_pair + j + 1] = work_pair + sum;
-      work_pair += all;
+      plan_scan(sum, min((pairs - j0 + 31) / 32, 32), all);
+      if (j < pairs) pre_pair[n_pair + j + 1] = work_pair + sum[0];
+      work_pair += all[0];
     }
     n_pair += pairs;
   }
@@ -335,46 +339,45 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
   // (2) a thread for each share of each kind
   const int k = tid < num_sms ? kPair : tid < 3 * num_sms ? kSingle : kFew;
   const int share = tid - (k == kPair ? 0 : k == kSingle ? num_sms : 3 * num_sms);
-  if (share < num_sms * kind_shares(k)) {
-    const long long cost_pair = work_pair * c.heads, cost_single = work_single * c.heads, cost_few = work_few * c.heads;
-    const long long line = 2 * cost_pair + cost_single + cost_few;
-    const bool small = line < 0x40000000;
-    const int halves = 2 * num_sms;
-    KaLine l;
-    l.per = max(small ? (static_cast<int>(line) + halves - 1) / halves : (line + halves - 1) / halves,
-                static_cast<long long>(kLeastShare));
-    l.small = small;
-    l.pair = k == kPair;
-    l.before = k == kPair ? 0 : k == kSingle ? 2 * cost_pair : 2 * cost_pair + cost_single;
-    l.all = k == kPair ? cost_pair : k == kSingle ? cost_single : cost_few;
-    const int n = k == kPair ? n_pair : k == kSingle ? n_single : n_few;
-    const long long* pre = k == kPair ? pre_pair : k == kSingle ? pre_single : pre_few;
+  const bool mine = share < num_sms * kind_shares(k);
+  const int extra = kind_extra(k);
+  const int n = k == kPair ? n_pair : k == kSingle ? n_single : n_few;
+  const long long* pre = k == kPair ? pre_pair : k == kSingle ? pre_single : pre_few;
+  const long long cost_pair = work_pair * c.heads, cost_single = work_single * c.heads, cost_few = work_few * c.heads;
+  const long long line = 2 * cost_pair + cost_single + cost_few;
+  KaLine l;
+  l.small = line < 0x40000000;
+  const int halves = 2 * num_sms;
+  l.per = max(l.small ? (static_cast<int>(line) + halves - 1) / halves : (line + halves - 1) / halves,
+              static_cast<long long>(kLeastShare));
+  l.pair = k == kPair;
+  l.before = k == kPair ? 0 : k == kSingle ? 2 * cost_pair : 2 * cost_pair + cost_single;
+  l.all = k == kPair ? cost_pair : k == kSingle ? cost_single : cost_few;
+  long long w0, w1;
+  l.range(share, &w0, &w1);
+  KaPlace p{};
+  p.tiles = l.all - static_cast<long long>(n) * extra * c.heads;
+  if (mine && w0 < l.all)
+    p = l.small ? plan_place<uint32_t>(pre, n, static_cast<uint32_t>(w0), c.heads, extra)
+                : plan_place<unsigned long long>(pre, n, static_cast<unsigned long long>(w0), c.heads, extra);
+  s_tiles[tid] = p.tiles;  // the next share begins where this one ends
+  __syncthreads();
+  if (mine) {
     const KaList list = w.kind(k);
-    const int extra = kind_extra(k);
-    long long w0, w1;
-    l.range(share, &w0, &w1);
-    KaStart st{0, 0, 0, 0};
-    if (w0 < w1) {
-      const KaPlace p = small ? plan_place<uint32_t>(pre, n, static_cast<uint32_t>(w0), c.heads, extra)
-                              : plan_place<unsigned long long>(pre, n, static_cast<unsigned long long>(w0), c.heads, extra);
-      long long end = l.all - static_cast<long long>(n) * extra * c.heads;
-      if (w1 < l.all)
-        end = (small ? plan_place<uint32_t>(pre, n, static_cast<uint32_t>(w1), c.heads, extra)
-                     : plan_place<unsigned long long>(pre, n, static_cast<unsigned long long>(w1), c.heads, extra)).tiles;
-      st = KaStart{p.item, p.head, p.tile, static_cast<int>(end - p.tiles)};
-      // a unit that is cut here first: its first tile lies in the share that ends here
-      if (p.tile > 0) {
-        const int first = l.share_of(p.unit + extra);
-        long long f0, f1;
-        l.range(first, &f0, &f1);
-        if (f1 == w0) {
-          const KaUnit u = list.list[p.item];
-          w.merge[atomicAdd(&s_merges, 1)] =
-              KaMerge{k, first, l.share_of(p.unit + p.cost - 1), p.head, u.row0, u.r0, u.rows, 0};
-        }
+    const long long end = share + 1 < num_sms * kind_shares(k)
+                              ? s_tiles[tid + 1] : l.all - static_cast<long long>(n) * extra * c.heads;
+    list.start[share] = KaStart{p.item, p.head, p.tile, static_cast<int>(end - p.tiles)};
+    // a unit that is cut here first: its first tile lies in the share that ends here
+    if (w0 < w1 && p.tile > 0) {
+      const int first = l.share_of(p.unit + extra);
+      long long f0, f1;
+      l.range(first, &f0, &f1);
+      if (f1 == w0) {
+        const KaUnit u = list.list[p.item];
+        w.merge[atomicAdd(&s_merges, 1)] =
+            KaMerge{k, first, l.share_of(p.unit + p.cost - 1), p.head, u.row0, u.r0, u.rows, 0};
       }
     }
-    list.start[share] = st;
   }
   __syncthreads();
   if (tid == 0) *w.n_merge = s_merges;
