@@ -422,6 +422,99 @@ def test_long_context_split_over_the_gpu() -> None:
     _attend_case("bf16", 16, 2, 64, 128, [(9001, 40)], seed=5)
 
 
+@pytest.mark.parametrize("dtype,dim", [("f16", 128), ("bf16", 64)])
+def test_rows_around_the_unit_sizes(dtype: str, dim: int) -> None:
+    """Chunks whose rows end at and around every size at which another form of the kernel
+    takes over, with few and with many older tokens, all in one batch."""
+    sizes = (15, 16, 17, 31, 32, 33, 64, 65, 127, 128, 129, 255, 256, 257, 288, 289, 384, 385)
+    _attend_case(dtype, 4, 4, dim, 32, [(m + (0, 1, 63, 130, 500)[i % 5], m) for i, m in enumerate(sizes)],
+                 seed=dim)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(200, 1), (34, 2), (5, 5)])
+def test_unusual_groups(heads: int, kv_heads: int) -> None:
+    _attend_case("f16", heads, kv_heads, 64, 16, [(70, 1), (130, 3), (9, 9), (1, 1), (300, 40)], seed=heads)
+
+
+def test_pool_past_32_bit_offsets() -> None:
+    """Pages whose bytes lie past 2^32 in the pool: append, copy on write, attention."""
+    layers, pages, page = 2, 18000, 64
+    k, v = (torch.empty((layers, pages, 8, page, 128), dtype=torch.float16, device="cuda") for _ in range(2))
+    assert k.numel() * 2 > 1 << 32
+    table = torch.full((3, 4), -1, dtype=torch.int32, device="cuda")
+    lengths = torch.zeros(3, dtype=torch.int32, device="cuda")
+    refs = torch.ones(pages, dtype=torch.int32, device="cuda")
+    refs[-6:] = 0                            # only the last pages are free
+    cache = PagedKVCache(k, v, table, lengths, refs)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    new = [torch.randn((100, 8, 128), generator=g, device="cuda").half() for _ in range(2)]
+    cache.reserve([0], [100])
+    cache.append(*new, [0], [0, 100], layer=1)
+    cache.fork([0], [2])
+    cache.reserve([2], [1])
+    one = [torch.randn((1, 8, 128), generator=g, device="cuda").half() for _ in range(2)]
+    cache.append(*one, [2], [0, 1], layer=1)
+    q = torch.randn((1, 96, 128), generator=g, device="cuda").half()
+    out = cache.attend(q, [2], [0, 1], layer=1)
+    cache.status()
+    assert table.tolist()[0][:2] == [pages - 6, pages - 5] and table.tolist()[2][:2] == [pages - 6, pages - 4]
+    kk, vv = (torch.cat([a, b]).double().cpu().numpy() for a, b in zip(new, one))
+    ref, _lse, mag = attend_chunk(q.double().cpu().numpy(), kk, vv, 1 / math.sqrt(128))
+    u = 2.0 ** -11
+    # as _check_rows: two roundings, and the fp32 scores (below 2^-11 too) twice
+    assert (np.abs(out.double().cpu().numpy() - ref) <= u * (mag + np.abs(ref)) + 2 * u * mag).all()
+
+
+def test_starts_past_the_rows_are_reported() -> None:
+    cache, _o = _filled("f16", 16, 2, 64, [77, 40], seed=2)
+    q = torch.randn((4, 4, 64), device="cuda").half()
+    out = torch.full_like(q, 5.0)
+    for starts in ([0, 2, 9], [0, 3, 2], [-3, 2, 4]):
+        cache.attend(q, [0, 1], starts, out=out)
+        with pytest.raises(ValueError):
+            cache.status()
+
+
+def test_two_streams_at_once() -> None:
+    """Attention calls on one cache that overlap on two streams."""
+    cache, _o = _filled("bf16", 32, 2, 128, [3000, 1700, 64, 900], seed=5)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    qs = [torch.randn((n, 16, 128), generator=g, device="cuda").bfloat16() for n in (4, 400)]
+    args = [([0, 1, 2, 3], [0, 1, 2, 3, 4]), ([3, 0], [0, 150, 400])]
+    args = [tuple(_i32(v) for v in a) for a in args]
+    want = [cache.attend(q, *a) for q, a in zip(qs, args)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for i in range(2):
+            got[i].append(cache.attend(qs[i], *args[i], stream=streams[i]))
+    torch.cuda.synchronize()
+    cache.status()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+def test_two_graphs_of_one_cache_replayed_in_turn() -> None:
+    cache, _o = _filled("f16", 16, 2, 64, [500, 90], seed=6, nan=False)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    qs = [torch.randn((n, 8, 64), generator=g, device="cuda").half() for n in (2, 60)]
+    args = [(_i32([0, 1]), _i32([0, 1, 2])), (_i32([1, 0]), _i32([0, 20, 60]))]
+    want = [cache.attend(q, *a) for q, a in zip(qs, args)]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for q, a in zip(qs, args):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(cache.attend(q, *a))
+    for _ in range(3):
+        for i in (0, 1, 1, 0):
+            outs[i].zero_()
+            graphs[i].replay()
+            assert torch.equal(outs[i], want[i])
+    cache.status()
+
+
 def test_many_short_sequences() -> None:
     rng = random.Random(8)
     _attend_case("bf16", 8, 2, 64, 16, [(rng.randint(1, 90), 1) for _ in range(700)], seed=8)
