@@ -144,50 +144,51 @@ __global__ void __launch_bounds__(kPlanThreads) kv_reserve_kernel(const KvView c
     return;
   }
   __syncthreads();
-  // (3) a warp per entry.  Copies: list slot j is entry order, so src / dst / rows of
-  // slot j come from entries i >= j; rows[] is read for all entries before any slot
-  // is written (two passes).
-  const int warp = tid >> 5, lane = tid & 31;
-  for (int i = warp; i < n; i += kPlanThreads / 32) {
-    const int s = seqs[i], have = c.len[s], more = counts[i];
-    if (more <= 0) continue;
-    int* row = c.table + static_cast<int64_t>(s) * c.max_blocks;
-    const int first = blocks_of(c, have), last = blocks_of(c, have + more);
-    const int slot = c.rows[i];
-    int from = c.off[i];
-    if (slot >= 0) {
-      if (lane == 0) {
-        const int old = row[first - 1], fresh = c.list[from];
-        row[first - 1] = fresh;
-        c.refs[fresh] = 1;
-        atomicSub(&c.refs[old], 1);
-        c.src[slot] = old;
-        c.dst[slot] = fresh;
-      }
-      ++from;
-    }
-    for (int j = first + lane; j < last; j += 32) {
-      const int pg = c.list[from + j - first];
-      row[j] = pg;
-      c.refs[pg] = 1;
-    }
-  }
-  __syncthreads();
-  // rows[slot] of each copy, then the lengths; slots are dense and slot <= i, and a
-  // chunk's slots are read by all threads before any of them is written
+  // (3) a thread per entry; entries with many pages by their whole warp.  A copy's slot is
+  // its rank among the copies, at most its entry's number: rows[] of a chunk is read by all
+  // threads before any slot of it is written.
+  const int lane = tid & 31;
   for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
     const int i = i0 + tid;
-    int slot = -1, s = 0, have = 0;
+    int s = 0, have = 0, more = 0, slot = -1, from = 0;
     if (i < n) {
-      slot = c.rows[i];
       s = seqs[i];
+      more = counts[i];
+      slot = c.rows[i];
+      from = c.off[i];
       have = c.len[s];
     }
+    int* row = c.table + static_cast<int64_t>(s) * c.max_blocks;
+    const int first = blocks_of(c, have), last = more > 0 ? blocks_of(c, have + more) : first;
     __syncthreads();
-    if (i < n) {
-      if (slot >= 0) c.rows[slot] = have & (c.page - 1);
-      c.len[s] = have + counts[i];
+    if (slot >= 0) {
+      const int old = row[first - 1], fresh = c.list[from++];
+      row[first - 1] = fresh;
+      c.refs[fresh] = 1;
+      atomicSub(&c.refs[old], 1);
+      c.src[slot] = old;
+      c.dst[slot] = fresh;
+      c.rows[slot] = have & (c.page - 1);
     }
+    const bool many = last - first > 4;
+    if (!many) {
+      for (int j = first; j < last; ++j) {
+        const int pg = c.list[from + j - first];
+        row[j] = pg;
+        c.refs[pg] = 1;
+      }
+    }
+    for (uint32_t todo = __ballot_sync(0xffffffffu, many); todo; todo &= todo - 1) {
+      const int l = __ffs(todo) - 1;
+      const int at = __shfl_sync(0xffffffffu, first, l), to = __shfl_sync(0xffffffffu, last, l);
+      const int lf = __shfl_sync(0xffffffffu, from, l), ls = __shfl_sync(0xffffffffu, s, l);
+      for (int j = at + lane; j < to; j += 32) {
+        const int pg = c.list[lf + j - at];
+        c.table[static_cast<int64_t>(ls) * c.max_blocks + j] = pg;
+        c.refs[pg] = 1;
+      }
+    }
+    if (i < n) c.len[s] = have + more;
     __syncthreads();
   }
   if (tid == 0) *c.count = static_cast<int>(run >> kCopyBit);
@@ -221,20 +222,21 @@ __global__ void __launch_bounds__(256) kv_copy_kernel(const KvView from, const K
     char* b = (val ? to.v : to.k) + l * ts[0] + from.dst[i] * ts[1] + h * ts[2];
     const int nc = (rows ? rows[i] : from.page) << chunks_shift;
     const int cmask = (1 << chunks_shift) - 1;
+    // lane's chunk of row r0, and the rows that 32 lanes cover in a step
+    const int step = 32 >> chunks_shift;
+    const int64_t fstep = step * fs[3], tstep = step * ts[3];
+    const char* pa = a + (lane >> chunks_shift) * fs[3] + (lane & cmask) * 16;
+    char* pb = b + (lane >> chunks_shift) * ts[3] + (lane & cmask) * 16;
     for (int c0 = lane; c0 < nc; c0 += 256) {
       uint4 q[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int ch = c0 + 32 * u;
-        if (ch < nc)
-          q[u] = *reinterpret_cast<const uint4*>(a + (ch >> chunks_shift) * fs[3] + (ch & cmask) * 16);
-      }
+      for (int u = 0; u < 8; ++u)
+        if (c0 + 32 * u < nc) q[u] = *reinterpret_cast<const uint4*>(pa + u * fstep);
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int ch = c0 + 32 * u;
-        if (ch < nc)
-          *reinterpret_cast<uint4*>(b + (ch >> chunks_shift) * ts[3] + (ch & cmask) * 16) = q[u];
-      }
+      for (int u = 0; u < 8; ++u)
+        if (c0 + 32 * u < nc) *reinterpret_cast<uint4*>(pb + u * tstep) = q[u];
+      pa += 8 * fstep;
+      pb += 8 * tstep;
     }
   }
 }
