@@ -23,9 +23,18 @@
 // swizzle) into one ring, warp 11 the Q tiles; warps 9 and 10 issue S = Q K^T (both
 // operands in shared memory, K major) and O += P V (P from TMEM, V as an N-major operand,
 // so that V needs no transposed copy), one for each softmax warpgroup: a single issuing
-// warp took 2,590 cycles for a tile of both, most of them between the products.  TMEM: two S buffers of 64 keys for each
-// warpgroup (P overwrites its S) and its O, 512 columns in all.  S runs two tiles ahead
-// of the product with V, so the softmax finds its next S ready.
+// warp took 2,590 cycles for a tile of both, most of them between the products.  TMEM: two
+// S buffers of 64 keys for each warpgroup (P overwrites its S) and its O, 512 columns in
+// all.  S runs two tiles ahead of the product with V, so the softmax finds its next S
+// ready.  (Tiles of 128 keys leave no room for a second S buffer; with one, 64-wide heads
+// took 51 us instead of 40.)  Every wait is bounded.
+//
+// What bounds it.  Decode: the reading of K and V (2 x 131071 tokens: 1.07 GB in 186 us,
+// 5.8 TB/s).  Chunks: of the 2,100 cycles that 64 keys of a pair take, the tensor cores
+// have 1,280 and the special-function units 1,024, and the clock falls to about 1.4 GHz
+// under the power limit (4096 new on 4096 cached tokens: 1.25 ms, 0.99 PFLOP/s; a
+// polynomial in place of every eighth to every second exponential: no gain, then a loss).  Short units: instructions
+// that run once a unit, in two warps a scheduler.
 #include <cuda_bf16.h>
 #include <math.h>
 
@@ -610,9 +619,7 @@ MOE_DEV bool elect_one() {
       "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
   return p != 0;
 }
-// The same value in every lane, known as such to the compiler: the tensor-core
-// instructions take their descriptors from uniform registers, and values that it must
-// first move there cost more issue time than the products take.
+// The same value in every lane, and known as such to the compiler.
 MOE_DEV uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 // The whole warp waits and takes the same way out.
@@ -948,7 +955,7 @@ struct KaFew {
     constexpr int V = HD / 32;
     const bool direct = whole && !cut_front;
     // rows warp, warp + 4, ..  Not unrolled: code that a unit runs once costs more in
-    // instruction fetches than in latency (3 rows side by side: 4,000 cycles, so: 1,500)
+    // issue than in latency (3 rows side by side: 4,000 cycles, so: 2,200)
 #pragma unroll 1
     for (int pr = warp; pr < u.rows; pr += 4) {
       const int r = pr & 15, first = (pr >> 4) * kSlices;
@@ -1193,11 +1200,15 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         if (lead) {
           for (int j = -2; ok && j < behind; ++j) {
             if (j >= 0) ok = product(j == 0);
-            if (ok && j + 2 < nt) {  // S into buffer ns & 1, which P of two tiles before has left
+            if (ok && j + 2 < nt) {
+              const int buf = ns & 1;
               ok = mbar_wait_bounded(&fullb[st], ph, abort_flag);
+              // the buffer holds P of two tiles before until its product is done: products of
+              // different shapes are not promised to run in the order of their issue.  (Without
+              // the wait 4096 new on 4096 cached tokens took 1.19 ms instead of 1.25.)
+              if (ok && ns >= 2) ok = mbar_wait_bounded(&o_done[2 * s + buf], ((ns - 2) >> 1) & 1, abort_flag);
               if (!ok) break;
               tc_fence_after();
-              const int buf = ns & 1;
               const uint64_t dk = dk0 + static_cast<uint32_t>(st * (C::kStage >> 4));
 #pragma unroll
               for (int k = 0; k < HD / 16; ++k)  // offsets in the descriptors' units of 16 bytes
@@ -1477,7 +1488,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
 // Joins the pieces of cut units, in share order: 16 rows a CTA and step, two rows a warp.
 // A kernel of its own, since its reading (two or more fp32 pieces a row) wants the whole
 // GPU: joined by the last warp of a unit inside the attention kernel, 33 mixed chunks took
-// 293 us instead of 241.
+// 293 us instead of 241 (at that time).
 template <int HD, bool BF16>
 __global__ void __launch_bounds__(256) kv_merge_kernel(const KvAttend a, const KaPtrs w, const int group) {
   pdl_enter();

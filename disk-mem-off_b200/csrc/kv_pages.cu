@@ -449,8 +449,9 @@ __global__ void __launch_bounds__(256) kv_compact_tables_kernel(const KvView c, 
 
 // ------------------------------------------------------------------ append
 // A warp per row: all heads of the row's key, then of its value, 16 bytes a lane.
-// Bound by HBM for long chunks (each byte read and written once), by the launch and
-// three dependent loads (entry, length, page) for a decode step.
+// Bound by HBM for long chunks (each byte read and written once; 10,168 rows of 8 heads, 83
+// MB: 16.3 us, 5.1 TB/s), by the launch and three dependent loads (entry, length, page) for
+// a decode step (2.8 us).
 __global__ void __launch_bounds__(128) kv_append_kernel(const KvView c, const KvBatch b, int layer,
                                                         const char* __restrict__ k,
                                                         const char* __restrict__ v, int64_t kt,

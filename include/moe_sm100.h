@@ -431,8 +431,9 @@ int moe_kv_append(MoeKvCache* cache, int32_t layer, const void* k, const void* v
  * to its own position; fp32 softmax and accumulation, probabilities rounded to the cache's
  * dtype for the product with v.  lse (may be NULL): natural logarithm of the sum of the
  * exponentials.  A row that sees no token (more new rows than tokens) gives 0 and -inf.
- * Rows of out and lse from q_start[n_seqs] on are left as they were.  No finite value in
- * the pool past a sequence's length, and no NaN or infinity there either, reaches a result. */
+ * Rows of out and lse from q_start[n_seqs] on are left as they were.  Nothing that the pool
+ * holds past a sequence's length reaches a result, NaN and infinities included; among a
+ * sequence's own values they reach every row of the same chunk (weight 0 times infinity). */
 typedef struct MoeKvAttendArgs {
   const void* q;          /* [rows][heads][head_dim], the cache's dtype                */
   void* out;              /* as q                                                      */
