@@ -70,7 +70,7 @@ struct KaStart {
 // A unit that the ends of shares cut: its pieces lie in shares first .. last.
 struct KaMerge {
   int kind, first, last, head;
-  int row0, r0, rows, pad;  // of the unit
+  int item, pad[3];
 };
 static_assert(sizeof(KaStart) == 16 && sizeof(KaMerge) == 32, "16-byte loads");
 constexpr int kMergeRows = 16;
@@ -381,11 +381,9 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
       const int first = l.share_of(p.unit + extra);
       long long f0, f1;
       l.range(first, &f0, &f1);
-      if (f1 == w0) {
-        const KaUnit u = list.list[p.item];
+      if (f1 == w0)
         w.merge[atomicAdd(&s_merges, 1)] =
-            KaMerge{k, first, l.share_of(p.unit + p.cost - 1), p.head, u.row0, u.r0, u.rows, 0};
-      }
+            KaMerge{k, first, l.share_of(p.unit + p.cost - 1), p.head, p.item, {0, 0, 0}};
     }
   }
   __syncthreads();
@@ -1492,54 +1490,69 @@ __global__ void __launch_bounds__(kAttThreads, 1)
 template <int HD, bool BF16>
 __global__ void __launch_bounds__(256) kv_merge_kernel(const KvAttend a, const KaPtrs w, const int group) {
   pdl_enter();
-  constexpr int V = HD / 32;
+  constexpr int V = HD / 32, P = 4;  // pieces at a time, for loads in flight
   const int lane = threadIdx.x & 31;
   const int r0 = blockIdx.y * kMergeRows + 2 * (threadIdx.x >> 5);
   const int n = *w.n_merge;
   for (int i = blockIdx.x; i < n; i += gridDim.x) {
-    const int4 e = reinterpret_cast<const int4*>(w.merge + i)[0], f = reinterpret_cast<const int4*>(w.merge + i)[1];
+    const int4 e = *reinterpret_cast<const int4*>(w.merge + i);
+    const int item = w.merge[i].item;
     const int kind = e.x, first = e.y, last = e.z;
-    KaUnit u;
-    u.row0 = f.x;
-    u.r0 = f.y;
-    u.rows = f.z;
-    if (r0 >= u.rows) continue;
     const KaList l = w.kind(kind);
-    const int two = r0 + 1 < u.rows ? 1 : 0;  // or the same row again, not written
+    const int4 u0 = *reinterpret_cast<const int4*>(l.list + item);  // seq, row0, r0, rows
     float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, acc[2][V] = {};
-    // the running maximum of the pieces moves with them: one pass, loads of four pieces
-    // in flight
-#pragma unroll 4
-    for (int s = first; s <= last; ++s) {
-      if (l.start[s].count == 0) continue;  // a share without tiles
-      const long long slot = piece_slot(kind, s, s == first, r0);
+    for (int base = first; base <= last; base += 32) {
+      // shares of the unit that have tiles
+      const int mine = base + lane;
+      const bool has = mine <= last && l.start[mine].count > 0;
+      if (r0 >= u0.w) break;
+      for (uint32_t todo = __ballot_sync(0xffffffffu, has); todo;) {
+        float2 ml[P][2];
+        float v[P][2][V];
+        bool on[P];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float2 ml = l.ml[slot + j * two];
-        const float* src = l.o + (slot + j * two) * HD + lane * V;
-        float v[V];
-        if constexpr (V == 4) {
-          const float4 t = *reinterpret_cast<const float4*>(src);
-          v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
-        } else {
-          const float2 t = *reinterpret_cast<const float2*>(src);
-          v[0] = t.x; v[1] = t.y;
+        for (int q = 0; q < P; ++q) {
+          on[q] = todo != 0;
+          const int s = base + (on[q] ? __ffs(todo) - 1 : 0);
+          todo &= todo - 1;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const long long slot = piece_slot(kind, s, s == first, min(r0 + j, u0.w - 1));
+            ml[q][j] = l.ml[slot];
+            const float* src = l.o + slot * HD + lane * V;
+            if constexpr (V == 4) {
+              const float4 t = *reinterpret_cast<const float4*>(src);
+              v[q][j][0] = t.x; v[q][j][1] = t.y; v[q][j][2] = t.z; v[q][j][3] = t.w;
+            } else {
+              const float2 t = *reinterpret_cast<const float2*>(src);
+              v[q][j][0] = t.x; v[q][j][1] = t.y;
+            }
+          }
         }
-        const float up = fmaxf(top[j], ml.x);
-        const float keep = top[j] == -INFINITY ? 0.f : exp2_ftz(top[j] - up);
-        const float f2 = ml.x == -INFINITY ? 0.f : exp2_ftz(ml.x - up);
-        top[j] = up;
-        sum[j] = sum[j] * keep + f2 * ml.y;
+        // the running maximum moves with the pieces, in share order
 #pragma unroll
-        for (int x = 0; x < V; ++x) acc[j][x] = fmaf(f2, v[x], acc[j][x] * keep);
+        for (int q = 0; q < P; ++q) {
+          if (!on[q]) break;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float up = fmaxf(top[j], ml[q][j].x);
+            const float keep = top[j] == -INFINITY ? 0.f : exp2_ftz(top[j] - up);
+            const float f = ml[q][j].x == -INFINITY ? 0.f : exp2_ftz(ml[q][j].x - up);
+            top[j] = up;
+            // a piece without a visible token holds nothing, whatever its rows say
+            sum[j] = sum[j] * keep + (f > 0.f ? f * ml[q][j].y : 0.f);
+#pragma unroll
+            for (int x = 0; x < V; ++x) acc[j][x] = acc[j][x] * keep + (f > 0.f ? f * v[q][j][x] : 0.f);
+          }
+        }
       }
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int packed = u.r0 + r0 + j, tok = packed / group;
-      if (j <= two)
-        write_row<HD, BF16>(a, static_cast<long long>(u.row0) + tok, e.w * group + packed - tok * group, acc[j],
-                            top[j], sum[j]);
+      const int packed = u0.z + r0 + j, tok = packed / group;
+      if (r0 + j < u0.w)
+        write_row<HD, BF16>(a, static_cast<long long>(u0.y) + tok, e.w * group + packed - tok * group, acc[j], top[j],
+                            sum[j]);
     }
   }
 }

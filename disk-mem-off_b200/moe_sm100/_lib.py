@@ -209,7 +209,7 @@ def lib() -> ctypes.CDLL:
 
 
 def check(rc: int) -> None:
-    if rc == MOE_OK:
+    if not rc:  # MOE_OK
         return
     msg = lib().moe_last_error().decode(errors="replace")
     if rc in (MOE_ERR_INVALID, MOE_ERR_WORKSPACE):

@@ -127,26 +127,31 @@ class PagedKVCache:
     # -- arguments ----------------------------------------------------------------
     # A decode step makes these calls once a layer, and its kernels take some
     # microseconds: the checks read the tensors as little as they can.
-    def _index(self, name: str, t: Any) -> Any:
-        """``t`` as a contiguous 1-D int32 tensor on the cache's device."""
+    def _index(self, name: str, t: Any) -> tuple[Any, int]:
+        """``t`` as a contiguous 1-D int32 tensor on the cache's device, and its length."""
         try:
-            if t.dtype is self._i32 and t.get_device() == self._dev and t.dim() == 1:
-                return t if t.is_contiguous() else t.contiguous()
-        except AttributeError:
-            return _torch().tensor(list(t), dtype=self._i32).to(self.device)
+            if t.dtype is self._i32 and t.get_device() == self._dev:
+                n, = t.shape
+                return (t if t.is_contiguous() else t.contiguous()), n
+        except AttributeError:  # not a tensor
+            t = _torch().tensor(list(t), dtype=self._i32).to(self.device)
+            return t, t.shape[0]
+        except ValueError:      # not 1-D
+            pass
         raise TypeError(f"{name} must be a 1-D int32 tensor on {self.device}")
 
-    def _indices(self, a: str, x: Any, b: str, y: Any) -> tuple[Any, Any, int]:
-        x, y = self._index(a, x), self._index(b, y)
-        n = len(x)
-        if len(y) != n:
+    def _indices(self, a: str, x: Any, b: str, y: Any) -> tuple[int, int, int, Any]:
+        """Two index arrays of one length: their addresses, the length, what keeps them alive."""
+        x, n = self._index(a, x)
+        y, m = self._index(b, y)
+        if n != m:
             raise ValueError(f"{a} and {b} must have one entry each")
-        return x, y, n
+        return x.data_ptr(), y.data_ptr(), n, (x, y)
 
     def _batch(self, seqs: Any, starts: Any) -> tuple[Any, Any, int]:
-        seqs, starts = self._index("seqs", seqs), self._index("starts", starts)
-        n = len(seqs)
-        if len(starts) != n + 1:
+        seqs, n = self._index("seqs", seqs)
+        starts, m = self._index("starts", starts)
+        if m != n + 1:
             raise ValueError("starts must have one entry more than seqs")
         return seqs, starts, n
 
@@ -180,40 +185,37 @@ class PagedKVCache:
         """Lengthen ``seqs[i]`` by ``counts[i]`` tokens, with pages for them."""
         if stream is not None:
             return self._on(stream, self.reserve, seqs, counts)
-        seqs, counts, n = self._indices("seqs", seqs, "counts", counts)
-        check(self._lib.moe_kv_reserve(self._h, seqs.data_ptr(), counts.data_ptr(), n, self._stream()))
+        x, y, n, _keep = self._indices("seqs", seqs, "counts", counts)
+        check(self._lib.moe_kv_reserve(self._h, x, y, n, self._raw_stream(self._dev)))
 
     def fork(self, parents: Any, children: Any, stream: Any = None) -> None:
         """Make the empty sequence ``children[i]`` a copy of ``parents[i]`` that shares
         its pages; a page is copied when one of its holders next writes to it."""
         if stream is not None:
             return self._on(stream, self.fork, parents, children)
-        parents, children, n = self._indices("parents", parents, "children", children)
-        check(self._lib.moe_kv_fork(self._h, parents.data_ptr(), children.data_ptr(), n,
-                                    self._stream()))
+        x, y, n, _keep = self._indices("parents", parents, "children", children)
+        check(self._lib.moe_kv_fork(self._h, x, y, n, self._raw_stream(self._dev)))
 
     def truncate(self, seqs: Any, lengths: Any, stream: Any = None) -> None:
         """Shorten ``seqs[i]`` to ``lengths[i]`` tokens and let its other pages go."""
         if stream is not None:
             return self._on(stream, self.truncate, seqs, lengths)
-        seqs, lengths, n = self._indices("seqs", seqs, "lengths", lengths)
-        check(self._lib.moe_kv_truncate(self._h, seqs.data_ptr(), lengths.data_ptr(), n,
-                                        self._stream()))
+        x, y, n, _keep = self._indices("seqs", seqs, "lengths", lengths)
+        check(self._lib.moe_kv_truncate(self._h, x, y, n, self._raw_stream(self._dev)))
 
     def free(self, seqs: Any, stream: Any = None) -> None:
         """Empty the sequences: ``truncate`` to no tokens."""
         if stream is not None:
             return self._on(stream, self.free, seqs)
-        seqs = self._index("seqs", seqs)
+        seqs, _n = self._index("seqs", seqs)
         self.truncate(seqs, _torch().zeros_like(seqs))
 
     def copy_pages(self, src: Any, dst: Any, stream: Any = None) -> None:
         """Copy pages ``src[i]`` to ``dst[i]`` in every layer; tables and refs stay."""
         if stream is not None:
             return self._on(stream, self.copy_pages, src, dst)
-        src, dst, n = self._indices("src", src, "dst", dst)
-        check(self._lib.moe_kv_copy_pages(self._h, src.data_ptr(), dst.data_ptr(), n,
-                                          self._stream()))
+        x, y, n, _keep = self._indices("src", src, "dst", dst)
+        check(self._lib.moe_kv_copy_pages(self._h, x, y, n, self._raw_stream(self._dev)))
 
     def compact(self, into: "PagedKVCache | None" = None, stream: Any = None) -> None:
         """Move the live pages to the lowest numbers, or, dense and in order, ``into``
