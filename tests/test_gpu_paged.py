@@ -520,6 +520,15 @@ def test_many_short_sequences() -> None:
     _attend_case("bf16", 8, 2, 64, 16, [(rng.randint(1, 90), 1) for _ in range(700)], seed=8)
 
 
+def test_more_units_than_the_plan_holds_on_chip() -> None:
+    """More than 512 units of 256 rows, and more entries than the planning CTA has threads,
+    chunks among the last of them."""
+    _attend_case("f16", 16, 1, 64, 16, [(230 + i, 230) for i in range(40)], seed=10)
+    rng = random.Random(11)
+    work = [(rng.randint(1, 70), 1) for _ in range(1400)] + [(300, 300), (170, 65), (9, 9), (64, 40)]
+    _attend_case("bf16", 4, 2, 64, 16, work, seed=11)
+
+
 def test_layers_scale_and_padding() -> None:
     _attend_case("f16", 8, 2, 128, 32, [(200, 3), (40, 1)], layers=3, layer=2, seed=6, scale=0.25,
                  pad=9)
