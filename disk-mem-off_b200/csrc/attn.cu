@@ -708,12 +708,14 @@ __global__ void __launch_bounds__(kFaThreads, 1) attn_fwd_kernel(const __grid_co
 __global__ void __launch_bounds__(256) attn_out_kernel(const float* __restrict__ x,
                                                        const float* __restrict__ planes, int nsplit,
                                                        size_t n, float* __restrict__ out,
-                                                       const int* __restrict__ rows, int H) {
+                                                       const int* __restrict__ first,
+                                                       const int* __restrict__ end, int H) {
   pdl_enter();
   // n is a multiple of 4 (H is a multiple of 64): float4 at a time, planes in order; with
-  // rows only its first *rows rows
-  const size_t n4 = (rows ? min(n, static_cast<size_t>(max(*rows, 0)) * H) : n) / 4;
-  for (size_t i = blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x; i < n4;
+  // first and end only rows *first .. *end - 1
+  const size_t n4 = (end ? min(n, static_cast<size_t>(max(*end, 0)) * H) : n) / 4;
+  const size_t i0 = first ? static_cast<size_t>(max(*first, 0)) * H / 4 : 0;
+  for (size_t i = i0 + blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x; i < n4;
        i += static_cast<size_t>(gridDim.x) * blockDim.x) {
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int s = 0; s < nsplit; ++s) {
@@ -789,7 +791,7 @@ static cudaError_t attn_launch(const AttnPlan& a, const AttnWs& w, char* ws, con
   const size_t n = static_cast<size_t>(T) * a.H;
   const int grid = static_cast<int>(std::min<size_t>((n + 255) / 256, static_cast<size_t>(a.num_sms) * 8));
   MOE_PDL(attn_out_kernel, dim3(grid), dim3(256), 0, s, x, reinterpret_cast<const float*>(ws + w.oplanes),
-          w.s2, n, out, static_cast<const int*>(nullptr), a.H);
+          w.s2, n, out, static_cast<const int*>(nullptr), static_cast<const int*>(nullptr), a.H);
   return cudaSuccess;
 }
 
@@ -826,7 +828,7 @@ static cudaError_t attn_cached_launch(const AttnPlan& a, const MoeKvCache& c, co
   const size_t n = static_cast<size_t>(T) * a.H;
   const int grid = static_cast<int>(std::min<size_t>((n + 255) / 256, static_cast<size_t>(a.num_sms) * 8));
   MOE_PDL(attn_out_kernel, dim3(grid), dim3(256), 0, s, x, reinterpret_cast<const float*>(ws + w.oplanes), w.s2, n,
-          out, b.q_start + b.n, a.H);
+          out, b.q_start, b.q_start + b.n, a.H);
   return cudaSuccess;
 }
 

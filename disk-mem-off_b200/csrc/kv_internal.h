@@ -54,11 +54,12 @@ struct KvBatch {
 };
 
 #ifdef __CUDACC__
-// The entry of row r: the last e with q_start[e] <= r, by a warp (32 probes a round).
+// The entry of row r: the last e with q_start[e] <= r, -1 before the first (n > 0), by a
+// warp (32 probes a round, one round at least: a single entry may begin after row r too).
 MOE_DEV int entry_of_row(const int* __restrict__ q_start, int n, int r) {
   const int lane = threadIdx.x & 31;
-  int lo = 0, hi = n;  // answer in [lo, hi)
-  while (hi - lo > 1) {
+  int lo = 0, hi = n;  // answer in [lo, hi), once q_start[lo] <= r
+  do {
     const int step = (hi - lo + 31) / 32;
     const int at = lo + lane * step;
     const bool le = at < hi && q_start[at] <= r;
@@ -67,7 +68,7 @@ MOE_DEV int entry_of_row(const int* __restrict__ q_start, int n, int r) {
     const int j = 31 - __clz(m);
     hi = min(hi, lo + (j + 1) * step);
     lo += j * step;
-  }
+  } while (hi - lo > 1);
   return lo;
 }
 #endif

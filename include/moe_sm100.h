@@ -422,8 +422,8 @@ int moe_kv_compact(MoeKvCache* cache, MoeKvCache* into, void* stream);
 /* New rows of a batch: entry i owns rows q_start[i] .. q_start[i+1]-1 (q_start: n_seqs + 1
  * non-decreasing offsets), the last tokens of sequence seqs[i]: row r is its token
  * lengths[seqs[i]] - (q_start[i+1] - r).  Reserve first.  k, v: [rows][kv_heads][head_dim] in
- * the cache's dtype, token and head strides in elements (multiples of 8).  Rows from
- * q_start[n_seqs] on are ignored.  The same sequence twice: the rows of one entry win. */
+ * the cache's dtype, token and head strides in elements (multiples of 8).  Rows before
+ * q_start[0] and from q_start[n_seqs] on are ignored.  The same sequence twice: the rows of one entry win. */
 int moe_kv_append(MoeKvCache* cache, int32_t layer, const void* k, const void* v, int64_t k_token,
                   int64_t k_head, int64_t v_token, int64_t v_head, const int32_t* seqs,
                   const int32_t* q_start, int32_t n_seqs, int32_t rows, void* stream);
@@ -431,7 +431,7 @@ int moe_kv_append(MoeKvCache* cache, int32_t layer, const void* k, const void* v
  * to its own position; fp32 softmax and accumulation, probabilities rounded to the cache's
  * dtype for the product with v.  lse (may be NULL): natural logarithm of the sum of the
  * exponentials.  A row that sees no token (more new rows than tokens) gives 0 and -inf.
- * Rows of out and lse from q_start[n_seqs] on are left as they were.  Nothing that the pool
+ * Rows of out and lse before q_start[0] and from q_start[n_seqs] on are left as they were.  Nothing that the pool
  * holds past a sequence's length reaches a result, NaN and infinities included; among a
  * sequence's own values they reach every row of the same chunk (weight 0 times infinity). */
 typedef struct MoeKvAttendArgs {
@@ -461,8 +461,8 @@ int moe_kv_status(MoeKvCache* cache, void* stream);
  * a paged cache: out = x + attention(x) for the T rows of x, each at its own position; the
  * rows' keys and values are written to layer `layer` of the cache, whose older tokens they
  * attend to.  Reserve first (once for all layers); seqs, q_start, n_seqs as moe_kv_append;
- * the cache is f16 with the plan's kv_heads and head_dim.  Rows of out from q_start[n_seqs]
- * on are left as they were.  Errors of the sequences are reported by moe_kv_status. */
+ * the cache is f16 with the plan's kv_heads and head_dim.  Rows of out before q_start[0] and
+ * from q_start[n_seqs] on are left as they were.  Errors of the sequences are reported by moe_kv_status. */
 uint64_t moe_attn_cached_workspace_bytes(const MoeAttn* attn, const MoeKvCache* cache, int32_t T,
                                          int32_t n_seqs);
 int moe_attn_forward_cached(MoeAttn* attn, MoeKvCache* cache, int32_t layer, const float* x_dev,
