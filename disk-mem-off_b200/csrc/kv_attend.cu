@@ -183,9 +183,10 @@ MOE_DEV void plan_scan(long long (&v)[N], int busy, long long (&total)[N]) {
 }
 
 MOE_DEV int key_tiles(int base, int last_token) {
-  // tokens visible to the unit's last row, at least one tile (rows that see nothing
-  // still have to be written); beyond the table they read as zeros and are masked
-  const long long vis = static_cast<long long>(max(base, 0)) + last_token + 1;
+  // tokens visible to the unit's last row, at least one tile (rows that see nothing still
+  // have to be written).  So only the last tile holds keys past the sequence's end, with
+  // fewer tokens than new rows (base < 0) too: the MMA warps rely on it when they clear V.
+  const long long vis = max(static_cast<long long>(base) + last_token + 1, 1ll);
   return static_cast<int>((vis + kKeys - 1) / kKeys);
 }
 
