@@ -736,17 +736,19 @@ MOE_DEV void store32(void* p, const uint32_t (&v)[8]) {
                : "memory");
 }
 
-// Results of one row and head: lane's HD / 32 values, the log of the sum.
+// Results of one row and head: lane's HD / 32 values, the log of the sum.  Whether the row
+// sees a token is told by its position, not by the sum: scores of NaN or of -inf alone leave
+// no maximum either, and give NaN.
 template <int HD, bool BF16>
-MOE_DEV void write_row(const KvAttend& a, long long row, int h, const float* v, float top, float sum) {
+MOE_DEV void write_row(const KvAttend& a, long long row, int h, const float* v, float top, float sum, bool sees) {
   constexpr int V = HD / 32;
   const int lane = threadIdx.x & 31;
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  const float inv = 1.f / sum;
   uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<__half*>(a.out) + row * a.os[0] + h * a.os[1]) + lane * (V / 2);
 #pragma unroll
-  for (int e = 0; e < V / 2; ++e) dst[e] = pack2<BF16>(v[2 * e] * inv, v[2 * e + 1] * inv);
+  for (int e = 0; e < V / 2; ++e) dst[e] = sees ? pack2<BF16>(v[2 * e] * inv, v[2 * e + 1] * inv) : 0u;
   if (a.lse && lane == 0)
-    a.lse[row * a.ls[0] + h * a.ls[1]] = sum > 0.f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+    a.lse[row * a.ls[0] + h * a.ls[1]] = sees ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
 }
 
 template <int HD, bool BF16>
@@ -769,7 +771,7 @@ struct KaFew {
   // head of its group.  A division, made once for all kv heads of an entry.
   int rows_of = -1;  // list entry of the next unit
   int next_tok, next_hg, next_sees;
-  int tok, hg;
+  int tok, hg;  // ~hg: the row sees no token
 
   // Q fragments of rows mi * 16 + g and + 8 of the cursor's unit, and the tokens they see
   MOE_DEV void fetch_q(const KaCursor& x) {
@@ -818,7 +820,7 @@ struct KaFew {
       for (int e = 0; e < 4; ++e) q[k][e] = next_q[k][e];
     const int seen[2] = {next_seen[0], next_seen[1]};
     tok = next_tok;
-    hg = next_hg;
+    hg = next_sees > 0 ? next_hg : ~next_hg;
     float o[HD / 8][4];
 #pragma unroll
     for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
@@ -945,7 +947,7 @@ struct KaFew {
       float sum = l[r];
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      if (t == 0) s_ml[warp * 16 + g + 8 * r] = make_float2(sum > 0.f ? m[r] - shift : -INFINITY, sum);
+      if (t == 0) s_ml[warp * 16 + g + 8 * r] = make_float2(m[r] - shift, sum);  // no token: -inf, 0
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&joined[1]);
@@ -968,15 +970,16 @@ struct KaFew {
       float acc[V] = {}, sum = 0.f;
 #pragma unroll
       for (int i = 0; i < kSlices; ++i) {
-        const float f = ml[i].y > 0.f ? exp2_ftz(ml[i].x - top) : 0.f;
+        const float f = ml[i].y == 0.f ? 0.f : exp2_ftz(ml[i].x - top);  // a sum of NaN stays
         const float* src = part + ((first + i) * 16 + r) * HD + (((lane * V / 2) ^ ((r & 7) << 2)) << 1);
         sum += f * ml[i].y;
 #pragma unroll
         for (int e = 0; e < V; ++e) acc[e] = fmaf(f, src[e], acc[e]);
       }
       if (direct) {
-        write_row<HD, BF16>(a, __shfl_sync(0xffffffffu, tok, pr), head * group + __shfl_sync(0xffffffffu, hg, pr),
-                            acc, top, sum);
+        const int h = __shfl_sync(0xffffffffu, hg, pr);
+        write_row<HD, BF16>(a, __shfl_sync(0xffffffffu, tok, pr), head * group + (h < 0 ? ~h : h), acc, top, sum,
+                            h >= 0);
       } else {
         const long long slot = piece_slot(kFew, share, !cut_front, pr);
         float* dst = w.few.o + slot * HD + lane * V;
@@ -1400,8 +1403,8 @@ __global__ void __launch_bounds__(kAttThreads, 1)
           if (whole && !cut_front) {
             const long long row = static_cast<long long>(u.row0) + tok;
             const int h = head * group + hg;
-            const bool saw = m != -INFINITY;  // else the row sees no token
-            const float inv = saw ? 1.f / l : 0.f;
+            const bool saw = seen > 0;  // as in write_row
+            const float inv = 1.f / l;
             // a thread writes its own row: its 32 lanes meet 32 lines in every store, so
             // the stores are as wide as they can be
             __half* dst = out16 + row * a.os[0] + h * a.os[1];
@@ -1447,7 +1450,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
                 }
               }
             }
-            if (valid) l_k.ml[slot] = m == -INFINITY ? make_float2(-INFINITY, 0.f) : make_float2(m - shift, l);
+            if (valid) l_k.ml[slot] = make_float2(m - shift, l);  // no token: -inf, 0
           }
         }
         tc_fence_before();  // O is read: the next unit's first product may overwrite it
@@ -1501,6 +1504,7 @@ __global__ void __launch_bounds__(256) kv_merge_kernel(const KvAttend a, const K
     const int kind = e.x, first = e.y, last = e.z;
     const KaList l = w.kind(kind);
     const int4 u0 = *reinterpret_cast<const int4*>(l.list + item);  // seq, row0, r0, rows
+    const int2 u1 = *reinterpret_cast<const int2*>(&l.list[item].base);  // base, len
     float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, acc[2][V] = {};
     for (int base = first; base <= last; base += 32) {
       // shares of the unit that have tiles
@@ -1536,14 +1540,16 @@ __global__ void __launch_bounds__(256) kv_merge_kernel(const KvAttend a, const K
           if (!on[q]) break;
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
+            // a piece without a visible token (sum 0) holds nothing, whatever its rows say; a
+            // sum of NaN counts, with or without a maximum
+            const bool some = ml[q][j].y != 0.f;
             const float up = fmaxf(top[j], ml[q][j].x);
             const float keep = top[j] == -INFINITY ? 0.f : exp2_ftz(top[j] - up);
-            const float f = ml[q][j].x == -INFINITY ? 0.f : exp2_ftz(ml[q][j].x - up);
+            const float f = some ? exp2_ftz(ml[q][j].x - up) : 0.f;
             top[j] = up;
-            // a piece without a visible token holds nothing, whatever its rows say
-            sum[j] = sum[j] * keep + (f > 0.f ? f * ml[q][j].y : 0.f);
+            sum[j] = sum[j] * keep + (some ? f * ml[q][j].y : 0.f);
 #pragma unroll
-            for (int x = 0; x < V; ++x) acc[j][x] = acc[j][x] * keep + (f > 0.f ? f * v[q][j][x] : 0.f);
+            for (int x = 0; x < V; ++x) acc[j][x] = acc[j][x] * keep + (some ? f * v[q][j][x] : 0.f);
           }
         }
       }
@@ -1553,7 +1559,7 @@ __global__ void __launch_bounds__(256) kv_merge_kernel(const KvAttend a, const K
       const int packed = u0.z + r0 + j, tok = packed / group;
       if (r0 + j < u0.w)
         write_row<HD, BF16>(a, static_cast<long long>(u0.y) + tok, e.w * group + packed - tok * group, acc[j], top[j],
-                            sum[j]);
+                            sum[j], min(u1.x + tok + 1, u1.y) > 0);
     }
   }
 }
