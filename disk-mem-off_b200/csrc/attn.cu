@@ -68,7 +68,7 @@ static size_t a256(size_t v) { return (v + 255) & ~size_t(255); }
 // Workspace of a forward over the paged cache: q and o rows by token, the place of each
 // token's keys and values, and the attention's own scratch.
 struct AttnCachedWs {
-  size_t rms, h16, qkv, rope, slot, q, o16, oplanes, attend, total;
+  size_t rms, h16, qkv, rope, slot, range, q, o16, oplanes, attend, total;
   int s1, s2;
 };
 
@@ -83,6 +83,7 @@ static AttnCachedWs attn_cached_ws(const AttnPlan& a, const MoeKvCache& c, int T
   w.qkv = take(static_cast<size_t>(w.s1) * T * a.nqkv * 4);
   w.rope = take(static_cast<size_t>(T) * (a.hd / 2) * 8);
   w.slot = take(static_cast<size_t>(T) * 8);
+  w.range = take(8);
   w.q = take(static_cast<size_t>(T) * a.nout * 2);
   w.o16 = take(static_cast<size_t>(T) * a.nout * 2);
   w.oplanes = take(static_cast<size_t>(w.s2) * T * a.H * 4);
@@ -289,14 +290,19 @@ __global__ void __launch_bounds__(256) attn_rope_kernel(float2* __restrict__ rop
 
 // The same for rows of the paged cache, at their own positions, and the place of each
 // row's keys and values.  A warp per row; rows that belong to no sequence (or whose page is
-// missing) get position 0 and no place.
+// missing) get position 0 and no place, and so do all rows of a batch that may not be
+// written.  range: the rows of the batch, first and end; none when its offsets are wrong.
 __global__ void __launch_bounds__(128) attn_place_kernel(const KvView c, const KvBatch b, float2* __restrict__ rope,
-                                                         int2* __restrict__ slot, int half, float theta) {
+                                                         int2* __restrict__ slot, int2* __restrict__ range, int half,
+                                                         float theta) {
   pdl_enter();
+  extern __shared__ uint32_t bits[];
+  const bool ok = batch_ok(c, b, bits);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *range = ok ? make_int2(b.q_start[0], b.q_start[b.n]) : make_int2(0, 0);
   const int lane = threadIdx.x & 31;
   const int r = blockIdx.x * 4 + (threadIdx.x >> 5);
   if (r >= b.rows) return;
-  const int e = r < b.q_start[b.n] ? entry_of_row(b.q_start, b.n, r) : -1;
+  const int e = ok && r < b.q_start[b.n] ? entry_of_row(b.q_start, b.n, r) : -1;
   int64_t pos = 0;
   int2 at = make_int2(-1, 0);
   if (e >= 0) {
@@ -708,13 +714,12 @@ __global__ void __launch_bounds__(kFaThreads, 1) attn_fwd_kernel(const __grid_co
 __global__ void __launch_bounds__(256) attn_out_kernel(const float* __restrict__ x,
                                                        const float* __restrict__ planes, int nsplit,
                                                        size_t n, float* __restrict__ out,
-                                                       const int* __restrict__ first,
-                                                       const int* __restrict__ end, int H) {
+                                                       const int2* __restrict__ range, int H) {
   pdl_enter();
-  // n is a multiple of 4 (H is a multiple of 64): float4 at a time, planes in order; with
-  // first and end only rows *first .. *end - 1
-  const size_t n4 = (end ? min(n, static_cast<size_t>(max(*end, 0)) * H) : n) / 4;
-  const size_t i0 = first ? static_cast<size_t>(max(*first, 0)) * H / 4 : 0;
+  // n is a multiple of 4 (H is a multiple of 64): float4 at a time, planes in order; with a
+  // range (first, end) its rows only
+  const size_t i0 = range ? static_cast<size_t>(range->x) * H / 4 : 0;
+  const size_t n4 = (range ? static_cast<size_t>(range->y) * H : n) / 4;
   for (size_t i = i0 + blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x; i < n4;
        i += static_cast<size_t>(gridDim.x) * blockDim.x) {
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -791,7 +796,7 @@ static cudaError_t attn_launch(const AttnPlan& a, const AttnWs& w, char* ws, con
   const size_t n = static_cast<size_t>(T) * a.H;
   const int grid = static_cast<int>(std::min<size_t>((n + 255) / 256, static_cast<size_t>(a.num_sms) * 8));
   MOE_PDL(attn_out_kernel, dim3(grid), dim3(256), 0, s, x, reinterpret_cast<const float*>(ws + w.oplanes),
-          w.s2, n, out, static_cast<const int*>(nullptr), static_cast<const int*>(nullptr), a.H);
+          w.s2, n, out, static_cast<const int2*>(nullptr), a.H);
   return cudaSuccess;
 }
 
@@ -805,8 +810,10 @@ static cudaError_t attn_cached_launch(const AttnPlan& a, const MoeKvCache& c, co
                                 reinterpret_cast<__half*>(ws + w.h16), a.d_err, s));
   MOE_CUDA_RET(launch_dense_gemm(a.tm_qkv, a.nqkv, a.H, reinterpret_cast<const __half*>(ws + w.h16), T,
                                  reinterpret_cast<float*>(ws + w.qkv), w.s1, a.d_err, a.num_sms, s));
-  MOE_PDL(attn_place_kernel, dim3((T + 3) / 4), dim3(128), 0, s, c.v, b, reinterpret_cast<float2*>(ws + w.rope),
-          reinterpret_cast<int2*>(ws + w.slot), a.rot / 2, a.cfg.rope_theta);
+  MOE_CUDA_RET(kv_launch_check(c.v, b, s));
+  MOE_PDL(attn_place_kernel, dim3((T + 3) / 4), dim3(128), bitmap_bytes(c.v), s, c.v, b,
+          reinterpret_cast<float2*>(ws + w.rope), reinterpret_cast<int2*>(ws + w.slot),
+          reinterpret_cast<int2*>(ws + w.range), a.rot / 2, a.cfg.rope_theta);
   const int groups = (a.nh + 2 * a.nkv + 7) / 8;
   const int gy = std::max(1, std::min(groups, (8 * a.num_sms + T - 1) / T));
   MOE_PDL((attn_qkv_kernel<HD, true>), dim3(T, gy), dim3(256), 0, s, reinterpret_cast<const float*>(ws + w.qkv), w.s1,
@@ -828,7 +835,7 @@ static cudaError_t attn_cached_launch(const AttnPlan& a, const MoeKvCache& c, co
   const size_t n = static_cast<size_t>(T) * a.H;
   const int grid = static_cast<int>(std::min<size_t>((n + 255) / 256, static_cast<size_t>(a.num_sms) * 8));
   MOE_PDL(attn_out_kernel, dim3(grid), dim3(256), 0, s, x, reinterpret_cast<const float*>(ws + w.oplanes), w.s2, n,
-          out, b.q_start, b.q_start + b.n, a.H);
+          out, reinterpret_cast<const int2*>(ws + w.range), a.H);
   return cudaSuccess;
 }
 

@@ -25,6 +25,7 @@ struct KvView {
   // scratch (see KvScratch)
   int* err;
   int* count;  // pages to copy, written by the kernel that plans a copy
+  int* ok;     // a batch may be written (kv_check_kernel)
   int* src;    // [cap] pages to copy from
   int* dst;    // [cap] pages to copy to
   int* rows;   // [cap] rows of each page to copy
@@ -32,8 +33,8 @@ struct KvView {
   int* off;    // [nseq] first free page of each entry
 };
 
-// The caller's scratch, zeroed once: 16 words (error word, copy count), then the
-// arrays above.
+// The caller's scratch, zeroed once: 16 words (error word, copy count, batch check), then
+// the arrays above.
 inline size_t kv_scratch_words(int pages, int nseq) {
   const size_t cap = static_cast<size_t>(pages > nseq ? pages : nseq);
   return 16 + 3 * cap + static_cast<size_t>(pages) + nseq;
@@ -53,7 +54,53 @@ struct KvBatch {
   int rows;  // rows of the tensors; those from q_start[n] on are left alone
 };
 
+inline size_t bitmap_bytes(const KvView& v) { return static_cast<size_t>((v.nseq + 31) / 32) * 4; }
+
 #ifdef __CUDACC__
+// Whether rows may be written for a batch, for every thread of the CTA: offsets that begin
+// at 0 or later, do not decrease and end within the rows, and no sequence with rows in two
+// entries (both would write its last places).  What is wrong is recorded.  bits:
+// bitmap_bytes of shared memory; U: entries of a thread at a time, for loads in flight.
+template <int U>
+MOE_DEV bool check_batch(const KvView& c, const KvBatch& b, uint32_t* bits) {
+  for (int i = threadIdx.x; i < (c.nseq + 31) / 32; i += blockDim.x) bits[i] = 0;
+  __syncthreads();
+  bool bad = false;
+  for (int i0 = threadIdx.x; i0 < b.n; i0 += U * blockDim.x) {
+    int at[U], end[U], s[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * blockDim.x;
+      at[u] = end[u] = s[u] = 0;
+      if (i < b.n) {
+        at[u] = b.q_start[i];
+        end[u] = b.q_start[i + 1];
+        s[u] = b.seqs[i];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (at[u] < 0 || end[u] < at[u] || end[u] > b.rows) {
+        record_error(c.err, DEV_BAD_LENGTH);
+        bad = true;
+      } else if (end[u] > at[u] && s[u] >= 0 && s[u] < c.nseq &&
+                 (atomicOr(&bits[s[u] >> 5], 1u << (s[u] & 31)) >> (s[u] & 31) & 1u)) {
+        record_error(c.err, DEV_BAD_SEQ);
+        bad = true;
+      }
+    }
+  }
+  return !__syncthreads_or(bad);
+}
+// Every CTA of a writing kernel knows before it writes: up to kCheckHere entries it checks
+// the batch itself, of more kv_check_kernel has left the answer in *c.ok.  Append of n rows
+// of n sequences, without a check / checked in each CTA / by the kernel: 64: 2.7 / 3.0 us,
+// 512: 3.1 / 4.2, 1,024: 4.0 / 7.4 / 6.5, 4,096: 5.6 / 24.7 / 9.8, 16,384: 19 / 170 / 30.
+constexpr int kCheckHere = 512;
+MOE_DEV bool batch_ok(const KvView& c, const KvBatch& b, uint32_t* bits) {
+  return b.n <= kCheckHere ? check_batch<1>(c, b, bits) : *c.ok != 0;
+}
+
 // The entry of row r: the last e with q_start[e] <= r, -1 before the first (n > 0), by a
 // warp (32 probes a round, one round at least: a single entry may begin after row r too).
 MOE_DEV int entry_of_row(const int* __restrict__ q_start, int n, int r) {
@@ -73,6 +120,8 @@ MOE_DEV int entry_of_row(const int* __restrict__ q_start, int n, int r) {
 }
 #endif
 
+// Before a kernel that calls batch_ok.
+cudaError_t kv_launch_check(const KvView& c, const KvBatch& b, cudaStream_t s);
 cudaError_t kv_launch_append(const KvView& c, const KvBatch& b, int layer, const void* k,
                              const void* v, const int64_t (&ks)[2], const int64_t (&vs)[2],
                              int num_sms, cudaStream_t s);

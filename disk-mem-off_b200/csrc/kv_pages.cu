@@ -450,16 +450,18 @@ __global__ void __launch_bounds__(256) kv_compact_tables_kernel(const KvView c, 
 // ------------------------------------------------------------------ append
 // A warp per row: all heads of the row's key, then of its value, 16 bytes a lane.
 // Bound by HBM for long chunks (each byte read and written once; 10,168 rows of 8 heads, 83
-// MB: 16.3 us, 5.1 TB/s), by the launch and three dependent loads (entry, length, page) for
-// a decode step (2.8 us).
-__global__ void __launch_bounds__(128) kv_append_kernel(const KvView c, const KvBatch b, int layer,
+// MB: 16.6 us, 5.0 TB/s), by the launch and three dependent loads (entry, length, page) for
+// a decode step (64 rows: 3.0 us, 0.3 of them the check of the batch).
+__global__ void __launch_bounds__(128, 8) kv_append_kernel(const KvView c, const KvBatch b, int layer,
                                                         const char* __restrict__ k,
                                                         const char* __restrict__ v, int64_t kt,
                                                         int64_t kh, int64_t vt, int64_t vh) {
   pdl_enter();
+  extern __shared__ uint32_t bits[];
+  if (!batch_ok(c, b, bits)) return;
   const int lane = threadIdx.x & 31;
   const int warps = gridDim.x * (blockDim.x >> 5);
-  const int total = min(b.q_start[b.n], b.rows);
+  const int total = b.q_start[b.n];
   const int shift = c.hd == 128 ? 4 : 3;  // chunks of a head
   const int nc = c.heads << shift;
   for (int r = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); r < total; r += warps) {
@@ -504,11 +506,25 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const KvView c, const Kv
   }
 }
 
+// One CTA: the check of a batch of more than kCheckHere entries.
+__global__ void __launch_bounds__(kPlanThreads) kv_check_kernel(const KvView c, const KvBatch b) {
+  pdl_enter();
+  extern __shared__ uint32_t bits[];
+  const bool ok = check_batch<4>(c, b, bits);
+  if (threadIdx.x == 0) *c.ok = ok;
+}
+cudaError_t kv_launch_check(const KvView& c, const KvBatch& b, cudaStream_t s) {
+  if (b.n <= kCheckHere) return cudaSuccess;
+  return pdl_launch(kv_check_kernel, dim3(1), dim3(kPlanThreads), bitmap_bytes(c), s, c, b);
+}
+
 cudaError_t kv_launch_append(const KvView& c, const KvBatch& b, int layer, const void* k,
                              const void* v, const int64_t (&ks)[2], const int64_t (&vs)[2],
                              int num_sms, cudaStream_t s) {
   const int grid = std::min((b.rows + 3) / 4, num_sms * 16);
-  return pdl_launch(kv_append_kernel, dim3(grid), dim3(128), 0, s, c, b, layer,
+  const cudaError_t st = kv_launch_check(c, b, s);
+  if (st != cudaSuccess) return st;
+  return pdl_launch(kv_append_kernel, dim3(grid), dim3(128), bitmap_bytes(c), s, c, b, layer,
                     static_cast<const char*>(k), static_cast<const char*>(v), ks[0] * 2, ks[1] * 2,
                     vs[0] * 2, vs[1] * 2);
 }
@@ -555,8 +571,6 @@ struct DeviceScope {
     if (st_ != cudaSuccess)                                                            \
       return kfail(MOE_ERR_CUDA, std::string(#call) + ": " + cudaGetErrorString(st_)); \
   } while (0)
-
-size_t bitmap_bytes(const KvView& v) { return static_cast<size_t>((v.nseq + 31) / 32) * 4; }
 
 // enough CTAs to fill the GPU for any number of pages (the count is on the device)
 dim3 copy_grid(const MoeKvCache* c) { return dim3(c->num_sms * 8); }
@@ -629,6 +643,7 @@ int moe_kv_create(const MoeKvConfig* cfg, MoeKvCache** out) {
   const size_t cap = std::max(c.pages, c.sequences);
   v.err = w;
   v.count = w + 1;
+  v.ok = w + 2;
   v.src = w + 16;
   v.dst = v.src + cap;
   v.rows = v.dst + cap;

@@ -228,7 +228,8 @@ class PagedKVCache:
     def append(self, k: Any, v: Any, seqs: Any, starts: Any, layer: int = 0,
                stream: Any = None) -> None:
         """Write the batch's keys and values ``[rows, kv_heads, head_dim]`` to the last
-        places of their sequences (after ``reserve``)."""
+        places of their sequences (after ``reserve``).  A batch with wrong ``starts``, or with
+        rows of one sequence in two entries, writes nothing (see ``status``)."""
         if stream is not None:
             return self._on(stream, self.append, k, v, seqs, starts, layer)
         seqs, starts, n = self._batch(seqs, starts)

@@ -366,9 +366,12 @@ int moe_attn_status(MoeAttn* attn, void* stream);
  * allocates nothing on the device.  An empty cache is all -1, 0 and 0.
  *
  * Index arguments (seqs, counts, q_start, ...) are int32 arrays in device memory, so
- * that calls can be captured in a graph.  A call on sequences outside [0, sequences),
- * or on the same sequence twice where that would be written twice, changes nothing;
- * such errors are found on the device and reported by moe_kv_status.  Calls on one
+ * that calls can be captured in a graph; errors in them are found on the device and
+ * reported by moe_kv_status.  A call on pages (reserve, fork, truncate) with a sequence
+ * outside [0, sequences) or the same sequence twice, or a batch of rows (append, the
+ * attention block) with a sequence that has rows in two entries or with offsets that
+ * decrease or leave the rows, writes nothing.  An entry of a batch whose sequence is
+ * outside is left out, the others are done.  Calls on one
  * cache run in stream order: the ones that change it (and attention while it is being
  * changed) must not overlap on two streams; attention calls may overlap each other. */
 enum { MOE_KV_F16 = 0, MOE_KV_BF16 = 1 };
@@ -423,7 +426,8 @@ int moe_kv_compact(MoeKvCache* cache, MoeKvCache* into, void* stream);
  * non-decreasing offsets), the last tokens of sequence seqs[i]: row r is its token
  * lengths[seqs[i]] - (q_start[i+1] - r).  Reserve first.  k, v: [rows][kv_heads][head_dim] in
  * the cache's dtype, token and head strides in elements (multiples of 8).  Rows before
- * q_start[0] and from q_start[n_seqs] on are ignored.  The same sequence twice: the rows of one entry win. */
+ * q_start[0] and from q_start[n_seqs] on are ignored, and so are rows without a place (more
+ * rows than the sequence has tokens, a page missing from its table), which are reported. */
 int moe_kv_append(MoeKvCache* cache, int32_t layer, const void* k, const void* v, int64_t k_token,
                   int64_t k_head, int64_t v_token, int64_t v_head, const int32_t* seqs,
                   const int32_t* q_start, int32_t n_seqs, int32_t rows, void* stream);
@@ -431,7 +435,8 @@ int moe_kv_append(MoeKvCache* cache, int32_t layer, const void* k, const void* v
  * to its own position; fp32 softmax and accumulation, probabilities rounded to the cache's
  * dtype for the product with v.  lse (may be NULL): natural logarithm of the sum of the
  * exponentials.  A row that sees no token (more new rows than tokens) gives 0 and -inf.
- * Rows of out and lse before q_start[0] and from q_start[n_seqs] on are left as they were.  Nothing that the pool
+ * Rows of out and lse before q_start[0] and from q_start[n_seqs] on are left as they were, and
+ * those of an entry whose offsets are wrong; the same sequence may come twice.  Nothing that the pool
  * holds past a sequence's length reaches a result, NaN and infinities included; among a
  * sequence's own values they reach every row of the same chunk (weight 0 times infinity). */
 typedef struct MoeKvAttendArgs {
@@ -462,7 +467,7 @@ int moe_kv_status(MoeKvCache* cache, void* stream);
  * rows' keys and values are written to layer `layer` of the cache, whose older tokens they
  * attend to.  Reserve first (once for all layers); seqs, q_start, n_seqs as moe_kv_append;
  * the cache is f16 with the plan's kv_heads and head_dim.  Rows of out before q_start[0] and
- * from q_start[n_seqs] on are left as they were.  Errors of the sequences are reported by moe_kv_status. */
+ * from q_start[n_seqs] on are left as they were; all of them when the offsets are wrong.  Errors of the sequences are reported by moe_kv_status. */
 uint64_t moe_attn_cached_workspace_bytes(const MoeAttn* attn, const MoeKvCache* cache, int32_t T,
                                          int32_t n_seqs);
 int moe_attn_forward_cached(MoeAttn* attn, MoeKvCache* cache, int32_t layer, const float* x_dev,

@@ -89,3 +89,107 @@ def test_the_block_leaves_rows_before_the_first_entry_alone(seqs: list, starts: 
         got = out[rows].cpu().numpy()
         assert _rel(got, ref) <= TOL_BLOCK and _rel(got - batch[rows], ref - batch[rows]) <= TOL_DELTA
     al.close()
+
+
+# ------------------------------------------------------------------ batches that are refused
+def _bits(cache) -> tuple:
+    return tuple(t.clone().view(torch.int16) for t in (cache.k, cache.v))
+
+
+def _status_raises_once(cache) -> None:
+    with pytest.raises(ValueError):
+        cache.status()
+    cache.status()
+
+
+BAD_BATCHES = [
+    ([0], [0, 9]),                # ends past the rows
+    ([0, 1], [0, 2, 9]),
+    ([0, 1], [0, 3, 2]),          # decreases
+    ([0, 1, 2], [0, 5, 3, 8]),
+    ([0, 1], [-3, 2, 4]),
+    ([0], [2147483647, -2147483648]),
+    ([0, 0], [0, 2, 4]),          # the same sequence with rows in two entries
+    ([2, 1, 0, 1], [0, 1, 2, 3, 4]),
+]
+
+
+@pytest.mark.parametrize("seqs,starts", BAD_BATCHES)
+def test_append_refuses_a_bad_batch_as_a_whole(seqs: list, starts: list) -> None:
+    cache, _o = _filled("bf16", 16, 2, 64, [20, 33, 12], seed=4)
+    k, v = (torch.randn((8, 2, 64), device="cuda").bfloat16() for _ in range(2))
+    before = _bits(cache)
+    cache.append(k, v, seqs, starts)
+    _status_raises_once(cache)
+    assert all(torch.equal(a, b) for a, b in zip(before, _bits(cache)))
+
+
+def test_append_refuses_among_many_entries() -> None:
+    """More entries than a CTA has threads and more sequences than a warp's bits; the last
+    one is wrong, then none is."""
+    n = 700
+    cache, o = _filled("f16", 16, 1, 64, [3] * n, seed=5, nan=False)
+    k, v = (torch.randn((n, 1, 64), device="cuda").half() for _ in range(2))
+    seqs = np.random.default_rng(1).permutation(n).tolist()
+    before = _bits(cache)
+    for bad_seqs, bad_starts in ((seqs[:-1] + [seqs[3]], list(range(n + 1))),
+                                 (seqs, list(range(n)) + [n + 1])):
+        cache.append(k, v, bad_seqs, bad_starts)
+        _status_raises_once(cache)
+        assert all(torch.equal(a, b) for a, b in zip(before, _bits(cache)))
+    cache.append(k, v, seqs, list(range(n + 1)))
+    cache.status()
+    o.append(0, k.double().cpu().numpy(), v.double().cpu().numpy(), seqs, list(range(n + 1)))
+    np.testing.assert_array_equal(cache.k.double().cpu().numpy(), o.k)
+    np.testing.assert_array_equal(cache.v.double().cpu().numpy(), o.v)
+
+
+def test_append_of_entries_without_rows() -> None:
+    """Padding entries: no rows, any sequence, the same one as often as wanted."""
+    cache, o = _filled("f16", 16, 2, 64, [20, 33, 12], seed=4, nan=False)
+    k, v = (torch.randn((8, 2, 64), device="cuda").half() for _ in range(2))
+    cache.append(k, v, [0, 0, 1, -1, 0, 99, 0], [0, 0, 0, 2, 2, 4, 4, 4])
+    cache.status()
+    o.append(0, k.double().cpu().numpy(), v.double().cpu().numpy(), [1, 0], [0, 2, 4])
+    np.testing.assert_array_equal(cache.k.double().cpu().numpy(), o.k)
+    np.testing.assert_array_equal(cache.v.double().cpu().numpy(), o.v)
+
+
+def test_append_leaves_out_what_has_no_place() -> None:
+    """A sequence that does not exist, more rows than tokens: the other rows are written."""
+    cache, o = _filled("f16", 16, 2, 64, [20, 3, 12], seed=4, nan=False)
+    k, v = (torch.randn((9, 2, 64), device="cuda").half() for _ in range(2))
+    kk, vv = k.double().cpu().numpy(), v.double().cpu().numpy()
+    cache.append(k, v, [0, 99, 2], [0, 2, 5, 6])
+    _status_raises_once(cache)
+    o.append(0, kk[[0, 1, 5]], vv[[0, 1, 5]], [0, 2], [0, 2, 3])
+    cache.append(k, v, [1], [0, 5])
+    _status_raises_once(cache)
+    o.append(0, kk[2:5], vv[2:5], [1], [0, 3])
+    np.testing.assert_array_equal(cache.k.double().cpu().numpy(), o.k)
+    np.testing.assert_array_equal(cache.v.double().cpu().numpy(), o.v)
+
+
+def test_the_block_refuses_a_bad_batch_as_a_whole() -> None:
+    spec = AttnSpec(hidden=512, heads=16, kv_heads=2, head_dim=128, tokens=40, seed=72)
+    x, t = make_attn_case(spec)
+    al = _layer(spec, t, 64)
+    cache = _cache(spec, 3, 3, 16)
+    for s, n in enumerate((20, 33, 12)):
+        cache.reserve([s], [n])
+        al.forward_cached(torch.from_numpy(x[:n]).cuda(), cache, [s], [0, n])
+    before = _bits(cache)
+    batch = torch.randn((8, spec.hidden), device="cuda")
+    for seqs, starts in BAD_BATCHES:
+        out = torch.full_like(batch, 3.0)
+        al.forward_cached(batch, cache, seqs, starts, out=out)
+        _status_raises_once(cache)
+        assert all(torch.equal(a, b) for a, b in zip(before, _bits(cache)))
+        assert (out == 3).all()
+    al.status()
+    out = al.forward_cached(batch, cache, [0, 99, 2], [0, 2, 5, 8])  # one entry has no sequence
+    _status_raises_once(cache)
+    assert torch.equal(out[2:5], batch[2:5])
+    good = al.forward_cached(batch, cache, [0, 2], [0, 2, 5])[:2]
+    assert _rel(out[:2].cpu().numpy(), good.double().cpu().numpy()) <= TOL_BLOCK
+    al.close()
