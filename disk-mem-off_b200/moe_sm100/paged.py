@@ -18,6 +18,10 @@ offsets of their rows in ``q`` / ``k`` / ``v``: sequence ``seqs[i]`` brings rows
 (or lists, copied to the device), so a step can be captured in a CUDA graph; errors
 in their values are found on the device and raised by ``status()``.  Every call takes
 ``stream=`` (default: the current stream of the cache's device).
+
+Calls on one cache are to run in order (attention calls may overlap each other).  A new
+handle may be used on any stream, and may be dropped while torch's streams still work on
+it; work on a stream given by its handle, and graphs, have to be over by then.
 """
 from __future__ import annotations
 
@@ -94,6 +98,11 @@ class PagedKVCache:
                                     dtype=torch.int32, device=k.device)
         cfg.scratch = self._scratch.data_ptr()
         check(lib().moe_kv_create(byref(cfg), byref(self._h)))
+        self._used_on: set[int] = set()  # streams that the tensors are recorded on
+        # the scratch is zero before another stream uses it
+        with torch.cuda.device(self.device):
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream().synchronize()
 
     @classmethod
     def allocate(cls, *, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int,
@@ -169,7 +178,21 @@ class PagedKVCache:
         return rows, heads, token if rows > 1 else 0, head if heads > 1 else 0
 
     def _stream(self) -> int:
-        return self._raw_stream(self._dev)
+        """The current stream's handle, for a call that is about to use it."""
+        raw = self._raw_stream(self._dev)
+        if raw not in self._used_on:
+            self._first_use(raw)
+        return raw
+
+    def _first_use(self, raw: int) -> None:
+        """Tell torch's allocator, so that memory let go with the cache waits for the stream.
+        Not of streams made elsewhere: those may be gone by then, and the allocator would
+        still ask them (and their handles may come again)."""
+        stream = _torch().cuda.current_stream(self.device)
+        if stream.stream_id == 0 or stream.stream_id & 1:  # torch's own are odd, or the default
+            for t in (self.k, self.v, self.block_table, self.lengths, self.refs, self._scratch):
+                t.record_stream(stream)
+            self._used_on.add(raw)
 
     def _on(self, stream: Any, method: Any, *args: Any) -> Any:
         """The call as if ``stream`` were current, so that the buffers it allocates belong
@@ -186,7 +209,7 @@ class PagedKVCache:
         if stream is not None:
             return self._on(stream, self.reserve, seqs, counts)
         x, y, n, _keep = self._indices("seqs", seqs, "counts", counts)
-        check(self._lib.moe_kv_reserve(self._h, x, y, n, self._raw_stream(self._dev)))
+        check(self._lib.moe_kv_reserve(self._h, x, y, n, self._stream()))
 
     def fork(self, parents: Any, children: Any, stream: Any = None) -> None:
         """Make the empty sequence ``children[i]`` a copy of ``parents[i]`` that shares
@@ -194,14 +217,14 @@ class PagedKVCache:
         if stream is not None:
             return self._on(stream, self.fork, parents, children)
         x, y, n, _keep = self._indices("parents", parents, "children", children)
-        check(self._lib.moe_kv_fork(self._h, x, y, n, self._raw_stream(self._dev)))
+        check(self._lib.moe_kv_fork(self._h, x, y, n, self._stream()))
 
     def truncate(self, seqs: Any, lengths: Any, stream: Any = None) -> None:
         """Shorten ``seqs[i]`` to ``lengths[i]`` tokens and let its other pages go."""
         if stream is not None:
             return self._on(stream, self.truncate, seqs, lengths)
         x, y, n, _keep = self._indices("seqs", seqs, "lengths", lengths)
-        check(self._lib.moe_kv_truncate(self._h, x, y, n, self._raw_stream(self._dev)))
+        check(self._lib.moe_kv_truncate(self._h, x, y, n, self._stream()))
 
     def free(self, seqs: Any, stream: Any = None) -> None:
         """Empty the sequences: ``truncate`` to no tokens."""
@@ -215,13 +238,15 @@ class PagedKVCache:
         if stream is not None:
             return self._on(stream, self.copy_pages, src, dst)
         x, y, n, _keep = self._indices("src", src, "dst", dst)
-        check(self._lib.moe_kv_copy_pages(self._h, x, y, n, self._raw_stream(self._dev)))
+        check(self._lib.moe_kv_copy_pages(self._h, x, y, n, self._stream()))
 
     def compact(self, into: "PagedKVCache | None" = None, stream: Any = None) -> None:
         """Move the live pages to the lowest numbers, or, dense and in order, ``into``
         another cache (whose sequences are overwritten): how a pool changes its size."""
         if stream is not None:
             return self._on(stream, self.compact, into)
+        if into is not None:
+            into._stream()  # its tensors are used too
         check(self._lib.moe_kv_compact(self._h, None if into is None else into._h, self._stream()))
 
     # -- tokens -------------------------------------------------------------------
