@@ -806,14 +806,15 @@ template <int HD>
 static cudaError_t attn_cached_launch(const AttnPlan& a, const MoeKvCache& c, const AttnCachedWs& w, char* ws,
                                       const float* x, float* out, int layer, const KvBatch& b, cudaStream_t s) {
   const int T = b.rows;
-  MOE_CUDA_RET(launch_norm_rows(x, a.win, a.H, a.cfg.rms_norm_eps, T, reinterpret_cast<float*>(ws + w.rms),
-                                reinterpret_cast<__half*>(ws + w.h16), a.d_err, s));
-  MOE_CUDA_RET(launch_dense_gemm(a.tm_qkv, a.nqkv, a.H, reinterpret_cast<const __half*>(ws + w.h16), T,
-                                 reinterpret_cast<float*>(ws + w.qkv), w.s1, a.d_err, a.num_sms, s));
+  int2* range = reinterpret_cast<int2*>(ws + w.range);
   MOE_CUDA_RET(kv_launch_check(c.v, b, s));
   MOE_PDL(attn_place_kernel, dim3((T + 3) / 4), dim3(128), bitmap_bytes(c.v), s, c.v, b,
-          reinterpret_cast<float2*>(ws + w.rope), reinterpret_cast<int2*>(ws + w.slot),
-          reinterpret_cast<int2*>(ws + w.range), a.rot / 2, a.cfg.rope_theta);
+          reinterpret_cast<float2*>(ws + w.rope), reinterpret_cast<int2*>(ws + w.slot), range, a.rot / 2,
+          a.cfg.rope_theta);
+  MOE_CUDA_RET(launch_norm_rows(x, a.win, a.H, a.cfg.rms_norm_eps, T, reinterpret_cast<float*>(ws + w.rms),
+                                reinterpret_cast<__half*>(ws + w.h16), a.d_err, s, range));
+  MOE_CUDA_RET(launch_dense_gemm(a.tm_qkv, a.nqkv, a.H, reinterpret_cast<const __half*>(ws + w.h16), T,
+                                 reinterpret_cast<float*>(ws + w.qkv), w.s1, a.d_err, a.num_sms, s));
   const int groups = (a.nh + 2 * a.nkv + 7) / 8;
   const int gy = std::max(1, std::min(groups, (8 * a.num_sms + T - 1) / T));
   MOE_PDL((attn_qkv_kernel<HD, true>), dim3(T, gy), dim3(256), 0, s, reinterpret_cast<const float*>(ws + w.qkv), w.s1,
@@ -835,7 +836,7 @@ static cudaError_t attn_cached_launch(const AttnPlan& a, const MoeKvCache& c, co
   const size_t n = static_cast<size_t>(T) * a.H;
   const int grid = static_cast<int>(std::min<size_t>((n + 255) / 256, static_cast<size_t>(a.num_sms) * 8));
   MOE_PDL(attn_out_kernel, dim3(grid), dim3(256), 0, s, x, reinterpret_cast<const float*>(ws + w.oplanes), w.s2, n,
-          out, reinterpret_cast<const int2*>(ws + w.range), a.H);
+          out, static_cast<const int2*>(range), a.H);
   return cudaSuccess;
 }
 

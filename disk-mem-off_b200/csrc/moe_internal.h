@@ -248,9 +248,10 @@ int router_tc_splits(const Plan& p, int T);
 int dense_gemm_splits(int m_rows, int T, int K, int num_sms);
 cudaError_t launch_dense_gemm(const CUtensorMap& a_map, int m_rows, int K, const __half* b, int T,
                               float* planes, int splits, int* err, int num_sms, cudaStream_t s);
-// rms[t] = sqrt(mean(x_t^2) + eps), h16[t] = f16(w * (x_t / rms[t])) for T rows.
+// rms[t] = sqrt(mean(x_t^2) + eps), h16[t] = f16(w * (x_t / rms[t])) for T rows; with a
+// range (first, end; in device memory) zeros for the rows outside it.
 cudaError_t launch_norm_rows(const float* x, const float* w, int H, float eps, int T, float* rms,
-                             __half* h16, int* err, cudaStream_t s);
+                             __half* h16, int* err, cudaStream_t s, const int2* range = nullptr);
 // Token rows are read as float4 vectors and by bulk copies.
 inline bool misaligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) != 0; }
 cudaError_t launch_scale_router_weights(const float* w, __half* rw16, int rows, int H, int* err,

@@ -1167,13 +1167,21 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const __half* __restri
 // ------------------------------------------------------------------ prefill router operands
 // Prefill routing prologue, one CTA per token: rms = sqrt(mean(x^2) + eps) and
 // h16 = f16(w * (x / rms)), the B operand of the router GEMM and the rows that
-// dispatch gathers for the experts.
+// dispatch gathers for the experts.  With a range (first, end) the rows outside it are not
+// read, give zeros and cannot overflow.
 __global__ void __launch_bounds__(256) router_prep_kernel(const float* __restrict__ x,
                                                           const float* __restrict__ wn, int H,
                                                           float eps, float* __restrict__ rms_out,
-                                                          __half* __restrict__ h16, int* err) {
+                                                          __half* __restrict__ h16, int* err,
+                                                          const int2* __restrict__ range) {
   pdl_enter();
   const int t = blockIdx.x;
+  if (range && (t < range->x || t >= range->y)) {
+    uint2* zero = reinterpret_cast<uint2*>(h16 + static_cast<size_t>(t) * H);
+    for (int i = threadIdx.x; i < H >> 2; i += blockDim.x) zero[i] = make_uint2(0, 0);
+    if (threadIdx.x == 0) rms_out[t] = 0.f;
+    return;
+  }
   const float4* xr = reinterpret_cast<const float4*>(x + static_cast<size_t>(t) * H);
   const float4* wr = reinterpret_cast<const float4*>(wn);
   const int nv = H >> 2;
@@ -1233,14 +1241,15 @@ __global__ void __launch_bounds__(256) scale_router_kernel(const float* __restri
 cudaError_t launch_row_prep(const Plan& p, const WsLayout& L, char* ws, const float* x, int T,
                             cudaStream_t s) {
   MOE_PDL(router_prep_kernel, dim3(T), dim3(256), 0, s, x, p.w.norm_w, p.H, p.cfg.rms_norm_eps,
-          reinterpret_cast<float*>(ws + L.rms), reinterpret_cast<__half*>(ws + L.h16), p.d_err);
+          reinterpret_cast<float*>(ws + L.rms), reinterpret_cast<__half*>(ws + L.h16), p.d_err,
+          static_cast<const int2*>(nullptr));
   return cudaSuccess;
 }
 
 cudaError_t launch_norm_rows(const float* x, const float* w, int H, float eps, int T, float* rms,
-                             __half* h16, int* err, cudaStream_t s) {
+                             __half* h16, int* err, cudaStream_t s, const int2* range) {
   if (T <= 0) return cudaSuccess;
-  MOE_PDL(router_prep_kernel, dim3(T), dim3(256), 0, s, x, w, H, eps, rms, h16, err);
+  MOE_PDL(router_prep_kernel, dim3(T), dim3(256), 0, s, x, w, H, eps, rms, h16, err, range);
   return cudaSuccess;
 }
 
@@ -1532,7 +1541,8 @@ cudaError_t launch_route(const Plan& p, const WsLayout& L, char* ws, const float
   if (tc) {
     MOE_PDL(router_prep_kernel, dim3(T), dim3(256), 0, s, x, p.w.norm_w, p.H, p.cfg.rms_norm_eps,
                                          reinterpret_cast<float*>(ws + L.rms),
-                                         reinterpret_cast<__half*>(ws + L.h16), p.d_err);
+                                         reinterpret_cast<__half*>(ws + L.h16), p.d_err,
+                                         static_cast<const int2*>(nullptr));
     st = cudaGetLastError();
     if (st != cudaSuccess) return st;
     st = launch_router_gemm(p, L, ws, T, s);
