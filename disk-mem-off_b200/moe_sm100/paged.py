@@ -246,6 +246,8 @@ class PagedKVCache:
         if stream is not None:
             return self._on(stream, self.compact, into)
         if into is not None:
+            if not into._h.value:  # null would mean: in place
+                raise ValueError("into is closed")
             into._stream()  # its tensors are used too
         check(self._lib.moe_kv_compact(self._h, None if into is None else into._h, self._stream()))
 
