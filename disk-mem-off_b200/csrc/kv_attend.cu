@@ -264,6 +264,7 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
   // (1)
   int n_pair = 0, n_single = 0, n_few = 0;
   long long work_pair = 0, work_single = 0, work_few = 0;  // of one kv head
+  bool bad = false;
   long long* pre_pair = cap0 <= kPlanSmem ? spre[0] : w.pair.pre;
   long long* pre_single = b.n <= kPlanSmem ? spre[1] : w.single.pre;
   long long* pre_few = b.n <= kPlanSmem ? spre[2] : w.few.pre;
@@ -276,6 +277,7 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
       const long long end = b.q_start[i + 1];
       if (row0 < 0 || end < row0 || end > b.rows) {
         record_error(c.err, DEV_BAD_LENGTH);
+        bad = true;
       } else {
         m = static_cast<int>(end) - row0;
       }
@@ -345,7 +347,11 @@ __global__ void __launch_bounds__(kPlanT) kv_plan_kernel(const KvView c, const K
     n_pair += pairs;
   }
   if (tid == 0) pre_pair[0] = pre_single[0] = pre_few[0] = 0;
-  __syncthreads();
+  // offsets that decrease can give a row to two entries: none is worked on then
+  if (__syncthreads_or(bad)) {
+    n_pair = n_single = n_few = 0;
+    work_pair = work_single = work_few = 0;
+  }
   // (2) a thread for each share of each kind
   const int k = tid < num_sms ? kPair : tid < 3 * num_sms ? kSingle : kFew;
   const int share = tid - (k == kPair ? 0 : k == kSingle ? num_sms : 3 * num_sms);

@@ -367,11 +367,11 @@ int moe_attn_status(MoeAttn* attn, void* stream);
  *
  * Index arguments (seqs, counts, q_start, ...) are int32 arrays in device memory, so
  * that calls can be captured in a graph; errors in them are found on the device and
- * reported by moe_kv_status.  A call on pages (reserve, fork, truncate) with a sequence
- * outside [0, sequences) or the same sequence twice, or a batch of rows (append, the
- * attention block) with a sequence that has rows in two entries or with offsets that
- * decrease or leave the rows, writes nothing.  An entry of a batch whose sequence is
- * outside is left out, the others are done.  Calls on one
+ * reported by moe_kv_status.  A call on pages (reserve, fork, truncate) changes nothing
+ * when a sequence is outside [0, sequences) or comes twice (parents may).  A batch of rows
+ * (append, attend, the attention block) writes nothing when its offsets decrease or leave
+ * the rows, and the two that write to the cache when a sequence has rows in two entries;
+ * an entry whose sequence is outside is left out, the others are done.  Calls on one
  * cache run in stream order: the ones that change it (and attention while it is being
  * changed) must not overlap on two streams; attention calls may overlap each other. */
 enum { MOE_KV_F16 = 0, MOE_KV_BF16 = 1 };
@@ -435,10 +435,11 @@ int moe_kv_append(MoeKvCache* cache, int32_t layer, const void* k, const void* v
  * to its own position; fp32 softmax and accumulation, probabilities rounded to the cache's
  * dtype for the product with v.  lse (may be NULL): natural logarithm of the sum of the
  * exponentials.  A row that sees no token (more new rows than tokens) gives 0 and -inf.
- * Rows of out and lse before q_start[0] and from q_start[n_seqs] on are left as they were, and
- * those of an entry whose offsets are wrong; the same sequence may come twice.  Nothing that the pool
- * holds past a sequence's length reaches a result, NaN and infinities included; among a
- * sequence's own values they reach every row of the same chunk (weight 0 times infinity). */
+ * Rows of out and lse before q_start[0] and from q_start[n_seqs] on are left as they were.  The
+ * same sequence may come twice.  Nothing that the pool holds past a sequence's length reaches a
+ * result, NaN and infinities included.  A row whose scores hold NaN or infinities gives what the
+ * formula gives; a value of the sequence that is NaN or infinite reaches every row of the same
+ * chunk (weight 0 times infinity). */
 typedef struct MoeKvAttendArgs {
   const void* q;          /* [rows][heads][head_dim], the cache's dtype                */
   void* out;              /* as q                                                      */
@@ -467,7 +468,8 @@ int moe_kv_status(MoeKvCache* cache, void* stream);
  * rows' keys and values are written to layer `layer` of the cache, whose older tokens they
  * attend to.  Reserve first (once for all layers); seqs, q_start, n_seqs as moe_kv_append;
  * the cache is f16 with the plan's kv_heads and head_dim.  Rows of out before q_start[0] and
- * from q_start[n_seqs] on are left as they were; all of them when the offsets are wrong.  Errors of the sequences are reported by moe_kv_status. */
+ * from q_start[n_seqs] on are left as they were, and those of x may hold anything.  Errors of
+ * the sequences are reported by moe_kv_status; a batch that is refused leaves out as it was. */
 uint64_t moe_attn_cached_workspace_bytes(const MoeAttn* attn, const MoeKvCache* cache, int32_t T,
                                          int32_t n_seqs);
 int moe_attn_forward_cached(MoeAttn* attn, MoeKvCache* cache, int32_t layer, const float* x_dev,

@@ -193,3 +193,21 @@ def test_the_block_refuses_a_bad_batch_as_a_whole() -> None:
     good = al.forward_cached(batch, cache, [0, 2], [0, 2, 5])[:2]
     assert _rel(out[:2].cpu().numpy(), good.double().cpu().numpy()) <= TOL_BLOCK
     al.close()
+
+
+def test_attend_refuses_wrong_offsets_as_a_whole() -> None:
+    """Decreasing offsets would give rows to two entries; more entries than the planning CTA
+    has threads, the wrong one among the last or the first."""
+    cache, _o = _filled("f16", 16, 2, 64, [20, 33, 12], seed=4)
+    q = torch.randn((8, 4, 64), device="cuda").half()
+    out, lse = torch.full_like(q, 3.0), torch.full((8, 4), 7.0, device="cuda")
+    many = [[0] * 1500 + [8], [0] * 1499 + [3, 2], [5, 3] + [8] * 1499]
+    batches = [(s, t) for s, t in BAD_BATCHES if len(set(s)) == len(s)] + \
+        [([0, 1, 2] * 500, t) for t in many[1:]]
+    for seqs, starts in batches:
+        cache.attend(q, seqs, starts, out=out, lse=lse)
+        _status_raises_once(cache)
+        assert (out == 3).all() and (lse == 7).all()
+    cache.attend(q, [0, 1, 2] * 500, many[0], out=out, lse=lse)  # the last entry has all rows
+    cache.status()
+    assert (out != 3).any(dim=(1, 2)).all()
