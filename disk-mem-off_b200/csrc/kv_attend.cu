@@ -36,6 +36,7 @@
 // polynomial in place of every eighth to every second exponential: no gain, then a loss).  Short units: instructions
 // that run once a unit, in two warps a scheduler.
 #include <cuda_bf16.h>
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -731,7 +732,11 @@ MOE_DEV uint64_t add_pair(uint64_t a, uint64_t b) {
 
 // A unit cut by the ends of shares leaves a piece in each of its shares: rows
 // unnormalised in fp32 with their maximum (base 2, scaled) and sum, in the share's slot 0
-// (the unit began in an earlier share) or 1 (it goes on in a later one).
+// (the unit began in an earlier share) or 1 (it goes on in a later one).  A maximum of -inf
+// is kept for rows that see no token at all: the merge tells them by it.
+MOE_DEV float2 piece_ml(float top, float sum, bool sees) {
+  return make_float2(sees ? fmaxf(top, -FLT_MAX) : -INFINITY, sum);
+}
 MOE_DEV long long piece_slot(int kind, int share, bool tail, int row) {
   return (2ll * share + (tail ? 1 : 0)) * kind_rows(kind) + row;
 }
@@ -982,8 +987,8 @@ struct KaFew {
 #pragma unroll
         for (int e = 0; e < V; ++e) acc[e] = fmaf(f, src[e], acc[e]);
       }
+      const int h = __shfl_sync(0xffffffffu, hg, pr);
       if (direct) {
-        const int h = __shfl_sync(0xffffffffu, hg, pr);
         write_row<HD, BF16>(a, __shfl_sync(0xffffffffu, tok, pr), head * group + (h < 0 ? ~h : h), acc, top, sum,
                             h >= 0);
       } else {
@@ -991,7 +996,7 @@ struct KaFew {
         float* dst = w.few.o + slot * HD + lane * V;
 #pragma unroll
         for (int e = 0; e < V; ++e) dst[e] = acc[e];
-        if (lane == 0) w.few.ml[slot] = make_float2(top, sum);
+        if (lane == 0) w.few.ml[slot] = piece_ml(top, sum, h >= 0);
       }
     }
     __syncwarp();
@@ -1456,7 +1461,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
                 }
               }
             }
-            if (valid) l_k.ml[slot] = make_float2(m - shift, l);  // no token: -inf, 0
+            if (valid) l_k.ml[slot] = piece_ml(m - shift, l, seen > 0);
           }
         }
         tc_fence_before();  // O is read: the next unit's first product may overwrite it
@@ -1510,7 +1515,6 @@ __global__ void __launch_bounds__(256) kv_merge_kernel(const KvAttend a, const K
     const int kind = e.x, first = e.y, last = e.z;
     const KaList l = w.kind(kind);
     const int4 u0 = *reinterpret_cast<const int4*>(l.list + item);  // seq, row0, r0, rows
-    const int2 u1 = *reinterpret_cast<const int2*>(&l.list[item].base);  // base, len
     float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, acc[2][V] = {};
     for (int base = first; base <= last; base += 32) {
       // shares of the unit that have tiles
@@ -1565,7 +1569,7 @@ __global__ void __launch_bounds__(256) kv_merge_kernel(const KvAttend a, const K
       const int packed = u0.z + r0 + j, tok = packed / group;
       if (r0 + j < u0.w)
         write_row<HD, BF16>(a, static_cast<long long>(u0.y) + tok, e.w * group + packed - tok * group, acc[j], top[j],
-                            sum[j], min(u1.x + tok + 1, u1.y) > 0);
+                            sum[j], top[j] != -INFINITY);
     }
   }
 }
