@@ -396,6 +396,8 @@ __global__ void __launch_bounds__(kPlanThreads) kv_compact_plan_kernel(const KvV
       int hi = holes + static_cast<int>((incl - both) & 0xffffffffu);
       int mv = movers + static_cast<int>((incl - both) >> 32);
       for (uint32_t m = used & low; m; m &= m - 1) c.list[p + __ffs(m) - 1] = p + __ffs(m) - 1;
+      // a page that nobody holds goes nowhere, should a table name it
+      for (uint32_t m = there & ~used; m; m &= m - 1) c.list[p + __ffs(m) - 1] = -1;
       for (uint32_t m = hole; m; m &= m - 1) c.dst[hi++] = p + __ffs(m) - 1;
       for (uint32_t m = move; m; m &= m - 1) c.src[mv++] = p + __ffs(m) - 1;
       holes += static_cast<int>(total & 0xffffffffu);
