@@ -1,5 +1,5 @@
 """Values that attention over the paged cache has to keep apart (needs a B200): what a page
-holds past a sequence's end, NaN and infinities."""
+holds past a sequence's end, NaN and infinities, maxima that grow along the keys."""
 from __future__ import annotations
 
 import numpy as np
@@ -10,6 +10,7 @@ torch = pytest.importorskip("torch")
 pytestmark = [pytest.mark.gpu,
               pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA GPU")]
 
+from moe_sm100.paged import PagedKVCache  # noqa: E402
 from oracle.paged_oracle import attend_chunk  # noqa: E402
 from test_gpu_paged import DTYPES, _attend_case, _check_rows, _filled  # noqa: E402
 
@@ -127,3 +128,63 @@ def test_infinite_scores(work: list, value: float) -> None:
         ref, ref_lse, _ = attend_chunk(clean[a:b], *o.cached(0, i), 0.125)
         got[b - 1, 1:3], lse[b - 1, 1:3] = ref[-1, 1:3], ref_lse[-1, 1:3]
     _check_rows(got, lse, clean, o, list(range(len(work))), starts, 0, 0.125, "bf16")
+
+
+# ------------------------------------------------------------------ growing maxima
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("work", [[(1000, 100), (1300, 300), (300, 300), (1000, 5), (64, 64), (900, 129)],
+                                  [(4000, 100)], [(4000, 300)], [(6000, 3)]],
+                         ids=lambda w: f"{len(w)}x{w[-1][1]}")
+def test_maxima_that_grow_along_the_keys(dtype: str, dim: int, work: list) -> None:
+    """Scores that rise along the keys, by 0 to 20 powers of two every 64 keys, rows of
+    different slopes side by side (in one warp): sums and outputs are rescaled at some tiles
+    and not at others, 7.9 being just too little for one tile and enough for two."""
+    heads, scale = 4, 1 / np.sqrt(dim)
+    cache, o, q, starts = _batch(dtype, heads, 4, dim, 32, work, seed=35)
+    for s, (n, _m) in enumerate(work):
+        pos = torch.arange(n, device="cuda")
+        pages = torch.tensor(o.table[s], device="cuda")[pos // 32]
+        rise = 4.0 * ((pos % 1024) / 64.0)   # keys of f16: the slope begins again every 1024
+        cache.k[0, pages, :, pos % 32, 0] = rise[:, None].to(DTYPES[dtype])
+    o.k[:] = cache.k.double().cpu().numpy()
+    slopes = torch.tensor([0.0, 9.0, 7.9, 20.0, -9.0, 3.0, 12.0], device="cuda")
+    at = torch.arange(q.shape[0], device="cuda")[:, None] + 2 * torch.arange(heads, device="cuda")
+    q[:, :, 0] = (slopes[at % 7] * np.log(2) / (scale * 4.0)).to(q.dtype)
+    got, lse = _attend(cache, q, len(work), starts)
+    _check_rows(got, lse, q.double().cpu().numpy(), o, list(range(len(work))), starts, 0, scale, dtype)
+
+
+# ------------------------------------------------------------------ strided pools
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim", [("f16", 12, 4, 128), ("bf16", 8, 8, 64)])
+def test_strided_pools(dtype: str, heads: int, kv_heads: int, dim: int) -> None:
+    """Keys and values interleaved in one tensor, rows outside heads: attention, copy on
+    write and compaction give what a contiguous pool gives."""
+    lens, page = [300, 41, 17, 700], 32
+    plain, o = _filled(dtype, page, kv_heads, dim, lens, layers=2, layer=1, seed=41, extra=9)
+    pages = plain.k.shape[1]
+    both = torch.zeros((2, pages, page, 2, kv_heads, dim), dtype=DTYPES[dtype], device="cuda")
+    k, v = both[:, :, :, 0].transpose(2, 3), both[:, :, :, 1].transpose(2, 3)
+    k.copy_(plain.k)
+    v.copy_(plain.v)
+    assert not k.is_contiguous()
+    cache = PagedKVCache(k, v, plain.block_table.clone(), plain.lengths.clone(), plain.refs.clone())
+    g = torch.Generator(device="cuda").manual_seed(42)
+    new = [300, 1, 5, 40]
+    starts = [0] + np.cumsum(new).tolist()
+    q = torch.randn((starts[-1], heads, dim), generator=g, device="cuda").to(DTYPES[dtype])
+    outs = [c.attend(q, [0, 1, 2, 3], starts, layer=1) for c in (plain, cache)]
+    assert torch.equal(*outs)
+    _check_rows(outs[1].double().cpu().numpy(), None, q.double().cpu().numpy(), o, [0, 1, 2, 3], starts, 1,
+                1 / np.sqrt(dim), dtype)
+    for c in (plain, cache):
+        c.truncate([0], [0])
+        c.fork([3], [0])
+        c.reserve([0, 3], [1, 2])
+        c.compact()
+        c.status()
+    for name in ("block_table", "lengths", "refs"):
+        assert torch.equal(getattr(plain, name), getattr(cache, name)), name
+    live = plain.refs > 0
+    for a, b in ((plain.k, k), (plain.v, v)):  # bits, NaN past the tokens included
+        assert torch.equal(a[:, live].contiguous().view(torch.int16), b[:, live].contiguous().view(torch.int16))
