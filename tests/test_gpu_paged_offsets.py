@@ -211,3 +211,32 @@ def test_attend_refuses_wrong_offsets_as_a_whole() -> None:
     cache.attend(q, [0, 1, 2] * 500, many[0], out=out, lse=lse)  # the last entry has all rows
     cache.status()
     assert (out != 3).any(dim=(1, 2)).all()
+
+
+def test_the_block_on_more_entries_than_a_cta_checks() -> None:
+    """One token of 600 sequences in one batch and in two; then a batch whose last entry is
+    wrong."""
+    spec = AttnSpec(hidden=512, heads=16, kv_heads=2, head_dim=128, tokens=40, seed=74)
+    x, t = make_attn_case(spec)
+    al = _layer(spec, t, 700)
+    n = 600
+    batch = torch.from_numpy(np.random.default_rng(6).standard_normal((n, spec.hidden)).astype(np.float32)).cuda()
+    outs, caches = [], [_cache(spec, n, 1, 16) for _ in range(2)]
+    for cache, cuts in zip(caches, ([0, n], [0, 300, n])):
+        cache.reserve(list(range(n)), [1] * n)
+        got = []
+        for a, b in zip(cuts, cuts[1:]):
+            got.append(al.forward_cached(batch[a:b], cache, list(range(a, b)), list(range(b - a + 1))))
+        cache.status()
+        outs.append(torch.cat(got))
+    al.status()
+    delta = [(o - batch).double().cpu().numpy() for o in outs]
+    assert _rel(*delta) <= TOL_DELTA
+    before = _bits(caches[0])
+    for seqs, starts in ((list(range(n - 1)) + [5], list(range(n + 1))),
+                         (list(range(n)), list(range(n)) + [n - 2])):
+        out = torch.full_like(batch, 3.0)
+        al.forward_cached(batch, caches[0], seqs, starts, out=out)
+        _status_raises_once(caches[0])
+        assert (out == 3).all() and all(torch.equal(a, b) for a, b in zip(before, _bits(caches[0])))
+    al.close()

@@ -101,3 +101,29 @@ def test_torch_streams_are_told_from_others() -> None:
         number = torch.cuda.current_stream().stream_id
     assert number != 0 and not number & 1
     _lib.check(_lib.lib().moe_rt_stream_destroy(handle))
+
+
+def test_a_cache_over_memory_that_is_not_torchs() -> None:
+    lib = _lib.lib()
+    ptr = c_void_p()
+    shape = (1, 40, 2, 16, 64)
+    _lib.check(lib.moe_rt_malloc(40 * 2 * 16 * 64 * 2, byref(ptr)))
+
+    class Pool:
+        __cuda_array_interface__ = dict(shape=shape, typestr="<f2", data=(ptr.value, False), version=3)
+
+    k = torch.as_tensor(Pool(), device="cuda")
+    assert k.data_ptr() == ptr.value
+    k.zero_()
+    cache = PagedKVCache(k, *_tensors()[1:])
+    side = torch.cuda.Stream()
+    row = torch.ones((3, 2, 64), dtype=torch.float16, device="cuda")
+    torch.cuda.synchronize()
+    cache.reserve([1], [3], stream=side)
+    cache.append(row, row, [1], [0, 3], stream=side)
+    cache.status(stream=side)
+    assert k.sum().item() == 3 * 2 * 64
+    cache.close()
+    del cache, k
+    torch.cuda.synchronize()
+    _lib.check(lib.moe_rt_free(ptr))
