@@ -29,12 +29,18 @@
 // ready.  (Tiles of 128 keys leave no room for a second S buffer; with one, 64-wide heads
 // took 51 us instead of 40.)  Every wait is bounded.
 //
-// What bounds it.  Decode: the reading of K and V (2 x 131071 tokens: 1.07 GB in 186 us,
-// 5.8 TB/s).  Chunks: of the 2,100 cycles that 64 keys of a pair take, the tensor cores
-// have 1,280 and the special-function units 1,024, and the clock falls to about 1.4 GHz
-// under the power limit (4096 new on 4096 cached tokens: 1.25 ms, 0.99 PFLOP/s; a
-// polynomial in place of every eighth to every second exponential: no gain, then a loss).  Short units: instructions
-// that run once a unit, in two warps a scheduler.
+// What bounds it (device time).  Decode: the reading of K and V (2 x 131071 tokens: 1.07 GB
+// in 186 us, 5.8 TB/s).  Chunks: of the 1,940 cycles that 64 keys of a pair take, starts and
+// ends of units included, the tensor cores have 1,280 and the special-function units 1,024,
+// and the clock falls to about 1.4 GHz under the power limit (4096 new on 4096 cached
+// tokens: 1.24 ms, 1.0 PFLOP/s; a polynomial in place of every eighth to every second
+// exponential: no gain, then a loss).  Short units: instructions that run once a unit, in
+// two warps a scheduler.
+//
+// Roundings.  Scores, maxima, sums and O are fp32.  The probabilities are rounded once, to
+// the cache's 16-bit type, since both operands of the product with V have one type: half a
+// step, 2^-11 or 2^-8 relative (the sum takes them unrounded).  The result is rounded to
+// that type once.
 #include <cuda_bf16.h>
 #include <float.h>
 #include <math.h>
@@ -126,7 +132,7 @@ size_t kv_attend_workspace(const KvView& c, int heads, int rows, int n_seqs, int
   return ka_ws(c, heads, rows, n_seqs, num_sms).total;
 }
 
-// The workspace by kind (0 pairs, 1 singles), for the kernels.
+// The workspace by kind (kPair, kSingle, kFew), for the kernels.
 struct KaList {
   KaStart* start;
   KaUnit* list;
@@ -1028,8 +1034,8 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(sR + C::kStages * C::kStage);
   uint64_t* full = bars;                       // [kStages]
   uint64_t* empty = full + C::kStages;         // [kStages]
-  uint64_t* half_full = empty + C::kStages;     // [2][kFewStages] the few-row units' rings
-  uint64_t* half_empty = half_full + C::kStages;  // [2][kFewStages]
+  uint64_t* half_full = empty + C::kStages;     // [2][kHalf] the rings of singles and few rows
+  uint64_t* half_empty = half_full + C::kStages;  // [2][kHalf]
   uint64_t* s_full = half_empty + C::kStages;   // [stream][buffer] S of a tile done
   uint64_t* p_full = s_full + 4;               // [stream][buffer] P of a tile written
   uint64_t* o_done = s_full + 8;               // [stream][buffer] P V of a tile done

@@ -22,7 +22,7 @@ struct KvView {
   int nseq, max_blocks;
   int* len;    // [nseq]
   int* refs;   // [pages]
-  // scratch (see KvScratch)
+  // scratch (kv_scratch_words)
   int* err;
   int* count;  // pages to copy, written by the kernel that plans a copy
   int* ok;     // a batch may be written (kv_check_kernel)

@@ -10,8 +10,10 @@
 //
 // A call checks its sequence indices (range, the same one twice) before it changes
 // anything and refuses as a whole; an entry whose own state forbids the step (a
-// child that is not empty, a longer new length) is left as it was.  Both are
-// reported by moe_kv_status.
+// child that is not empty, a longer new length) is left as it was.  A batch of rows is
+// refused as a whole for its offsets and for a sequence with rows in two entries; an entry
+// without a sequence and a row without a place are left out.  All are reported by
+// moe_kv_status.
 #include <algorithm>
 #include <new>
 #include <string>
@@ -819,10 +821,12 @@ int moe_kv_status(MoeKvCache* cache, void* stream) {
   switch (code) {
     case DEV_OK: return MOE_OK;
     case DEV_BAD_SEQ:
-      return kfail(MOE_ERR_INVALID, "a sequence index is out of range, or the same sequence came twice");
+      return kfail(MOE_ERR_INVALID, "a sequence index is out of range, or the same sequence came twice "
+                                    "where it is written");
     case DEV_BAD_LENGTH:
       return kfail(MOE_ERR_INVALID, "a length does not fit: a child that is not empty, a longer new length, "
-                                    "more tokens than the block table holds, or more new rows than tokens");
+                                    "more tokens than the block table holds, more new rows than tokens, or "
+                                    "offsets of rows that decrease or leave the rows");
     case DEV_BAD_PAGE:
       return kfail(MOE_ERR_INVALID, "a page is out of range or missing from the block table, or a copied "
                                     "page came twice");

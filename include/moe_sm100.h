@@ -371,9 +371,10 @@ int moe_attn_status(MoeAttn* attn, void* stream);
  * when a sequence is outside [0, sequences) or comes twice (parents may).  A batch of rows
  * (append, attend, the attention block) writes nothing when its offsets decrease or leave
  * the rows, and the two that write to the cache when a sequence has rows in two entries;
- * an entry whose sequence is outside is left out, the others are done.  Calls on one
- * cache run in stream order: the ones that change it (and attention while it is being
- * changed) must not overlap on two streams; attention calls may overlap each other. */
+ * an entry whose sequence is outside is left out (attend gives zeros, the block x), the
+ * others are done.  Calls on one cache run in stream order: the ones that change it (and
+ * attention while it is being changed) must not overlap on two streams; attention calls
+ * may overlap each other. */
 enum { MOE_KV_F16 = 0, MOE_KV_BF16 = 1 };
 
 typedef struct MoeKvConfig {
@@ -420,7 +421,8 @@ int moe_kv_copy_pages(MoeKvCache* cache, const int32_t* src, const int32_t* dst,
                       void* stream);
 /* into NULL: the live pages move to the lowest page numbers (those already there stay).
  * Otherwise they are copied, dense and in order, into another cache of the same device,
- * dtype and page shape, whose tables are overwritten; MOE_ERR_NO_PAGES if they do not fit. */
+ * dtype and page shape, whose tables are overwritten and whose memory lies apart from this
+ * one's; MOE_ERR_NO_PAGES if they do not fit.  A page without references goes nowhere. */
 int moe_kv_compact(MoeKvCache* cache, MoeKvCache* into, void* stream);
 /* New rows of a batch: entry i owns rows q_start[i] .. q_start[i+1]-1 (q_start: n_seqs + 1
  * non-decreasing offsets), the last tokens of sequence seqs[i]: row r is its token
